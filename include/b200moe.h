@@ -264,6 +264,47 @@ int b200moe_ep_gather(const void* x, const int* ids, const float* wts, const int
                       int experts_per_rank, int max_rows, void* sx, int* meta, void* stream);
 int b200moe_ep_combine_rows(const void* back, const int* pos, int m, int h, int world, void* out, void* stream);
 
+/* ---- the router from logits, its load-balance loss, with gradients (the reference's ids and weights come from torch's softmax and
+ * top-k: sm120fp4/kernels/moe_layer.py:195-200). dtype 0 = bf16, 1 = f32, 2 = f16; logits [tokens, E] with rows `stride` elements apart; E <= 512
+ * (B200MOE_ERR_LIMIT beyond).
+ * gate: ids i32 [tokens, k] = the k largest logits in falling order, ties to the lowest index; weights f32 [tokens, k] = their softmax over all E,
+ * divided by their sum where renormalize; k <= 16. A logit of -inf may not be taken: where none else is left, id -1 and weight 0. NaN ranks above all and
+ * makes its token's weights NaN. gate_backward: grad_logits [tokens, E] (type of logits, contiguous) from grad_weights f32 [tokens, k], and the weights and
+ * ids of the call; logits are read (and may be null otherwise) where renormalize is 0. */
+int b200moe_gate(const void* logits, int dtype, long long stride, int tokens, int E, int k, int renormalize, float* weights, int* ids, void* stream);
+int b200moe_gate_backward(const float* grad_weights, const float* weights, const int* ids, const void* logits, int dtype, long long stride, int tokens, int E,
+                          int k, int renormalize, void* grad_logits, void* stream);
+/* balance_loss: loss f32 [1] = E * sum_e (counts_e / sum counts) * (mean over live tokens of softmax(logits)_e), counts i32 [E] = pairs of each expert in
+ * ids i32 [tokens, k], k <= 32. An id outside 0..E-1 is an empty slot; a token of empty slots alone is not live: it counts nowhere and its gradient is 0. No
+ * live token: loss 0. stats f32 [2] is kept for the backward pass (1 / pairs, E / live tokens). The workspace holds nothing between calls. */
+long long b200moe_balance_workspace_bytes(int tokens, int E);
+int b200moe_balance_loss(const void* logits, int dtype, long long stride, int tokens, int E, const int* ids, int k, float* loss, int* counts, float* stats,
+                         void* workspace, long long workspace_bytes, void* stream);
+int b200moe_balance_backward(const float* grad_loss, const void* logits, int dtype, long long stride, int tokens, int E, const int* ids, int k, const int* counts,
+                             const float* stats, void* grad_logits, void* stream);
+
+/* ---- FP8 (E4M3) with fp32 scales per 128 values, for the matrices of a model that are not NVFP4 (no counterpart in the reference).
+ * scale = fl(max(max|x|, 1e-12) / 448), code = e4m3(fl(x * fl(448 / max))), to nearest, ties to even; a value stands for code * scale.
+ * quantize_fp8: x [x_rows, K] (dtype as above, rows x_stride elements apart) -> codes u8 [rows, K] with rows codes_stride bytes apart, scales f32 [rows,
+ * ceil(K/128)]: one per 128 values of a row. Row r is source row src_row[r] (null: r, and rows == x_rows); one outside 0..x_rows-1 gives zero codes and scales.
+ * quantize_fp8_blocks: w [E, N, K] contiguous -> codes u8 [E, N, K] (rows codes_stride bytes apart), scales f32 [E, ceil(N/128), ceil(K/128)]: one per 128x128. */
+int b200moe_quantize_fp8(const void* x, int dtype, long long x_stride, int x_rows, const int* src_row, int rows, int K, void* codes, long long codes_stride,
+                         float* scales, void* stream);
+int b200moe_quantize_fp8_blocks(const void* w, int dtype, int E, int N, int K, void* codes, long long codes_stride, float* scales, void* stream);
+/* matmul_fp8: out [M, N] (out_dtype as above, rows out_stride elements apart) = a x w^T of such codes: a u8 [M, K] with a_scales f32 [M, ceil(K/128)], w u8
+ * [N, K] with w_scales f32 [ceil(N/128), ceil(K/128)]. Codes start on 16 bytes and their row strides (bytes) are multiples of 16; M, N, K are any sizes.
+ * matmul_fp8_experts: rows offsets[u] .. offsets[u+1] - 1 of a times w[experts[u]]^T, u < runs <= 1024; w u8 [E, N, K] with rows w_stride bytes apart,
+ * w_scales f32 [E, ceil(N/128), ceil(K/128)]; experts and offsets are the tables of b200moe_route (the pairs' rows laid out by b200moe_quantize_fp8 with src_row).
+ * Rows outside every run, and those of an expert outside 0..E-1, are left as they were, or written 0 where zero_rest.
+ * Sums over a group are the tensor core's (exact products, fp32 accumulator), sums over groups fp32; results are the same bits from call to call.
+ * status: B200MOE_ERR_TIMEOUT if a bounded device-side wait of such a call ran out on the current device since the last read; synchronises. */
+int b200moe_matmul_fp8(const void* a, long long a_stride, const float* a_scales, const void* w, long long w_stride, const float* w_scales, int M, int N, int K,
+                       void* out, int out_dtype, long long out_stride, void* stream);
+int b200moe_matmul_fp8_experts(const void* a, long long a_stride, const float* a_scales, int rows, const void* w, long long w_stride, const float* w_scales, int E,
+                               const int* experts, const int* offsets, int runs, int N, int K, void* out, int out_dtype, long long out_stride, int zero_rest,
+                               void* stream);
+int b200moe_matmul_fp8_status(void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -8,3 +8,5 @@ __version__ = "0.1.0"
 from .layouts import from_128x4, padded_sf_shape, to_128x4  # noqa: E402,F401
 from .quant import global_scale_for, quantize_nvfp4, quantize_nvfp4_128x4, quantize_nvfp4_experts  # noqa: E402,F401
 from .router import route, route_tables  # noqa: E402,F401
+from .gate import balance_loss, top_k_gate  # noqa: E402,F401
+from .fp8 import matmul_fp8, matmul_fp8_experts, matmul_fp8_status, quantize_fp8, quantize_fp8_weight  # noqa: E402,F401

@@ -79,6 +79,16 @@ SIGNATURES = {
     "b200moe_ep_combine_rows": (_I, [_P, _P, _I, _I, _I, _P, _P]),
     "b200moe_umma_probe": (_I, [_P, _P, _P, _P, _I, _I, _P, _I, _P, _P]),
     "b200moe_umma_pair_probe": (_I, [_P, _P, _P, _P, _I, _P, _P, _P]),
+    "b200moe_gate": (_I, [_P, _I, _LL, _I, _I, _I, _I, _P, _P, _P]),
+    "b200moe_gate_backward": (_I, [_P, _P, _P, _P, _I, _LL, _I, _I, _I, _I, _P, _P]),
+    "b200moe_balance_workspace_bytes": (_LL, [_I, _I]),
+    "b200moe_balance_loss": (_I, [_P, _I, _LL, _I, _I, _P, _I, _P, _P, _P, _P, _LL, _P]),
+    "b200moe_balance_backward": (_I, [_P, _P, _I, _LL, _I, _I, _P, _I, _P, _P, _P, _P]),
+    "b200moe_quantize_fp8": (_I, [_P, _I, _LL, _I, _P, _I, _I, _P, _LL, _P, _P]),
+    "b200moe_quantize_fp8_blocks": (_I, [_P, _I, _I, _I, _I, _P, _LL, _P, _P]),
+    "b200moe_matmul_fp8": (_I, [_P, _LL, _P, _P, _LL, _P, _I, _I, _I, _P, _I, _LL, _P]),
+    "b200moe_matmul_fp8_experts": (_I, [_P, _LL, _P, _I, _P, _LL, _P, _I, _P, _P, _I, _I, _I, _P, _I, _LL, _I, _P]),
+    "b200moe_matmul_fp8_status": (_I, [_P]),
 }
 # exported only by a diagnostic build (include/b200moe_diag.h); bound when present
 DIAG_SIGNATURES = {
@@ -143,6 +153,32 @@ def check(code: int, what: str = "") -> None:
     if code == ERR_CUDA:
         msg += f": {h.b200moe_last_cuda_error().decode()}"
     raise B200MoEError(code, f"{what or 'b200moe'}: {msg} ({code})")
+
+
+DTYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}   # dtype codes of the C ABI
+
+
+def one_device(what: str, *tensors) -> torch.device:
+    """The device that all of them are on: a GPU."""
+    device = tensors[0].device
+    for t in tensors:
+        if not t.is_cuda:
+            raise RuntimeError(f"{what} runs on the GPU; there is no CPU path in this package")
+        if t.device != device:
+            raise RuntimeError(f"{what}: tensors on {device} and {t.device}")
+    return device
+
+
+def call(device: torch.device, what: str, fn, *args) -> None:
+    """fn(*args, stream) on the current stream of `device`."""
+    here = torch._C._cuda_getDevice()
+    if device.index != here:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    else:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(here))
+    if rc:
+        check(rc, what)
 
 
 def ptr(t) -> int:

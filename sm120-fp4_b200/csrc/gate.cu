@@ -1,0 +1,427 @@
+// Router from logits and its load-balance loss, with gradients.
+//   gate     ids = the k largest logits of a token (ties: the lowest index), w_j = softmax(l)[id_j], divided by their sum if asked
+//            dl = w_j (g_j - sum g w) at id_j (normalised), or p_e (g_e - sum g w) for all experts
+//   balance  L = E sum_e f_e P_e, f_e = n_e / sum n, P_e = mean over live tokens of softmax(l)_e
+//            dl = g E / T' p_e (f_e - sum_j p_j f_j)
+// A warp per token with its logits in registers; sums in fp32, statistics by shuffles, no atomic decides a value. A logit of -inf is an
+// expert that may not be taken: a slot for which none is left gets id -1 (an empty slot of the layer) and weight 0.
+#include "common.cuh"
+#include "fp8_math.cuh"
+#include <type_traits>
+
+namespace b200 {
+
+constexpr int GATE_MAXE = 512, GATE_MAXK = 16;
+
+// Lane l holds the logits of experts l*V .. l*V + V - 1; pad for those beyond E.
+template <typename T, int V, bool kVec>
+__device__ __forceinline__ void load_row(const T* __restrict__ row, int E, int lane, float (&x)[V], float pad) {
+  if constexpr (kVec && V * Elem<T>::kSize >= 16) {
+    constexpr int P = 16 / Elem<T>::kSize;
+#pragma unroll
+    for (int i = 0; i < V / P; ++i) {
+      const int e = lane * V + i * P;
+      float v[P];
+      if (e < E) unpack16<T>(__ldg(reinterpret_cast<const uint4*>(row + e)), v);      // (E is a multiple of P)
+#pragma unroll
+      for (int j = 0; j < P; ++j) x[i * P + j] = e < E ? v[j] : pad;
+    }
+  } else if constexpr (kVec && V == 4) {      // 16 bits
+    const int e = lane * V;
+    uint2 w = make_uint2(0u, 0u);
+    if (e < E) w = __ldg(reinterpret_cast<const uint2*>(row + e));
+    Elem<T>::unpack(w.x, x[0], x[1]), Elem<T>::unpack(w.y, x[2], x[3]);
+    if (e >= E) x[0] = x[1] = x[2] = x[3] = pad;
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) x[j] = lane * V + j < E ? Elem<T>::load(row + lane * V + j) : pad;
+  }
+}
+template <typename T, int V, bool kVec>
+__device__ __forceinline__ void store_row(T* __restrict__ row, int E, int lane, const float (&x)[V]) {
+  if constexpr (kVec && V * Elem<T>::kSize >= 16) {
+    constexpr int P = 16 / Elem<T>::kSize;
+#pragma unroll
+    for (int i = 0; i < V / P; ++i) {
+      const int e = lane * V + i * P;
+      uint4 w;
+      if constexpr (P == 8) w = make_uint4(Elem<T>::pack(x[8 * i], x[8 * i + 1]), Elem<T>::pack(x[8 * i + 2], x[8 * i + 3]), Elem<T>::pack(x[8 * i + 4], x[8 * i + 5]), Elem<T>::pack(x[8 * i + 6], x[8 * i + 7]));
+      else w = make_uint4(__float_as_uint(x[4 * i]), __float_as_uint(x[4 * i + 1]), __float_as_uint(x[4 * i + 2]), __float_as_uint(x[4 * i + 3]));
+      if (e < E) *reinterpret_cast<uint4*>(row + e) = w;
+    }
+  } else if constexpr (kVec && V == 4) {
+    if (lane * V < E) *reinterpret_cast<uint2*>(row + lane * V) = make_uint2(Elem<T>::pack(x[0], x[1]), Elem<T>::pack(x[2], x[3]));
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (lane * V + j < E) row[lane * V + j] = Elem<T>::make(x[j]);
+  }
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+// Softmax numerators against the row's maximum and their sum. Rows of -inf alone: zeros, sum 0. An infinity or a NaN makes the row NaN.
+template <int V>
+__device__ __forceinline__ float softmax_terms(const float (&x)[V], float (&p)[V]) {
+  float m = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < V; ++j) m = max_nan(m, x[j]);
+  m = warp_max(m);
+  if (m == -INFINITY) m = 0.f;
+  float s = 0.f;
+#pragma unroll
+  for (int j = 0; j < V; ++j) p[j] = expf(x[j] - m), s += p[j];
+  return warp_sum(s);
+}
+
+// An unsigned number in the order of the logits: NaN above all, -0 = +0. 0 is left for experts that are not there.
+__device__ __forceinline__ uint32_t order_key(float v) {
+  if (v != v) return 0xffffffffu;
+  const uint32_t u = __float_as_uint(v + 0.f);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+  if (k == 0xffffffffu) return NAN;
+  return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+}
+constexpr uint32_t kKeyMasked = 0x007fffffu;      // order_key(-inf)
+
+template <typename T, int V, bool kVec>
+__global__ void __launch_bounds__(256) k_gate(const T* __restrict__ logits, long long stride, int tokens, int E, int k, int renorm, float* __restrict__ weights,
+                                              int* __restrict__ ids) {
+  const int lane = threadIdx.x & 31;
+  grid_dependency_wait();
+  const int t = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (t >= tokens) return;
+  float x[V];
+  load_row<T, V, kVec>(logits + (long long)t * stride, E, lane, x, -INFINITY);
+  uint32_t key[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) key[j] = lane * V + j < E ? order_key(x[j]) : 0u;
+  uint32_t mine = 0u;      // lane j: key and index of the j-th largest
+  int at = -1;
+  for (int j = 0; j < k; ++j) {
+    uint32_t best = 0u;
+    int bi = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (key[i] > best) best = key[i], bi = i;
+    const uint32_t top = __reduce_max_sync(0xffffffffu, best);
+    const int src = __ffs(__ballot_sync(0xffffffffu, best == top)) - 1;
+    const int e = __shfl_sync(0xffffffffu, lane * V + bi, src);
+    if (lane == j) mine = top, at = e;
+    if (lane == src) {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (i == bi) key[i] = 0u;
+    }
+  }
+  const bool live = lane < k && mine > kKeyMasked;
+  const uint32_t first = __shfl_sync(0xffffffffu, mine, 0);
+  const float m = first <= kKeyMasked ? 0.f : key_value(first);
+  float w = live ? expf(key_value(mine) - m) : 0.f, s;
+  if (renorm) {
+    s = warp_sum(w);
+  } else {
+    s = 0.f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) s += expf(x[j] - m);
+    s = warp_sum(s);
+  }
+  if (lane < k) {
+    weights[(long long)t * k + lane] = live ? w / s : 0.f;
+    ids[(long long)t * k + lane] = live ? at : -1;
+  }
+}
+
+template <typename T, int V, bool kVec>
+__global__ void __launch_bounds__(256) k_gate_backward(const float* __restrict__ grad, const float* __restrict__ weights, const int* __restrict__ ids,
+                                                       const T* __restrict__ logits, long long stride, int tokens, int E, int k, int renorm, T* __restrict__ out) {
+  const int lane = threadIdx.x & 31;
+  grid_dependency_wait();
+  const int t = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (t >= tokens) return;
+  int e = -1;
+  float g = 0.f, w = 0.f;
+  if (lane < k) {
+    e = ids[(long long)t * k + lane];
+    if (e >= E) e = -1;
+    if (e >= 0) g = grad[(long long)t * k + lane], w = weights[(long long)t * k + lane];
+  }
+  const float dot = warp_sum(g * w);
+  float d[V];
+  if (renorm) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) d[j] = 0.f;
+  } else {
+    float x[V];
+    load_row<T, V, kVec>(logits + (long long)t * stride, E, lane, x, -INFINITY);
+    const float s = softmax_terms<V>(x, d);
+    const float c = s == 0.f ? 0.f : -dot / s;
+#pragma unroll
+    for (int j = 0; j < V; ++j) d[j] *= c;
+  }
+  T* row = out + (long long)t * E;
+  store_row<T, V, kVec>(row, E, lane, d);
+  __syncwarp();      // orders the row's stores ahead of the chosen experts'
+  if (e >= 0) row[e] = Elem<T>::make(w * (g - dot));
+}
+
+// ---------------------------------------------------------------------------------------------------- balance loss
+// Each block sums its tokens' probabilities per expert (fp32, a warp's tokens in order, then the warps in order) and counts its pairs; a second
+// launch adds the blocks in order. part: per block E floats, E ints, live tokens.
+__host__ __device__ inline int balance_words(int E) { return 2 * E + 4; }
+
+template <typename T, int V, bool kVec>
+__global__ void __launch_bounds__(256) k_balance_part(const T* __restrict__ logits, long long stride, int tokens, int E, const int* __restrict__ ids, int k,
+                                                      float* __restrict__ part) {
+  __shared__ float sp[8][GATE_MAXE];
+  __shared__ int cnt[GATE_MAXE], live_n;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int i = threadIdx.x; i < GATE_MAXE; i += 256) cnt[i] = 0;
+  if (threadIdx.x == 0) live_n = 0;
+  __syncthreads();
+  grid_dependency_wait();
+  float acc[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) acc[j] = 0.f;
+  int n = 0;
+  for (int t = blockIdx.x * 8 + warp; t < tokens; t += gridDim.x * 8) {
+    const int e = lane < k ? ids[(long long)t * k + lane] : -1;
+    const bool used = e >= 0 && e < E;
+    if (used) atomicAdd(&cnt[e], 1);
+    if (!__any_sync(0xffffffffu, used)) continue;      // an empty token
+    ++n;
+    float x[V], p[V];
+    load_row<T, V, kVec>(logits + (long long)t * stride, E, lane, x, -INFINITY);
+    const float s = softmax_terms<V>(x, p);
+    const float r = s == 0.f ? 0.f : 1.f / s;
+#pragma unroll
+    for (int j = 0; j < V; ++j) acc[j] = fmaf(p[j], r, acc[j]);
+  }
+  if (lane == 0 && n) atomicAdd(&live_n, n);
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+    if (lane * V + j < GATE_MAXE) sp[warp][lane * V + j] = acc[j];
+  __syncthreads();
+  float* o = part + (long long)blockIdx.x * balance_words(E);
+  for (int e = threadIdx.x; e < E; e += 256) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += sp[i][e];
+    o[e] = s;
+    reinterpret_cast<int*>(o)[E + e] = cnt[e];
+  }
+  if (threadIdx.x == 0) reinterpret_cast<int*>(o)[2 * E] = live_n;
+}
+
+// stats: f32 [2]: 1 / pairs, E / live tokens (0 without any)
+__global__ void __launch_bounds__(GATE_MAXE) k_balance_sum(const float* __restrict__ part, int blocks, int E, float* __restrict__ loss, int* __restrict__ counts, float* __restrict__ stats) {
+  __shared__ double red[GATE_MAXE / 32];
+  __shared__ long long reds[GATE_MAXE / 32];
+  __shared__ int live_s;
+  const int e = threadIdx.x, W = balance_words(E);
+  grid_dependency_wait();
+  double p = 0.0;
+  int c = 0;
+  if (e < E) {
+    for (int b0 = 0; b0 < blocks; b0 += 8) {
+      float pv[8];
+      int cv[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const bool in = b0 + i < blocks;
+        pv[i] = in ? part[(long long)(b0 + i) * W + e] : 0.f;
+        cv[i] = in ? reinterpret_cast<const int*>(part)[(long long)(b0 + i) * W + E + e] : 0;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) p += (double)pv[i], c += cv[i];
+    }
+    counts[e] = c;
+  }
+  if (e < 32) {
+    int l = 0;
+    for (int b = e; b < blocks; b += 32) l += reinterpret_cast<const int*>(part)[(long long)b * W + 2 * E];
+    l = __reduce_add_sync(0xffffffffu, l);
+    if (e == 0) live_s = l;
+  }
+  double v = p * (double)c;
+  long long n = c;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o), n += __shfl_xor_sync(0xffffffffu, n, o);
+  if ((e & 31) == 0) red[e >> 5] = v, reds[e >> 5] = n;
+  __syncthreads();
+  if (e == 0) {
+    v = 0.0, n = 0;
+    for (int i = 0; i < (int)(blockDim.x >> 5); ++i) v += red[i], n += reds[i];
+    const double live = live_s ? (double)live_s : 1.0, pairs = n ? (double)n : 1.0;
+    *loss = (float)((double)E * v / (live * pairs));
+    stats[0] = (float)(1.0 / pairs), stats[1] = (float)((double)E / live);
+  }
+}
+
+template <typename T, int V, bool kVec>
+__global__ void __launch_bounds__(256) k_balance_backward(const float* __restrict__ grad, const T* __restrict__ logits, long long stride, int tokens, int E,
+                                                          const int* __restrict__ ids, int k, const int* __restrict__ counts, const float* __restrict__ stats,
+                                                          T* __restrict__ out) {
+  const int lane = threadIdx.x & 31;
+  grid_dependency_wait();
+  const float inv = stats[0], c = *grad * stats[1];
+  float f[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) f[j] = lane * V + j < E ? (float)counts[lane * V + j] * inv : 0.f;
+  for (int t = blockIdx.x * 8 + (threadIdx.x >> 5); t < tokens; t += gridDim.x * 8) {
+    const int e = lane < k ? ids[(long long)t * k + lane] : -1;
+    float d[V];
+    if (__any_sync(0xffffffffu, e >= 0 && e < E)) {
+      float x[V];
+      load_row<T, V, kVec>(logits + (long long)t * stride, E, lane, x, -INFINITY);
+      const float s = softmax_terms<V>(x, d);
+      const float r = s == 0.f ? 0.f : 1.f / s;
+      float dot = 0.f;
+#pragma unroll
+      for (int j = 0; j < V; ++j) d[j] *= r, dot = fmaf(d[j], f[j], dot);
+      dot = warp_sum(dot);
+#pragma unroll
+      for (int j = 0; j < V; ++j) d[j] *= (f[j] - dot) * c;
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) d[j] = 0.f;
+    }
+    store_row<T, V, kVec>(out + (long long)t * E, E, lane, d);
+  }
+}
+
+// Calls `f` with the kernel's type, values per lane and whether rows are taken 8 or 16 bytes at a time.
+template <typename F> static int with_type(int dtype, F&& f) {
+  if (dtype == DT_BF16) return f((__nv_bfloat16*)nullptr);
+  if (dtype == DT_F16) return f((__half*)nullptr);
+  return f((float*)nullptr);
+}
+template <typename F> static int with_values(int E, F&& f) {
+  if (E <= 32) return f(std::integral_constant<int, 1>());
+  if (E <= 64) return f(std::integral_constant<int, 2>());
+  if (E <= 128) return f(std::integral_constant<int, 4>());
+  if (E <= 256) return f(std::integral_constant<int, 8>());
+  return f(std::integral_constant<int, 16>());
+}
+static bool vec_rows(const void* p, long long stride, int E, int size) {      // every row and every lane's run on 16 bytes (8 for four 16-bit values)
+  const int unit = E <= 128 && size == 2 ? 8 : 16;
+  return ((uintptr_t)p % unit) == 0 && (stride * size) % unit == 0 && ((long long)E * size) % unit == 0;
+}
+static int balance_blocks(int tokens) {
+  const int want = (tokens + 7) / 8;
+  return want < 592 ? want : 592;
+}
+
+}  // namespace b200
+
+extern "C" {
+
+static int gate_args(int dtype, long long stride, int tokens, int E, int k) {
+  if (dtype < 0 || dtype > 2 || tokens < 0 || E < 1 || k < 1 || k > E || (stride < E && tokens > 1)) return B200MOE_ERR_ARG;
+  if (E > b200::GATE_MAXE || k > b200::GATE_MAXK) return B200MOE_ERR_LIMIT;
+  return B200MOE_OK;
+}
+
+int b200moe_gate(const void* logits, int dtype, long long stride, int tokens, int E, int k, int renormalize, float* weights, int* ids, void* stream) {
+  using namespace b200;
+  if (int rc = gate_args(dtype, stride, tokens, E, k)) return rc;
+  if (tokens == 0) return B200MOE_OK;
+  if (!logits || !weights || !ids || ((uintptr_t)logits & (dtype == DT_F32 ? 3 : 1))) return B200MOE_ERR_ARG;
+  return with_type(dtype, [&](auto* tp) {
+    using T = std::remove_pointer_t<decltype(tp)>;
+    return with_values(E, [&](auto v) {
+      constexpr int V = decltype(v)::value;
+      const T* lp = (const T*)logits;
+      void* args[] = {&lp, &stride, &tokens, &E, &k, &renormalize, &weights, &ids};
+      const void* fn = vec_rows(logits, stride, E, sizeof(T)) ? (const void*)k_gate<T, V, true> : (const void*)k_gate<T, V, false>;
+      return launch_kernel(fn, (tokens + 7) / 8, 256, 0, true, args, (cudaStream_t)stream);
+    });
+  });
+}
+
+int b200moe_gate_backward(const float* grad_weights, const float* weights, const int* ids, const void* logits, int dtype, long long stride, int tokens, int E, int k,
+                          int renormalize, void* grad_logits, void* stream) {
+  using namespace b200;
+  if (int rc = gate_args(dtype, stride, tokens, E, k)) return rc;
+  if (tokens == 0) return B200MOE_OK;
+  if (!grad_weights || !weights || !ids || !grad_logits || (!renormalize && !logits) || (((uintptr_t)logits | (uintptr_t)grad_logits) & (dtype == DT_F32 ? 3 : 1)))
+    return B200MOE_ERR_ARG;
+  return with_type(dtype, [&](auto* tp) {
+    using T = std::remove_pointer_t<decltype(tp)>;
+    return with_values(E, [&](auto v) {
+      constexpr int V = decltype(v)::value;
+      const T* lp = (const T*)logits;
+      T* op = (T*)grad_logits;
+      void* args[] = {&grad_weights, &weights, &ids, &lp, &stride, &tokens, &E, &k, &renormalize, &op};
+      const bool vec = (renormalize || vec_rows(logits, stride, E, sizeof(T))) && vec_rows(grad_logits, E, E, sizeof(T));
+      const void* fn = vec ? (const void*)k_gate_backward<T, V, true> : (const void*)k_gate_backward<T, V, false>;
+      return launch_kernel(fn, (tokens + 7) / 8, 256, 0, true, args, (cudaStream_t)stream);
+    });
+  });
+}
+
+long long b200moe_balance_workspace_bytes(int tokens, int E) {
+  if (tokens < 0 || E < 1) return B200MOE_ERR_ARG;
+  if (E > b200::GATE_MAXE) return B200MOE_ERR_LIMIT;
+  return 4ll * b200::balance_words(E) * b200::balance_blocks(tokens);
+}
+
+int b200moe_balance_loss(const void* logits, int dtype, long long stride, int tokens, int E, const int* ids, int k, float* loss, int* counts, float* stats,
+                         void* workspace, long long workspace_bytes, void* stream) {
+  using namespace b200;
+  if (dtype < 0 || dtype > 2 || tokens < 0 || E < 1 || k < 1 || (stride < E && tokens > 1)) return B200MOE_ERR_ARG;
+  if (E > GATE_MAXE || k > 32) return B200MOE_ERR_LIMIT;
+  if (!loss || !counts || !stats || (tokens && (!logits || !ids || !workspace)) || ((uintptr_t)logits & (dtype == DT_F32 ? 3 : 1)) || ((uintptr_t)workspace & 3)) return B200MOE_ERR_ARG;
+  if (workspace_bytes < b200moe_balance_workspace_bytes(tokens, E)) return B200MOE_ERR_WORKSPACE;
+  int blocks = balance_blocks(tokens);
+  float* part = (float*)workspace;
+  const int rc = tokens == 0 ? B200MOE_OK : with_type(dtype, [&](auto* tp) {
+    using T = std::remove_pointer_t<decltype(tp)>;
+    return with_values(E, [&](auto v) {
+      constexpr int V = decltype(v)::value;
+      const T* lp = (const T*)logits;
+      void* args[] = {&lp, &stride, &tokens, &E, &ids, &k, &part};
+      const void* fn = vec_rows(logits, stride, E, sizeof(T)) ? (const void*)k_balance_part<T, V, true> : (const void*)k_balance_part<T, V, false>;
+      return launch_kernel(fn, blocks, 256, 0, true, args, (cudaStream_t)stream);
+    });
+  });
+  if (rc) return rc;
+  const float* cp = part;
+  void* args[] = {&cp, &blocks, &E, &loss, &counts, &stats};
+  return launch_kernel((const void*)k_balance_sum, 1, (E + 31) & ~31, 0, true, args, (cudaStream_t)stream);
+}
+
+int b200moe_balance_backward(const float* grad_loss, const void* logits, int dtype, long long stride, int tokens, int E, const int* ids, int k, const int* counts,
+                             const float* stats, void* grad_logits, void* stream) {
+  using namespace b200;
+  if (dtype < 0 || dtype > 2 || tokens < 0 || E < 1 || k < 1 || (stride < E && tokens > 1)) return B200MOE_ERR_ARG;
+  if (E > GATE_MAXE || k > 32) return B200MOE_ERR_LIMIT;
+  if (tokens == 0) return B200MOE_OK;
+  if (!grad_loss || !logits || !ids || !counts || !stats || !grad_logits || (((uintptr_t)logits | (uintptr_t)grad_logits) & (dtype == DT_F32 ? 3 : 1))) return B200MOE_ERR_ARG;
+  return with_type(dtype, [&](auto* tp) {
+    using T = std::remove_pointer_t<decltype(tp)>;
+    return with_values(E, [&](auto v) {
+      constexpr int V = decltype(v)::value;
+      const T* lp = (const T*)logits;
+      T* op = (T*)grad_logits;
+      void* args[] = {&grad_loss, &lp, &stride, &tokens, &E, &ids, &k, &counts, &stats, &op};
+      const bool vec = vec_rows(logits, stride, E, sizeof(T)) && vec_rows(grad_logits, E, E, sizeof(T));
+      const void* fn = vec ? (const void*)k_balance_backward<T, V, true> : (const void*)k_balance_backward<T, V, false>;
+      const int want = (tokens + 7) / 8;
+      return launch_kernel(fn, want < 1184 ? want : 1184, 256, 0, true, args, (cudaStream_t)stream);
+    });
+  });
+}
+
+}  // extern "C"

@@ -1,0 +1,209 @@
+// FP8 quantiser: E4M3 codes with one fp32 scale per 1x128 values of a row (activations) or per 128x128 block (weights).
+//   scale = fl(amax / 448), factor = fl(448 / amax), amax = max(max|x|, 1e-12); code = e4m3(fl(x * factor))
+// One pass over the data: a group's values stay in registers between its maximum and its codes. HBM-bound byte movers:
+// 3 bytes per 16-bit value (5 per 32-bit one) plus a scale per group.
+#include "common.cuh"
+#include "fp8_math.cuh"
+
+namespace b200 {
+
+// Rows, 16 bytes at a time: K and both row strides are multiples of 16 values, so that a lane's 16 values are whole. Eight lanes share a
+// group of 128; a lane whose values lie beyond K (the last group of a row) takes part in the maximum with zeros.
+template <typename T>
+__global__ void __launch_bounds__(256) k_quantize_fp8_rows(const T* __restrict__ x, long long ldx, int x_rows, const int* __restrict__ src_row, int rows, int K,
+                                                           uint8_t* __restrict__ codes, long long ldc, float* __restrict__ scales) {
+  constexpr int W = 16 * Elem<T>::kSize / 16;      // 16-byte words of a lane's values
+  const int KB = (K + 127) >> 7;
+  const long long units = (long long)rows * KB;
+  grid_dependency_wait();
+  for (long long u = (long long)blockIdx.x * 32 + (threadIdx.x >> 3); u < ((units + 3) & ~3ll); u += (long long)gridDim.x * 32) {   // (whole warps: four units each)
+    const bool in = u < units;
+    const int row = in ? (int)(u / KB) : 0, g = in ? (int)(u - (long long)row * KB) : 0;
+    const int c = g * 128 + (threadIdx.x & 7) * 16;
+    int src = row;
+    if (src_row && in) src = src_row[row];
+    const bool gone = src < 0 || src >= x_rows;      // an empty row: zero codes and scales
+    const bool have = in && !gone && c < K;
+    uint4 w[W];
+#pragma unroll
+    for (int i = 0; i < W; ++i) w[i] = have ? *(reinterpret_cast<const uint4*>(x + (long long)src * ldx + c) + i) : make_uint4(0u, 0u, 0u, 0u);
+    float v[16];
+#pragma unroll
+    for (int i = 0; i < W; ++i) unpack16<T>(w[i], v + i * (16 / W));
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) m = max_nan(m, fabsf(v[i]));
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const Fp8Scale s = fp8_scale(m);
+    if (!in) continue;
+    if (c < K) {
+      uint4 q;
+      q.x = cvt_e4m3x4(v[0] * s.factor, v[1] * s.factor, v[2] * s.factor, v[3] * s.factor);
+      q.y = cvt_e4m3x4(v[4] * s.factor, v[5] * s.factor, v[6] * s.factor, v[7] * s.factor);
+      q.z = cvt_e4m3x4(v[8] * s.factor, v[9] * s.factor, v[10] * s.factor, v[11] * s.factor);
+      q.w = cvt_e4m3x4(v[12] * s.factor, v[13] * s.factor, v[14] * s.factor, v[15] * s.factor);
+      *reinterpret_cast<uint4*>(codes + (long long)row * ldc + c) = q;
+    }
+    if ((threadIdx.x & 7) == 0) scales[(long long)row * KB + g] = gone ? 0.f : s.scale;
+  }
+}
+
+// Rows of any length, stride and alignment: a warp per group, four values a lane, one at a time.
+template <typename T>
+__global__ void __launch_bounds__(256) k_quantize_fp8_rows_any(const T* __restrict__ x, long long ldx, int x_rows, const int* __restrict__ src_row, int rows, int K,
+                                                               uint8_t* __restrict__ codes, long long ldc, float* __restrict__ scales) {
+  const int lane = threadIdx.x & 31, KB = (K + 127) >> 7;
+  const long long units = (long long)rows * KB;
+  grid_dependency_wait();
+  for (long long u = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); u < units; u += (long long)gridDim.x * 8) {
+    const int row = (int)(u / KB), g = (int)(u - (long long)row * KB);
+    const int src = src_row ? src_row[row] : row;
+    const bool gone = src < 0 || src >= x_rows;
+    float v[4], m = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c = g * 128 + i * 32 + lane;
+      v[i] = !gone && c < K ? Elem<T>::load(x + (long long)src * ldx + c) : 0.f;
+      m = max_nan(m, fabsf(v[i]));
+    }
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const Fp8Scale s = fp8_scale(m);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c = g * 128 + i * 32 + lane;
+      if (c < K) codes[(long long)row * ldc + c] = (uint8_t)cvt_e4m3x4(v[i] * s.factor, 0.f, 0.f, 0.f);
+    }
+    if (lane == 0) scales[(long long)row * KB + g] = gone ? 0.f : s.scale;
+  }
+}
+
+// 128x128 blocks: one thread block each, its values in registers as they were loaded (64 a thread of 16 bits, 32 of 32). A row of the block is
+// 128 consecutive values: 16 (32) lanes of 16 bytes.
+template <typename T, bool kVec>
+__global__ void __launch_bounds__(Elem<T>::kSize == 2 ? 256 : 512) k_quantize_fp8_blocks(const T* __restrict__ w, int N, int K, uint8_t* __restrict__ codes, long long ldc,
+                                                                                         float* __restrict__ scales) {
+  constexpr int kThreads = Elem<T>::kSize == 2 ? 256 : 512, kPer = 16 / Elem<T>::kSize, kLanes = 128 / kPer, kRows = kThreads / kLanes, kSteps = 128 / kRows;
+  __shared__ float red[kThreads / 32];
+  const int kb = blockIdx.x, nb = blockIdx.y, KB = gridDim.x, NB = gridDim.y;
+  const long long e = blockIdx.z;
+  const int c = kb * 128 + (threadIdx.x % kLanes) * kPer, r0 = nb * 128 + threadIdx.x / kLanes;
+  const T* src = w + e * N * K + c;
+  grid_dependency_wait();
+  uint4 d[kSteps];
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) {
+    const int r = r0 + i * kRows;
+    d[i] = make_uint4(0u, 0u, 0u, 0u);
+    if constexpr (kVec) {
+      if (r < N && c < K) d[i] = __ldcs(reinterpret_cast<const uint4*>(src + (long long)r * K));
+    } else if (r < N) {
+      T t[kPer];
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) t[j] = c + j < K ? src[(long long)r * K + j] : Elem<T>::make(0.f);
+      memcpy(&d[i], t, 16);
+    }
+  }
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) {
+    float v[kPer];
+    unpack16<T>(d[i], v);
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) m = max_nan(m, fabsf(v[j]));
+  }
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+  __syncthreads();
+  m = red[0];
+#pragma unroll
+  for (int i = 1; i < kThreads / 32; ++i) m = max_nan(m, red[i]);
+  const Fp8Scale s = fp8_scale(m);
+  if (threadIdx.x == 0) scales[(e * NB + nb) * KB + kb] = s.scale;
+  uint8_t* dst = codes + e * N * ldc + c;
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) {
+    const int r = r0 + i * kRows;
+    if (r >= N || c >= K) continue;
+    float v[kPer];
+    unpack16<T>(d[i], v);
+    uint32_t q[kPer / 4];
+#pragma unroll
+    for (int j = 0; j < kPer / 4; ++j) q[j] = cvt_e4m3x4(v[4 * j] * s.factor, v[4 * j + 1] * s.factor, v[4 * j + 2] * s.factor, v[4 * j + 3] * s.factor);
+    if constexpr (kVec) {
+      if constexpr (kPer == 8) __stcs(reinterpret_cast<uint2*>(dst + (long long)r * ldc), make_uint2(q[0], q[1]));
+      else __stcs(reinterpret_cast<uint32_t*>(dst + (long long)r * ldc), q[0]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j)
+        if (c + j < K) dst[(long long)r * ldc + j] = (uint8_t)(q[j / 4] >> (8 * (j & 3)));
+    }
+  }
+}
+
+template <typename T>
+static int quantize_fp8_rows(const void* x, long long ldx, int x_rows, const int* src_row, int rows, int K, void* codes, long long ldc, float* scales, cudaStream_t st) {
+  const long long units = (long long)rows * ((K + 127) / 128);
+  const bool vec = K % 16 == 0 && ldx % (16 / Elem<T>::kSize) == 0 && ldc % 16 == 0 && ((uintptr_t)x & 15) == 0 && ((uintptr_t)codes & 15) == 0;
+  const long long blocks = (units + (vec ? 31 : 7)) / (vec ? 32 : 8);
+  const void* fn = vec ? (const void*)k_quantize_fp8_rows<T> : (const void*)k_quantize_fp8_rows_any<T>;
+  const T* xt = (const T*)x;
+  uint8_t* ct = (uint8_t*)codes;
+  void* args[] = {&xt, &ldx, &x_rows, &src_row, &rows, &K, &ct, &ldc, &scales};
+  return launch_kernel(fn, (int)(blocks < 1 << 30 ? blocks : 1 << 30), 256, 0, true, args, st);
+}
+
+template <typename T>
+static int quantize_fp8_blocks(const void* w, int E, int N, int K, void* codes, long long ldc, float* scales, cudaStream_t st) {
+  const bool vec = K % 16 == 0 && ldc % 16 == 0 && ((uintptr_t)w & 15) == 0 && ((uintptr_t)codes & 15) == 0;
+  const T* wt = (const T*)w;
+  uint8_t* ct = (uint8_t*)codes;
+  for (int e0 = 0; e0 < E; e0 += 65535) {      // (grid limit of the third dimension)
+    const int n = E - e0 < 65535 ? E - e0 : 65535;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((K + 127) / 128, (N + 127) / 128, n), cfg.blockDim = dim3(Elem<T>::kSize == 2 ? 256 : 512), cfg.stream = st;
+    const T* we = wt + (long long)e0 * N * K;
+    uint8_t* ce = ct + (long long)e0 * N * ldc;
+    float* se = scales + (long long)e0 * cfg.gridDim.x * cfg.gridDim.y;
+    void* args[] = {&we, &N, &K, &ce, &ldc, &se};
+    B200_CUDA_TRY(cudaLaunchKernelExC(&cfg, vec ? (const void*)k_quantize_fp8_blocks<T, true> : (const void*)k_quantize_fp8_blocks<T, false>, args));
+  }
+  return B200MOE_OK;
+}
+
+}  // namespace b200
+
+extern "C" {
+
+int b200moe_quantize_fp8(const void* x, int dtype, long long x_stride, int x_rows, const int* src_row, int rows, int K, void* codes, long long codes_stride,
+                         float* scales, void* stream) {
+  using namespace b200;
+  if (rows < 0 || x_rows < 0 || K < 1 || dtype < 0 || dtype > 2 || (x_stride < K && x_rows > 1) || codes_stride < K) return B200MOE_ERR_ARG;
+  if (!src_row && rows != x_rows) return B200MOE_ERR_ARG;
+  if (rows == 0) return B200MOE_OK;
+  if ((!x && x_rows) || !codes || !scales) return B200MOE_ERR_ARG;
+  const int size = dtype == DT_F32 ? 4 : 2;
+  if (((uintptr_t)x & (size - 1)) || ((uintptr_t)scales & 3)) return B200MOE_ERR_ARG;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (dtype == DT_BF16) return quantize_fp8_rows<__nv_bfloat16>(x, x_stride, x_rows, src_row, rows, K, codes, codes_stride, scales, st);
+  if (dtype == DT_F16) return quantize_fp8_rows<__half>(x, x_stride, x_rows, src_row, rows, K, codes, codes_stride, scales, st);
+  return quantize_fp8_rows<float>(x, x_stride, x_rows, src_row, rows, K, codes, codes_stride, scales, st);
+}
+
+int b200moe_quantize_fp8_blocks(const void* w, int dtype, int E, int N, int K, void* codes, long long codes_stride, float* scales, void* stream) {
+  using namespace b200;
+  if (E < 0 || N < 0 || K < 1 || dtype < 0 || dtype > 2 || codes_stride < K) return B200MOE_ERR_ARG;
+  if (E == 0 || N == 0) return B200MOE_OK;
+  if (!w || !codes || !scales) return B200MOE_ERR_ARG;
+  if ((N + 127) / 128 > 65535) return B200MOE_ERR_LIMIT;
+  const int size = dtype == DT_F32 ? 4 : 2;
+  if (((uintptr_t)w & (size - 1)) || ((uintptr_t)scales & 3)) return B200MOE_ERR_ARG;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (dtype == DT_BF16) return quantize_fp8_blocks<__nv_bfloat16>(w, E, N, K, codes, codes_stride, scales, st);
+  if (dtype == DT_F16) return quantize_fp8_blocks<__half>(w, E, N, K, codes, codes_stride, scales, st);
+  return quantize_fp8_blocks<float>(w, E, N, K, codes, codes_stride, scales, st);
+}
+
+}  // extern "C"

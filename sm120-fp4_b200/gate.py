@@ -1,0 +1,122 @@
+"""The router from its logits on: `top_k_gate` gives the (weights, ids) that `Weights.forward` and `route` take, `balance_loss` the auxiliary loss that
+keeps experts evenly used, with the number of pairs of each. Both have gradients with respect to the logits. The reference leaves this part to
+torch (softmax, top-k, renormalise: sm120fp4/kernels/moe_layer.py:195-200).
+
+Nothing here synchronises or keeps state between calls: forward and backward can be captured into a CUDA graph. A capture of a backward pass wants, as with
+every autograd function, that no eager graph of the same leaves is alive."""
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+
+MAX_EXPERTS, MAX_TOP_K = 512, 16
+
+
+def _logits(logits: torch.Tensor, what: str) -> torch.Tensor:
+    if logits.dim() != 2:
+        raise ValueError(f"{what}: expected logits [tokens, experts], got {tuple(logits.shape)}")
+    if logits.dtype not in _lib.DTYPES:
+        raise TypeError(f"{what} takes bf16, fp16 or fp32 logits, not {logits.dtype}")
+    if not 1 <= logits.shape[1] <= MAX_EXPERTS:
+        raise ValueError(f"{what} takes 1 to {MAX_EXPERTS} experts, not {logits.shape[1]}")
+    _lib.one_device(what, logits)
+    if logits.stride(1) != 1 and logits.shape[1] > 1 or logits.stride(0) < logits.shape[1] and logits.shape[0] > 1:
+        return logits.contiguous()
+    return logits
+
+
+def _gate(logits: torch.Tensor, top_k: int, renormalize: bool):
+    tokens, e = logits.shape
+    weights = torch.empty((tokens, top_k), dtype=torch.float32, device=logits.device)
+    ids = torch.empty((tokens, top_k), dtype=torch.int32, device=logits.device)
+    _lib.call(logits.device, "top_k_gate", _lib.lib().b200moe_gate, logits.data_ptr(), _lib.DTYPES[logits.dtype], max(logits.stride(0), e), tokens, e, top_k,
+              int(renormalize), weights.data_ptr(), ids.data_ptr())
+    return weights, ids
+
+
+class _Gate(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, top_k, renormalize):
+        weights, ids = _gate(logits, top_k, renormalize)
+        ctx.mark_non_differentiable(ids)
+        ctx.save_for_backward(weights, ids, None if renormalize else logits)      # (normalised weights do not depend on the experts left out)
+        ctx.like, ctx.renormalize = (logits.dtype, logits.shape[1]), renormalize
+        return weights, ids
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad, _):
+        weights, ids, logits = ctx.saved_tensors
+        dtype, e = ctx.like
+        tokens, k = weights.shape
+        out = torch.empty((tokens, e), dtype=dtype, device=weights.device)
+        grad = grad.contiguous()
+        _lib.call(out.device, "top_k_gate backward", _lib.lib().b200moe_gate_backward, grad.data_ptr(), weights.data_ptr(), ids.data_ptr(), _lib.ptr(logits),
+                  _lib.DTYPES[dtype], e if logits is None else max(logits.stride(0), e), tokens, e, k, int(ctx.renormalize), out.data_ptr())
+        return out, None, None
+
+
+def top_k_gate(logits: torch.Tensor, top_k: int, renormalize: bool = True):
+    """logits [T, E] bf16, fp16 or fp32 -> (weights f32 [T, top_k], ids int32 [T, top_k]): each token's top_k largest logits in falling order (ties to
+    the lowest index) and their softmax probabilities, divided by their sum where `renormalize`. Up to 512 experts and 16 of them a token; rows may be any
+    stride apart. A logit of -inf is an expert that may not be taken: a slot for which none is left gets id -1 (an empty slot of the layer calls) and weight 0. A NaN
+    ranks above all numbers and makes its token's weights NaN. Differentiable with respect to the logits through the weights."""
+    top_k = int(top_k)
+    logits = _logits(logits, "top_k_gate")
+    if not 1 <= top_k <= min(MAX_TOP_K, logits.shape[1]):
+        raise ValueError(f"top_k_gate takes 1 to {min(MAX_TOP_K, logits.shape[1])} of {logits.shape[1]} experts, not {top_k}")
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _Gate.apply(logits, top_k, bool(renormalize))
+    return _gate(logits, top_k, bool(renormalize))
+
+
+def _balance(logits: torch.Tensor, ids: torch.Tensor):
+    tokens, e = logits.shape
+    h = _lib.lib()
+    nbytes = h.b200moe_balance_workspace_bytes(tokens, e)
+    ws = torch.empty(max(nbytes, 4), dtype=torch.uint8, device=logits.device)
+    sums = torch.empty(3, dtype=torch.float32, device=logits.device)      # the loss, and what the backward pass reads
+    counts = torch.empty(e, dtype=torch.int32, device=logits.device)
+    _lib.call(logits.device, "balance_loss", h.b200moe_balance_loss, logits.data_ptr(), _lib.DTYPES[logits.dtype], max(logits.stride(0), e), tokens, e, ids.data_ptr(),
+              ids.shape[1], sums.data_ptr(), counts.data_ptr(), sums.data_ptr() + 4, ws.data_ptr(), nbytes)
+    return sums, counts
+
+
+class _Balance(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, ids):
+        sums, counts = _balance(logits, ids)
+        ctx.mark_non_differentiable(counts)
+        ctx.save_for_backward(logits, ids, sums, counts)
+        return sums[0].clone(), counts
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad, _):
+        logits, ids, sums, counts = ctx.saved_tensors
+        tokens, e = logits.shape
+        out = torch.empty((tokens, e), dtype=logits.dtype, device=logits.device)
+        grad = grad.contiguous()
+        _lib.call(out.device, "balance_loss backward", _lib.lib().b200moe_balance_backward, grad.data_ptr(), logits.data_ptr(), _lib.DTYPES[logits.dtype],
+                  max(logits.stride(0), e), tokens, e, ids.data_ptr(), ids.shape[1], counts.data_ptr(), sums.data_ptr() + 4, out.data_ptr())
+        return out, None
+
+
+def balance_loss(logits: torch.Tensor, ids: torch.Tensor):
+    """logits [T, E], ids int32 [T, k] (the router's choice) -> (loss f32 [], counts int32 [E]):
+    loss = E * sum_e f_e P_e with f_e expert e's share of all pairs and P_e the mean over tokens of softmax(logits)_e; it is 1 where experts are used
+    evenly. counts are the pairs of each expert. An id outside 0..E-1 is an empty slot, and a token of empty slots alone (padding) counts nowhere; without any
+    live token the loss is 0. Differentiable with respect to the logits through P (f is a count). k up to 32, experts up to 512."""
+    logits = _logits(logits, "balance_loss")
+    if ids.dtype != torch.int32:
+        raise TypeError(f"balance_loss takes int32 ids, not {ids.dtype}")
+    if ids.dim() != 2 or ids.shape[0] != logits.shape[0] or not 1 <= ids.shape[1] <= 32:
+        raise ValueError(f"balance_loss: expected ids [{logits.shape[0]}, 1 to 32], got {tuple(ids.shape)}")
+    _lib.one_device("balance_loss", logits, ids)
+    ids = ids.contiguous()
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _Balance.apply(logits, ids)
+    sums, counts = _balance(logits, ids)
+    return sums[0], counts

@@ -1,0 +1,337 @@
+"""GPU parity of the router from logits and of the balance loss: against their formulas in 64 bits, and gradients against differences.
+
+Tolerances count roundings. expf is within 2 ulp (2^-22 relative) and its argument x - m rounded once (|x - m| 2^-24 relative in the result); a sum over E
+is a tree of at most V + 5 additions, V = values of a lane; quotients and products one rounding each."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def lane_values(e):
+    return next(v for v in (1, 2, 4, 8, 16) if e <= 32 * v)
+
+
+def softmax64(x):
+    """Rows of -inf alone: zeros."""
+    x = x.double()
+    m = x.amax(1, keepdim=True)
+    p = torch.exp(x - torch.where(m == -math.inf, torch.zeros_like(m), m))
+    s = p.sum(1, keepdim=True)
+    return p / torch.where(s == 0, torch.ones_like(s), s)
+
+
+def spread(x):
+    x = x.double()
+    live = x > -math.inf
+    top = torch.where(live, x, -torch.ones_like(x) * math.inf).amax(1, keepdim=True)
+    d = torch.where(live, top - x, torch.zeros_like(x)).amax()
+    return float(d) if math.isfinite(float(d)) else 0.0
+
+
+def rel_p(x):
+    """Relative error of one probability (a quotient of an exponential and a sum of them)."""
+    one = min(spread(x), 104.0) * U + 4 * U      # (exponentials of differences above 104 are zero in fp32)
+    return 2 * one + (lane_values(x.shape[1]) + 7) * U
+
+
+def gate64(x, k, renormalize):
+    x = x.detach().double()
+    ids = torch.sort(x, dim=1, descending=True, stable=True)[1][:, :k]
+    live = x.gather(1, ids) > -math.inf
+    p = softmax64(x)
+    w = torch.where(live, p.gather(1, ids), torch.zeros_like(ids, dtype=torch.float64))
+    if renormalize:
+        s = w.sum(1, keepdim=True)
+        w = w / torch.where(s == 0, torch.ones_like(s), s)
+    return w, torch.where(live, ids, -torch.ones_like(ids)).int(), p
+
+
+def gate_grad64(x, k, renormalize, g):
+    w, ids, p = gate64(x, k, renormalize)
+    live = ids >= 0
+    g = torch.where(live, g.double(), torch.zeros_like(w))
+    dot, size = (g * w).sum(1, keepdim=True), (g.abs() * w).sum(1, keepdim=True)
+    at = ids.clamp(min=0).long()
+    if renormalize:
+        d, m = [torch.zeros_like(p).scatter_add_(1, at, torch.where(live, v, torch.zeros_like(v))) for v in (w * (g - dot), w * (g.abs() + size))]
+    else:
+        dense = torch.zeros_like(p).scatter_add_(1, at, g)
+        d, m = p * (dense - dot), p * (dense.abs() + size)
+    return d, m
+
+
+def logits(t, e, dtype, seed, masked=False, scale=2.0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(t, e, generator=g) * scale
+    if masked:
+        x[torch.rand(t, e, generator=g) < 0.4] = -math.inf
+        if t > 2:
+            x[1] = -math.inf
+            x[2, 1:] = -math.inf
+    return x.to(dtype).cuda()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("t,e,k", [(1, 128, 8), (1, 1, 1), (3, 7, 7), (5, 8, 2), (33, 60, 4), (9, 33, 16), (17, 100, 6), (64, 128, 8), (130, 256, 10), (31, 257, 3), (40, 384, 8),
+                                   (21, 511, 16), (12, 512, 16), (5000, 64, 6)])
+def test_gate(dtype, t, e, k):
+    import sm120fp4_b200 as pkg
+    for masked in (False, True):
+        x = logits(t, e, dtype, t * 1000 + e + masked, masked)
+        for renormalize in (True, False):
+            w, ids, _ = gate64(x, k, renormalize)
+            got_w, got_ids = pkg.top_k_gate(x, k, renormalize)
+            assert got_w.dtype == torch.float32 and got_ids.dtype == torch.int32 and got_w.shape == got_ids.shape == (t, k)
+            assert torch.equal(got_ids, ids)
+            tol = rel_p(x) * w + 2.0 ** -126
+            assert bool(((got_w.double() - w).abs() <= tol).all())
+            leaf = x.clone().requires_grad_(True)
+            w2, ids2 = pkg.top_k_gate(leaf, k, renormalize)
+            assert torch.equal(w2.detach(), got_w) and torch.equal(ids2, got_ids)
+            g = torch.randn(t, k, generator=torch.Generator().manual_seed(5)).cuda()
+            w2.backward(g)
+            d, size = gate_grad64(x, k, renormalize, g)
+            assert leaf.grad.dtype == dtype
+            tol = (3 * rel_p(x) + 12 * U) * size + half_step(dtype) * d.abs() + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps + 2.0 ** -126
+            assert bool(((leaf.grad.double() - d).abs() <= tol).all())
+
+
+def test_gate_ties_go_to_the_lowest_index():
+    import sm120fp4_b200 as pkg
+    for e in (7, 64, 128, 300):
+        x = torch.randint(-2, 3, (200, e), generator=torch.Generator().manual_seed(e)).float()
+        x[::3] = 0.0
+        x[1::3, ::2] *= -0.0
+        for dtype in TYPES:
+            y = x.to(dtype).cuda()
+            w, ids = pkg.top_k_gate(y, min(8, e - 1))
+            assert torch.equal(ids, gate64(y, min(8, e - 1), True)[1])
+
+
+def test_gate_extreme_values():
+    import sm120fp4_b200 as pkg
+    low = torch.finfo(torch.bfloat16).min
+    x = torch.full((6, 16), low, dtype=torch.bfloat16)
+    x[0] = 0                                                       # all alike
+    x[1, 3] = 1.0                                                  # one above the type's lowest value
+    x[2, :] = low                                                  # the lowest value everywhere: still a softmax of equals
+    x[3, 5], x[3, 6] = float("nan"), 2.0
+    x[4, 2] = math.inf
+    x[5, :] = -math.inf
+    w, ids = pkg.top_k_gate(x.cuda(), 2)
+    w, ids = w.cpu(), ids.cpu()
+    assert ids[0].tolist() == [0, 1] and w[0].tolist() == [0.5, 0.5]
+    assert ids[1].tolist() == [3, 0] and w[1].tolist() == [1.0, 0.0]
+    assert ids[2].tolist() == [0, 1] and w[2].tolist() == [0.5, 0.5]
+    assert ids[3].tolist() == [5, 6] and w[3].isnan().all()        # NaN above all, and seen in the weights
+    assert ids[4, 0] == 2 and w[4].isnan().any()
+    assert ids[5].tolist() == [-1, -1] and w[5].tolist() == [0.0, 0.0]
+    assert int(ids.max()) < 16
+
+
+def test_gate_gradient_of_empty_slots_is_zero_whatever_comes_in():
+    import sm120fp4_b200 as pkg
+    x = torch.full((3, 8), -math.inf)
+    x[0, 2], x[1] = 1.0, torch.arange(8.0)
+    for renormalize in (True, False):
+        leaf = x.cuda().requires_grad_(True)
+        w, ids = pkg.top_k_gate(leaf, 2, renormalize)
+        assert ids.tolist() == [[2, -1], [7, 6], [-1, -1]]
+        g = torch.tensor([[1.0, math.nan], [1.0, 2.0], [math.inf, math.nan]]).cuda()
+        w.backward(g)
+        assert bool(torch.isfinite(leaf.grad).all()) and float(leaf.grad[0].abs().max()) == 0.0 and float(leaf.grad[2].abs().max()) == 0.0
+
+
+def test_gate_strides_and_views():
+    """Rows apart, rows off 16 bytes, a column-major matrix, one row for all tokens (whose gradient is the sum over them)."""
+    import sm120fp4_b200 as pkg
+    big = logits(40, 300, torch.bfloat16, 3)
+    for x in (big[:, :128], big[:, 1:129], big[::2, 3:67], big.t()[:256, :30], big[:1, :64]):
+        w, ids = pkg.top_k_gate(x, 4)
+        w2, ids2 = pkg.top_k_gate(x.contiguous(), 4)
+        assert torch.equal(w, w2) and torch.equal(ids, ids2)
+        base = x.detach().clone().requires_grad_(True)
+        for renormalize in (True, False):
+            g = torch.randn(w.shape, generator=torch.Generator().manual_seed(1)).cuda()
+            got = torch.autograd.grad(pkg.top_k_gate(base, 4, renormalize)[0], base, g)[0]
+            want, size = gate_grad64(x, 4, renormalize, g)
+            assert bool(((got.double() - want).abs() <= (3 * rel_p(x) + 12 * U) * size + half_step(x.dtype) * want.abs() + 2.0 ** -126).all())
+    row = logits(1, 64, torch.float32, 9).requires_grad_(True)
+    g = torch.randn(50, 4, generator=torch.Generator().manual_seed(2)).cuda()
+    got = torch.autograd.grad(pkg.top_k_gate(row.expand(50, 64), 4)[0], row, g)[0]
+    want, size = gate_grad64(row.detach().expand(50, 64), 4, True, g)
+    assert bool(((got.double() - want.sum(0)).abs() <= (3 * rel_p(row.detach()) + 12 * U + 50 * U) * size.sum(0) + 2.0 ** -126).all())
+
+
+def test_gate_gradient_against_differences():
+    """Central differences of the 64-bit forward, step 2^-10: their own error is of the third derivative, below 2^-20 for softmax terms of at most 1."""
+    import sm120fp4_b200 as pkg
+    x = logits(3, 12, torch.float32, 77, scale=1.0)
+    g = torch.randn(3, 4, generator=torch.Generator().manual_seed(8)).cuda()
+    h = 2.0 ** -10
+    for renormalize in (True, False):
+        leaf = x.clone().requires_grad_(True)
+        got = torch.autograd.grad(pkg.top_k_gate(leaf, 4, renormalize)[0], leaf, g)[0]
+        ids = gate64(x, 4, renormalize)[1]
+        for c in range(12):
+            up, down = x.double(), x.double()
+            up[:, c] += h
+            down[:, c] -= h
+            a, b = gate64(up, 4, renormalize), gate64(down, 4, renormalize)
+            assert torch.equal(a[1].sort(1)[0], ids.sort(1)[0]) and torch.equal(b[1].sort(1)[0], ids.sort(1)[0])      # (the step changes no choice)
+            at = ids.long()
+            wide = [torch.zeros_like(up).scatter_(1, o[1].long(), o[0]).gather(1, at) for o in (a, b)]
+            diff = ((wide[0] - wide[1]) / (2 * h) * g.double()).sum(1)
+            assert bool(((got[:, c].double() - diff).abs() <= 4 * 4 * 2.0 ** -20 + 2.0 ** -18).all())
+
+
+def test_gate_refusals():
+    import sm120fp4_b200 as pkg
+    x = torch.zeros(2, 8, device="cuda")
+    for k in (0, 9, -1):
+        with pytest.raises(ValueError):
+            pkg.top_k_gate(x, k)
+    with pytest.raises(ValueError):
+        pkg.top_k_gate(torch.zeros(2, 64, device="cuda"), 17)
+    w, ids = pkg.top_k_gate(torch.zeros(0, 8, device="cuda", requires_grad=True), 2)
+    assert w.shape == ids.shape == (0, 2)
+    w.sum().backward()
+
+
+# ---------------------------------------------------------------------------------------------------- balance loss
+
+def balance64(x, ids, e):
+    p = softmax64(x)
+    used = (ids >= 0) & (ids < e)
+    live = used.any(1)
+    counts = torch.bincount(ids[used].long(), minlength=e)
+    f = counts.double() / max(1, int(counts.sum()))
+    tokens = max(1, int(live.sum()))
+    p = p * live[:, None]
+    loss = e / tokens * (p.sum(0) @ f)
+    dot = (p @ f)[:, None]
+    return loss, counts.int(), e / tokens * p * (f - dot), e / tokens * p * (f + dot)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("t,e,k", [(1, 8, 2), (2, 1, 1), (7, 60, 4), (333, 60, 4), (64, 128, 8), (9, 100, 32), (513, 257, 3), (20000, 256, 8), (33, 512, 16)])
+def test_balance(dtype, t, e, k):
+    import sm120fp4_b200 as pkg
+    gen = torch.Generator().manual_seed(t + e)
+    for kind in ("plain", "padded", "masked"):
+        x = logits(t, e, dtype, t + e, kind == "masked")
+        ids = torch.rand(t, e, generator=gen).argsort(1)[:, :min(k, e)].int()
+        if kind != "plain":
+            ids[torch.rand(ids.shape, generator=gen) < 0.3] = -1
+            ids[t // 2:t // 2 + 2] = -1
+            ids[0, 0] = e + 5 if t > 1 else ids[0, 0]      # beyond the experts: an empty slot
+        ids = ids.cuda()
+        loss, counts, dx, size = balance64(x, ids, e)
+        leaf = x.clone().requires_grad_(True)
+        got, got_counts = pkg.balance_loss(leaf, ids)
+        assert got.shape == () and torch.equal(got_counts, counts)
+        adds = -(-t // (8 * min(592, -(-t // 8)))) + 8
+        tol = (rel_p(x) + (adds + 4) * U)
+        assert abs(float(got.double() - loss)) <= tol * float(loss) + 2.0 ** -126
+        again = pkg.balance_loss(x, ids)
+        assert torch.equal(again[0], got.detach()) and torch.equal(again[1], counts)
+        up = torch.tensor(0.37, device="cuda")
+        got.backward(up)
+        scale = float(up.double())
+        tol = (2 * rel_p(x) + (lane_values(e) + 16) * U) * size * scale + half_step(dtype) * dx.abs() * scale + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps + 2.0 ** -120
+        assert bool(((leaf.grad.double() - dx * scale).abs() <= tol).all())
+
+
+def test_balance_gradient_against_differences():
+    """As for the gate: the loss in 64 bits, step 2^-10."""
+    import sm120fp4_b200 as pkg
+    x = logits(5, 6, torch.float32, 4, scale=1.0)
+    ids = torch.tensor([[0, 1], [1, 2], [-1, -1], [5, -1], [1, 0]], dtype=torch.int32, device="cuda")
+    leaf = x.clone().requires_grad_(True)
+    pkg.balance_loss(leaf, ids)[0].backward()
+    h = 2.0 ** -10
+    for t in range(5):
+        for c in range(6):
+            up, down = x.double(), x.double()
+            up[t, c] += h
+            down[t, c] -= h
+            diff = float(balance64(up, ids, 6)[0] - balance64(down, ids, 6)[0]) / (2 * h)
+            assert abs(float(leaf.grad[t, c]) - diff) <= 6 * 2.0 ** -20 + 2.0 ** -18
+    assert float(leaf.grad[2].abs().max()) == 0.0
+
+
+def test_balance_without_a_live_token():
+    import sm120fp4_b200 as pkg
+    for t in (0, 3):
+        x = torch.full((t, 8), math.nan, device="cuda", requires_grad=True)      # padding may hold anything
+        loss, counts = pkg.balance_loss(x, torch.full((t, 2), -1, dtype=torch.int32, device="cuda"))
+        loss.backward()
+        assert float(loss) == 0.0 and counts.tolist() == [0] * 8 and x.grad.shape == x.shape and not bool((x.grad != 0).any())
+
+
+def test_balance_nan_in_padding_stays_there():
+    import sm120fp4_b200 as pkg
+    x = logits(50, 32, torch.bfloat16, 6)
+    ids = torch.rand(50, 32, generator=torch.Generator().manual_seed(3)).argsort(1)[:, :4].int()
+    ids[30:] = -1
+    ids = ids.cuda()
+    clean = x[:30].clone().requires_grad_(True)
+    a = pkg.balance_loss(clean, ids[:30].contiguous())
+    a[0].backward()
+    x[30:] = math.nan
+    x.requires_grad_(True)
+    b = pkg.balance_loss(x, ids)
+    b[0].backward()
+    assert torch.equal(a[1], b[1]) and abs(float(a[0]) - float(b[0])) <= 64 * U * float(a[0])
+    assert torch.equal(x.grad[:30], clean.grad) and float(x.grad[30:].float().abs().max()) == 0.0
+
+
+def test_balance_refusals():
+    import sm120fp4_b200 as pkg
+    x = torch.zeros(4, 8, device="cuda")
+    with pytest.raises(TypeError):
+        pkg.balance_loss(x, torch.zeros(4, 2, dtype=torch.int64, device="cuda"))
+    with pytest.raises(ValueError):
+        pkg.balance_loss(x, torch.zeros(3, 2, dtype=torch.int32, device="cuda"))
+    with pytest.raises(ValueError):
+        pkg.balance_loss(x, torch.zeros(4, 33, dtype=torch.int32, device="cuda"))
+    with pytest.raises(RuntimeError):
+        pkg.balance_loss(x, torch.zeros(4, 2, dtype=torch.int32))
+
+
+def test_gate_and_balance_in_a_graph_and_on_another_stream():
+    import sm120fp4_b200 as pkg
+    x = logits(300, 64, torch.float32, 12)
+    static, grad = x.clone().requires_grad_(True), torch.randn(300, 4, generator=torch.Generator().manual_seed(1)).cuda()
+
+    def step(leaf):
+        w, ids = pkg.top_k_gate(leaf, 4)
+        loss, counts = pkg.balance_loss(leaf, ids)
+        g, = torch.autograd.grad([w, loss], leaf, [grad, torch.ones_like(loss)])
+        return w.detach(), ids, loss.detach(), counts, g
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(static)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(static)
+    for seed in (1, 2):
+        y = logits(300, 64, torch.float32, 100 + seed)
+        with torch.no_grad():
+            static.copy_(y)
+        graph.replay()
+        want = step(y.clone().requires_grad_(True))
+        for a, b in zip(out, want):
+            assert torch.equal(a, b)
