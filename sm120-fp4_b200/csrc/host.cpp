@@ -8,7 +8,10 @@
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 namespace {
@@ -117,9 +120,257 @@ PyObject* py_quantize_128x4(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---------------------------------------------------------------------------------------------------- router and FP8 operators
+// The same for the router from logits, its balance loss and the FP8 operators: what gate.py and fp8.py do for plain tensors, gradients included (as nodes of
+// the autograd engine that call the library; a gradient of one training step of 16384 x 128 logits took 100 us of which 85 were Python's).
+struct Ops {
+  int (*gate)(const void*, int, long long, int, int, int, int, void*, void*, void*);
+  int (*gate_backward)(const void*, const void*, const void*, const void*, int, long long, int, int, int, int, void*, void*);
+  long long (*balance_workspace_bytes)(int, int);
+  int (*balance_loss)(const void*, int, long long, int, int, const void*, int, void*, void*, void*, void*, long long, void*);
+  int (*balance_backward)(const void*, const void*, int, long long, int, int, const void*, int, const void*, const void*, void*, void*);
+  int (*quantize_fp8)(const void*, int, long long, int, const void*, int, int, void*, long long, void*, void*);
+  int (*matmul_fp8)(const void*, long long, const void*, const void*, long long, const void*, int, int, int, void*, int, long long, void*);
+  int (*matmul_fp8_experts)(const void*, long long, const void*, int, const void*, long long, const void*, int, const void*, const void*, int, int, int, void*, int, long long,
+                            int, void*);
+  const char* (*error_string)(int);
+} ops = {};
+constexpr int64_t kMaxExperts = 512, kMaxTopK = 16, kMaxSize = 1ll << 30;
+
+void* stream() { return (void*)c10::cuda::getCurrentCUDAStream().stream(); }
+int dtype_code(at::ScalarType t) { return t == at::kBFloat16 ? 0 : t == at::kFloat ? 1 : t == at::kHalf ? 2 : -1; }
+at::Tensor fresh(at::IntArrayRef size, at::ScalarType t, const at::Tensor& like) { return at::empty(size, at::TensorOptions().dtype(t).device(like.device())); }
+bool here(const at::Tensor& t) { return plain_tensor(t) && t.get_device() == c10::cuda::current_device(); }
+bool plain_logits(const at::Tensor& x) {
+  return here(x) && x.dim() == 2 && dtype_code(x.scalar_type()) >= 0 && x.size(0) > 0 && x.size(0) <= kMaxSize && x.size(1) > 0 && x.size(1) <= kMaxExperts && x.stride(1) == 1 &&
+         (x.stride(0) >= x.size(1) || x.size(0) == 1);
+}
+long long row_stride(const at::Tensor& x) { return std::max(x.stride(0), x.size(1)); }
+bool vector_of(const at::Tensor& t, at::ScalarType type) { return here(t) && t.dim() == 1 && t.scalar_type() == type && t.is_contiguous(); }
+void checked(int rc, const char* what) { TORCH_CHECK(rc == 0, what, ": ", ops.error_string(rc), " (", rc, ")"); }
+// The gradient of a gradient is not there: whoever asks for it is told so.
+at::Tensor once(at::Tensor out, const char* what) {
+  if (!at::GradMode::is_enabled()) return out;
+  auto error = std::make_shared<torch::autograd::DelayedError>(std::string(what) + " is differentiable once", 1);
+  return (*error)({out.detach().requires_grad_(true)})[0];
+}
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+int run_gate(const at::Tensor& x, int64_t k, bool renormalize, at::Tensor& weights, at::Tensor& ids) {
+  weights = fresh({x.size(0), k}, at::kFloat, x), ids = fresh({x.size(0), k}, at::kInt, x);
+  return ops.gate(x.data_ptr(), dtype_code(x.scalar_type()), row_stride(x), (int)x.size(0), (int)x.size(1), (int)k, renormalize, weights.data_ptr(), ids.data_ptr(), stream());
+}
+struct Gate : torch::autograd::Function<Gate> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& x, int64_t k, bool renormalize) {
+    at::Tensor weights, ids;
+    checked(run_gate(x, k, renormalize, weights, ids), "top_k_gate");
+    ctx->mark_non_differentiable({ids});
+    ctx->save_for_backward({weights, ids, renormalize ? at::Tensor() : x});      // (normalised weights do not depend on the experts left out)
+    ctx->saved_data["e"] = x.size(1), ctx->saved_data["dtype"] = (int64_t)x.scalar_type(), ctx->saved_data["renormalize"] = renormalize;
+    return {weights, ids};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    if (!grads[0].defined()) return {at::Tensor(), at::Tensor(), at::Tensor()};
+    const variable_list saved = ctx->get_saved_variables();
+    const at::Tensor &weights = saved[0], &ids = saved[1], &x = saved[2], grad = grads[0].detach().contiguous();
+    const int64_t e = ctx->saved_data["e"].toInt();
+    const auto dtype = (at::ScalarType)ctx->saved_data["dtype"].toInt();
+    const at::Tensor out = fresh({weights.size(0), e}, dtype, weights);
+    checked(ops.gate_backward(grad.data_ptr(), weights.data_ptr(), ids.data_ptr(), x.defined() ? x.data_ptr() : nullptr, dtype_code(dtype), x.defined() ? row_stride(x) : e,
+                              (int)weights.size(0), (int)e, (int)weights.size(1), ctx->saved_data["renormalize"].toBool(), out.data_ptr(), stream()),
+            "top_k_gate backward");
+    return {once(out, "top_k_gate"), at::Tensor(), at::Tensor()};
+  }
+};
+
+int run_balance(const at::Tensor& x, const at::Tensor& ids, at::Tensor& loss, at::Tensor& counts, at::Tensor& stats) {
+  const int tokens = (int)x.size(0), e = (int)x.size(1);
+  const long long bytes = ops.balance_workspace_bytes(tokens, e);
+  if (bytes < 0) return (int)bytes;
+  const at::Tensor ws = fresh({(bytes + 3) / 4}, at::kFloat, x);
+  loss = fresh({}, at::kFloat, x), counts = fresh({e}, at::kInt, x), stats = fresh({2}, at::kFloat, x);
+  return ops.balance_loss(x.data_ptr(), dtype_code(x.scalar_type()), row_stride(x), tokens, e, ids.data_ptr(), (int)ids.size(1), loss.data_ptr(), counts.data_ptr(), stats.data_ptr(),
+                          ws.data_ptr(), bytes, stream());
+}
+struct Balance : torch::autograd::Function<Balance> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& ids) {
+    at::Tensor loss, counts, stats;
+    checked(run_balance(x, ids, loss, counts, stats), "balance_loss");
+    ctx->mark_non_differentiable({counts});
+    ctx->save_for_backward({x, ids, counts, stats});
+    return {loss, counts};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    if (!grads[0].defined()) return {at::Tensor(), at::Tensor()};
+    const variable_list saved = ctx->get_saved_variables();
+    const at::Tensor &x = saved[0], &ids = saved[1], &counts = saved[2], &stats = saved[3], grad = grads[0].detach().contiguous();
+    const at::Tensor out = fresh({x.size(0), x.size(1)}, x.scalar_type(), x);
+    checked(ops.balance_backward(grad.data_ptr(), x.data_ptr(), dtype_code(x.scalar_type()), row_stride(x), (int)x.size(0), (int)x.size(1), ids.data_ptr(), (int)ids.size(1),
+                                 counts.data_ptr(), stats.data_ptr(), out.data_ptr(), stream()),
+            "balance_loss backward");
+    return {once(out, "balance_loss"), at::Tensor()};
+  }
+};
+
+PyObject* pair(int rc, const at::Tensor& a, const at::Tensor& b) {
+  if (rc) return PyLong_FromLong(rc);
+  PyObject *p = THPVariable_Wrap(a), *q = THPVariable_Wrap(b), *t = p && q ? PyTuple_New(2) : nullptr;
+  if (!t) {
+    Py_XDECREF(p), Py_XDECREF(q);
+    return nullptr;
+  }
+  PyTuple_SET_ITEM(t, 0, p), PyTuple_SET_ITEM(t, 1, q);
+  return t;
+}
+bool tensors(PyObject* const* args, Py_ssize_t n) {
+  for (Py_ssize_t i = 0; i < n; ++i)
+    if (!THPVariable_CheckExact(args[i])) return false;
+  return ops.gate && plain_call();
+}
+
+// bind_ops(addresses of the library's functions in the order of Ops)
+PyObject* py_bind_ops(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  constexpr Py_ssize_t count = sizeof(Ops) / sizeof(void*);
+  void* at[count];
+  if (n != count) {
+    PyErr_SetString(PyExc_TypeError, "bind_ops takes the addresses of the operators");
+    return nullptr;
+  }
+  for (Py_ssize_t i = 0; i < n; ++i) at[i] = PyLong_AsVoidPtr(args[i]);
+  if (PyErr_Occurred()) return nullptr;
+  memcpy(&ops, at, sizeof ops);
+  Py_RETURN_NONE;
+}
+
+// top_k_gate(logits, k, renormalize)
+PyObject* py_top_k_gate(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 3 || !tensors(args, 1) || !PyLong_CheckExact(args[1]) || !PyBool_Check(args[2])) Py_RETURN_NONE;
+  const at::Tensor x = THPVariable_Unpack(args[0]);
+  int over = 0;
+  const long long k = PyLong_AsLongLongAndOverflow(args[1], &over);
+  if (over || !plain_logits(x) || k < 1 || k > kMaxTopK || k > x.size(1)) Py_RETURN_NONE;
+  const bool renormalize = args[2] == Py_True;
+  at::Tensor weights, ids;
+  int rc = 0;
+  {
+    Released released;
+    if (x.requires_grad() && at::GradMode::is_enabled()) {
+      const variable_list out = Gate::apply(x, (int64_t)k, renormalize);
+      weights = out[0], ids = out[1];
+    } else {
+      rc = run_gate(x, k, renormalize, weights, ids);
+    }
+  }
+  return pair(rc, weights, ids);
+  END_HANDLE_TH_ERRORS
+}
+
+// balance_loss(logits, ids)
+PyObject* py_balance_loss(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 2 || !tensors(args, 2)) Py_RETURN_NONE;
+  const at::Tensor x = THPVariable_Unpack(args[0]), ids = THPVariable_Unpack(args[1]);
+  if (!plain_logits(x) || !here(ids) || ids.dim() != 2 || ids.scalar_type() != at::kInt || !ids.is_contiguous() || ids.size(0) != x.size(0) || ids.size(1) < 1 || ids.size(1) > 32)
+    Py_RETURN_NONE;
+  at::Tensor loss, counts, stats;
+  int rc = 0;
+  {
+    Released released;
+    if (x.requires_grad() && at::GradMode::is_enabled()) {
+      const variable_list out = Balance::apply(x, ids);
+      loss = out[0], counts = out[1];
+    } else {
+      rc = run_balance(x, ids, loss, counts, stats);
+    }
+  }
+  return pair(rc, loss, counts);
+  END_HANDLE_TH_ERRORS
+}
+
+// quantize_fp8(x, src_row or None)
+PyObject* py_quantize_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 2 || !tensors(args, args[1] == Py_None ? 1 : 2)) Py_RETURN_NONE;
+  const at::Tensor x = THPVariable_Unpack(args[0]), src = args[1] == Py_None ? at::Tensor() : THPVariable_Unpack(args[1]);
+  if (!here(x) || x.dim() != 2 || dtype_code(x.scalar_type()) < 0 || x.size(0) < 1 || x.size(1) < 1 || x.size(0) > kMaxSize || x.size(1) > kMaxSize || x.stride(1) != 1 ||
+      (x.stride(0) < x.size(1) && x.size(0) > 1) || (src.defined() && (!vector_of(src, at::kInt) || src.size(0) > kMaxSize)))
+    Py_RETURN_NONE;
+  const int64_t k = x.size(1), rows = src.defined() ? src.size(0) : x.size(0), ld = (k + 15) & ~15ll;
+  at::Tensor codes, scales;
+  int rc;
+  {
+    Released released;
+    codes = at::empty_strided({rows, k}, {ld, 1}, at::TensorOptions().dtype(at::kFloat8_e4m3fn).device(x.device())), scales = fresh({rows, (k + 127) / 128}, at::kFloat, x);
+    rc = ops.quantize_fp8(x.data_ptr(), dtype_code(x.scalar_type()), x.size(0) > 1 ? x.stride(0) : ld, (int)x.size(0), src.defined() ? src.data_ptr() : nullptr, (int)rows, (int)k,
+                          codes.data_ptr(), ld, scales.data_ptr(), stream());
+  }
+  return pair(rc, codes, scales);
+  END_HANDLE_TH_ERRORS
+}
+
+// bytes between rows of codes that the products take as they are, 0 for others
+int64_t codes_stride(const at::Tensor& t) {
+  if (!here(t) || t.scalar_type() != at::kFloat8_e4m3fn) return 0;
+  const int64_t k = t.size(-1), ld = t.size(-2) > 1 ? t.stride(-2) : (k + 15) & ~15ll;
+  return k >= 1 && k <= kMaxSize && (t.stride(-1) == 1 || k == 1) && ld >= k && ld % 16 == 0 && (uintptr_t)t.data_ptr() % 16 == 0 ? ld : 0;
+}
+bool scales_of(const at::Tensor& s, at::IntArrayRef size) { return here(s) && s.scalar_type() == at::kFloat && s.sizes() == size && s.is_contiguous(); }
+
+// matmul_fp8(a, a_scale, w, w_scale, dtype), matmul_fp8_experts(a, a_scale, w, w_scale, experts, offsets, dtype): a new output
+PyObject* matmul(PyObject* const* args, bool experts) {
+  HANDLE_TH_ERRORS
+  const int count = experts ? 6 : 4;
+  if (!tensors(args, count) || !THPDtype_Check(args[count])) Py_RETURN_NONE;
+  const at::ScalarType type = reinterpret_cast<THPDtype*>(args[count])->scalar_type;
+  const at::Tensor a = THPVariable_Unpack(args[0]), sa = THPVariable_Unpack(args[1]), w = THPVariable_Unpack(args[2]), sw = THPVariable_Unpack(args[3]);
+  if (dtype_code(type) < 0 || a.dim() != 2 || w.dim() != (experts ? 3 : 2) || a.size(1) != w.size(-1)) Py_RETURN_NONE;
+  const int64_t lda = codes_stride(a), ldw = codes_stride(w), m = a.size(0), n = w.size(-2), k = a.size(1), g = (k + 127) / 128;
+  if (!lda || !ldw || m < 1 || n < 1 || m > kMaxSize || n > kMaxSize || !scales_of(sa, {m, g})) Py_RETURN_NONE;
+  at::Tensor table, offsets;
+  if (experts) {
+    table = THPVariable_Unpack(args[4]), offsets = THPVariable_Unpack(args[5]);
+    const int64_t e = w.size(0);
+    if (e < 1 || e > kMaxSize || (e > 1 && w.stride(0) != n * ldw) || !scales_of(sw, {e, (n + 127) / 128, g}) || !vector_of(table, at::kInt) || !vector_of(offsets, at::kInt) ||
+        table.size(0) < 1 || table.size(0) > 1024 || offsets.size(0) != table.size(0) + 1)
+      Py_RETURN_NONE;
+  } else if (!scales_of(sw, {(n + 127) / 128, g})) {
+    Py_RETURN_NONE;
+  }
+  at::Tensor out;
+  int rc;
+  {
+    Released released;
+    out = fresh({m, n}, type, a);
+    if (experts)
+      rc = ops.matmul_fp8_experts(a.data_ptr(), lda, sa.data_ptr(), (int)m, w.data_ptr(), ldw, sw.data_ptr(), (int)w.size(0), table.data_ptr(), offsets.data_ptr(), (int)table.size(0),
+                                  (int)n, (int)k, out.data_ptr(), dtype_code(type), n, 1, stream());
+    else
+      rc = ops.matmul_fp8(a.data_ptr(), lda, sa.data_ptr(), w.data_ptr(), ldw, sw.data_ptr(), (int)m, (int)n, (int)k, out.data_ptr(), dtype_code(type), n, stream());
+  }
+  return rc ? PyLong_FromLong(rc) : THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+PyObject* py_matmul_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 5) Py_RETURN_NONE;
+  return matmul(args, false);
+}
+PyObject* py_matmul_fp8_experts(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 7) Py_RETURN_NONE;
+  return matmul(args, true);
+}
+
 PyMethodDef methods[] = {{"bind", (PyCFunction)(void (*)(void))py_bind, METH_FASTCALL, nullptr},
                          {"quantize_own_scale", (PyCFunction)(void (*)(void))py_quantize_own_scale, METH_FASTCALL, nullptr},
                          {"quantize_128x4", (PyCFunction)(void (*)(void))py_quantize_128x4, METH_FASTCALL, nullptr},
+                         {"bind_ops", (PyCFunction)(void (*)(void))py_bind_ops, METH_FASTCALL, nullptr},
+                         {"top_k_gate", (PyCFunction)(void (*)(void))py_top_k_gate, METH_FASTCALL, nullptr},
+                         {"balance_loss", (PyCFunction)(void (*)(void))py_balance_loss, METH_FASTCALL, nullptr},
+                         {"quantize_fp8", (PyCFunction)(void (*)(void))py_quantize_fp8, METH_FASTCALL, nullptr},
+                         {"matmul_fp8", (PyCFunction)(void (*)(void))py_matmul_fp8, METH_FASTCALL, nullptr},
+                         {"matmul_fp8_experts", (PyCFunction)(void (*)(void))py_matmul_fp8_experts, METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -33,6 +33,9 @@ def quantize_fp8(x: torch.Tensor, src_row: torch.Tensor | None = None):
     scale = amax / 448, codes = x * (448 / amax) to nearest, amax at least 1e-12. With `src_row` (int32 [R]) row r is x[src_row[r]], which lays tokens out in runs per
     expert without a separate gather; an index outside x gives zero codes and scales. Rows of the codes start on 16 bytes: for K that is no multiple of 16
     they are further apart than K. A NaN makes its group NaN; with an infinity the group's scale is inf."""
+    out = (_lib._host or _lib.host()).quantize_fp8(x, src_row)      # plain tensors in one native call (csrc/host.cpp), else None
+    if out is not None:
+        return out if type(out) is tuple else _lib.check(out, "quantize_fp8")
     if x.dim() != 2 or x.shape[1] < 1:
         raise ValueError(f"expected [M, K] with K >= 1, got {tuple(x.shape)}")
     if x.dtype not in _lib.DTYPES:
@@ -111,6 +114,10 @@ def matmul_fp8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale:
                out: torch.Tensor | None = None) -> torch.Tensor:
     """a [M, K] x w [N, K]^T -> [M, N] in out_dtype (bf16 where neither it nor `out` says; fp16, fp32), for one row to many: codes and scales as quantize_fp8 (a) and
     quantize_fp8_weight (w) give them, any M, N and K >= 1. Products are exact, sums fp32, rounded once. `out` may be a view whose rows are apart."""
+    if out is None:
+        new = (_lib._host or _lib.host()).matmul_fp8(a, a_scale, w, w_scale, out_dtype or torch.bfloat16)      # (as in quantize_fp8)
+        if new is not None:
+            return new if type(new) is not int else _lib.check(new, "matmul_fp8")
     if a.dim() != 2 or w.dim() != 2 or a.shape[1] != w.shape[1] or a.shape[1] < 1:
         raise ValueError(f"matmul_fp8: expected [M, K] and [N, K] with K >= 1, got {tuple(a.shape)} and {tuple(w.shape)}")
     lda, ldw = _row_stride(a, "matmul_fp8", "a"), _row_stride(w, "matmul_fp8", "w")
@@ -130,6 +137,10 @@ def matmul_fp8_experts(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, 
     gives them (ascending offsets, at most 1024 runs; -1 and empty runs where fewer experts have rows). Types and arithmetic as in matmul_fp8. Rows outside
     every run, and those of an expert outside 0..E-1, are zeros; in an `out` that was given they are left as they were."""
     what = "matmul_fp8_experts"
+    if out is None:
+        new = (_lib._host or _lib.host()).matmul_fp8_experts(a, a_scale, w, w_scale, experts, offsets, out_dtype or torch.bfloat16)      # (as in quantize_fp8)
+        if new is not None:
+            return new if type(new) is not int else _lib.check(new, what)
     if a.dim() != 2 or w.dim() != 3 or a.shape[1] != w.shape[2] or a.shape[1] < 1 or w.shape[0] < 1:
         raise ValueError(f"{what}: expected [P, K] and [E, N, K] with K >= 1, got {tuple(a.shape)} and {tuple(w.shape)}")
     lda, ldw = _row_stride(a, what, "a"), _row_stride(w, what, "w")

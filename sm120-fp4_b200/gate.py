@@ -63,6 +63,9 @@ def top_k_gate(logits: torch.Tensor, top_k: int, renormalize: bool = True):
     the lowest index) and their softmax probabilities, divided by their sum where `renormalize`. Up to 512 experts and 16 of them a token; rows may be any
     stride apart. A logit of -inf is an expert that may not be taken: a slot for which none is left gets id -1 (an empty slot of the layer calls) and weight 0. A NaN
     ranks above all numbers and makes its token's weights NaN. Differentiable with respect to the logits through the weights."""
+    out = (_lib._host or _lib.host()).top_k_gate(logits, top_k, renormalize)      # plain tensors in one native call (csrc/host.cpp), else None
+    if out is not None:
+        return out if type(out) is tuple else _lib.check(out, "top_k_gate")
     top_k = int(top_k)
     logits = _logits(logits, "top_k_gate")
     if not 1 <= top_k <= min(MAX_TOP_K, logits.shape[1]):
@@ -77,30 +80,30 @@ def _balance(logits: torch.Tensor, ids: torch.Tensor):
     h = _lib.lib()
     nbytes = h.b200moe_balance_workspace_bytes(tokens, e)
     ws = torch.empty(max(nbytes, 4), dtype=torch.uint8, device=logits.device)
-    sums = torch.empty(3, dtype=torch.float32, device=logits.device)      # the loss, and what the backward pass reads
+    loss, stats = torch.empty((), dtype=torch.float32, device=logits.device), torch.empty(2, dtype=torch.float32, device=logits.device)
     counts = torch.empty(e, dtype=torch.int32, device=logits.device)
     _lib.call(logits.device, "balance_loss", h.b200moe_balance_loss, logits.data_ptr(), _lib.DTYPES[logits.dtype], max(logits.stride(0), e), tokens, e, ids.data_ptr(),
-              ids.shape[1], sums.data_ptr(), counts.data_ptr(), sums.data_ptr() + 4, ws.data_ptr(), nbytes)
-    return sums, counts
+              ids.shape[1], loss.data_ptr(), counts.data_ptr(), stats.data_ptr(), ws.data_ptr(), nbytes)
+    return loss, counts, stats
 
 
 class _Balance(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, ids):
-        sums, counts = _balance(logits, ids)
+        loss, counts, stats = _balance(logits, ids)
         ctx.mark_non_differentiable(counts)
-        ctx.save_for_backward(logits, ids, sums, counts)
-        return sums[0].clone(), counts
+        ctx.save_for_backward(logits, ids, counts, stats)
+        return loss, counts
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad, _):
-        logits, ids, sums, counts = ctx.saved_tensors
+        logits, ids, counts, stats = ctx.saved_tensors
         tokens, e = logits.shape
         out = torch.empty((tokens, e), dtype=logits.dtype, device=logits.device)
         grad = grad.contiguous()
         _lib.call(out.device, "balance_loss backward", _lib.lib().b200moe_balance_backward, grad.data_ptr(), logits.data_ptr(), _lib.DTYPES[logits.dtype],
-                  max(logits.stride(0), e), tokens, e, ids.data_ptr(), ids.shape[1], counts.data_ptr(), sums.data_ptr() + 4, out.data_ptr())
+                  max(logits.stride(0), e), tokens, e, ids.data_ptr(), ids.shape[1], counts.data_ptr(), stats.data_ptr(), out.data_ptr())
         return out, None
 
 
@@ -109,6 +112,9 @@ def balance_loss(logits: torch.Tensor, ids: torch.Tensor):
     loss = E * sum_e f_e P_e with f_e expert e's share of all pairs and P_e the mean over tokens of softmax(logits)_e; it is 1 where experts are used
     evenly. counts are the pairs of each expert. An id outside 0..E-1 is an empty slot, and a token of empty slots alone (padding) counts nowhere; without any
     live token the loss is 0. Differentiable with respect to the logits through P (f is a count). k up to 32, experts up to 512."""
+    out = (_lib._host or _lib.host()).balance_loss(logits, ids)      # (as in top_k_gate)
+    if out is not None:
+        return out if type(out) is tuple else _lib.check(out, "balance_loss")
     logits = _logits(logits, "balance_loss")
     if ids.dtype != torch.int32:
         raise TypeError(f"balance_loss takes int32 ids, not {ids.dtype}")
@@ -118,5 +124,4 @@ def balance_loss(logits: torch.Tensor, ids: torch.Tensor):
     ids = ids.contiguous()
     if logits.requires_grad and torch.is_grad_enabled():
         return _Balance.apply(logits, ids)
-    sums, counts = _balance(logits, ids)
-    return sums[0], counts
+    return _balance(logits, ids)[:2]
