@@ -7,6 +7,7 @@
 // expert that may not be taken: a slot for which none is left gets id -1 (an empty slot of the layer) and weight 0.
 #include "common.cuh"
 #include "fp8_math.cuh"
+#include "tcgen05.cuh"
 #include <type_traits>
 
 namespace b200 {
@@ -181,13 +182,15 @@ __global__ void __launch_bounds__(256) k_gate_backward(const float* __restrict__
 // launch adds the blocks in order. part: per block E floats, E ints, live tokens.
 __host__ __device__ inline int balance_words(int E) { return 2 * E + 4; }
 
+constexpr int kBalanceWarps = 16, kBalanceRanks = 8;
+
 template <typename T, int V, bool kVec>
-__global__ void __launch_bounds__(256) k_balance_part(const T* __restrict__ logits, long long stride, int tokens, int E, const int* __restrict__ ids, int k,
-                                                      float* __restrict__ part) {
-  __shared__ float sp[8][GATE_MAXE];
-  __shared__ int cnt[GATE_MAXE], live_n;
+__global__ void __launch_bounds__(kBalanceWarps * 32) k_balance_part(const T* __restrict__ logits, long long stride, int tokens, int E, const int* __restrict__ ids, int k,
+                                                                     float* __restrict__ part) {
+  __shared__ float sp[kBalanceWarps][32 * V];
+  __shared__ int cnt[32 * V], live_n;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int i = threadIdx.x; i < GATE_MAXE; i += 256) cnt[i] = 0;
+  for (int i = threadIdx.x; i < 32 * V; i += kBalanceWarps * 32) cnt[i] = 0;
   if (threadIdx.x == 0) live_n = 0;
   __syncthreads();
   grid_dependency_wait();
@@ -195,14 +198,14 @@ __global__ void __launch_bounds__(256) k_balance_part(const T* __restrict__ logi
 #pragma unroll
   for (int j = 0; j < V; ++j) acc[j] = 0.f;
   int n = 0;
-  for (int t = blockIdx.x * 8 + warp; t < tokens; t += gridDim.x * 8) {
+  for (int t = blockIdx.x * kBalanceWarps + warp; t < tokens; t += gridDim.x * kBalanceWarps) {
     const int e = lane < k ? ids[(long long)t * k + lane] : -1;
+    float x[V], p[V];
+    load_row<T, V, kVec>(logits + (long long)t * stride, E, lane, x, -INFINITY);
     const bool used = e >= 0 && e < E;
     if (used) atomicAdd(&cnt[e], 1);
     if (!__any_sync(0xffffffffu, used)) continue;      // an empty token
     ++n;
-    float x[V], p[V];
-    load_row<T, V, kVec>(logits + (long long)t * stride, E, lane, x, -INFINITY);
     const float s = softmax_terms<V>(x, p);
     const float r = s == 0.f ? 0.f : 1.f / s;
 #pragma unroll
@@ -210,59 +213,79 @@ __global__ void __launch_bounds__(256) k_balance_part(const T* __restrict__ logi
   }
   if (lane == 0 && n) atomicAdd(&live_n, n);
 #pragma unroll
-  for (int j = 0; j < V; ++j)
-    if (lane * V + j < GATE_MAXE) sp[warp][lane * V + j] = acc[j];
+  for (int j = 0; j < V; ++j) sp[warp][lane * V + j] = acc[j];
   __syncthreads();
   float* o = part + (long long)blockIdx.x * balance_words(E);
-  for (int e = threadIdx.x; e < E; e += 256) {
+  for (int e = threadIdx.x; e < E; e += kBalanceWarps * 32) {
     float s = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s += sp[i][e];
+    for (int i = 0; i < kBalanceWarps; ++i) s += sp[i][e];
     o[e] = s;
     reinterpret_cast<int*>(o)[E + e] = cnt[e];
   }
   if (threadIdx.x == 0) reinterpret_cast<int*>(o)[2 * E] = live_n;
 }
 
-// stats: f32 [2]: 1 / pairs, E / live tokens (0 without any)
-__global__ void __launch_bounds__(GATE_MAXE) k_balance_sum(const float* __restrict__ part, int blocks, int E, float* __restrict__ loss, int* __restrict__ counts, float* __restrict__ stats) {
-  __shared__ double red[GATE_MAXE / 32];
-  __shared__ long long reds[GATE_MAXE / 32];
+// One cluster: a block takes an eighth of the experts, its threads eight shares of the partial sums (loads of eight in flight); the sums of the
+// experts meet in block 0. stats: f32 [2]: 1 / pairs, E / live tokens (the larger of it and 1 in both quotients).
+__global__ void __cluster_dims__(kBalanceRanks, 1, 1) __launch_bounds__(512)
+    k_balance_sum(const float* __restrict__ part, int blocks, int E, float* __restrict__ loss, int* __restrict__ counts, float* __restrict__ stats) {
+  __shared__ double sp[8][64];
+  __shared__ int sc[8][64];
+  __shared__ double rank_v[kBalanceRanks];      // of block 0: every block's sum of products
+  __shared__ long long rank_n[kBalanceRanks];
   __shared__ int live_s;
-  const int e = threadIdx.x, W = balance_words(E);
+  const int tid = threadIdx.x, col = tid & 63, slice = tid >> 6, rank = blockIdx.x;
+  const int per = (E + kBalanceRanks - 1) / kBalanceRanks, e = rank * per + col;
+  const long long W = balance_words(E);
   grid_dependency_wait();
   double p = 0.0;
   int c = 0;
-  if (e < E) {
-    for (int b0 = 0; b0 < blocks; b0 += 8) {
+  const bool mine = col < per && e < E;
+  if (mine) {
+    for (int b0 = slice; b0 < blocks; b0 += 64) {
       float pv[8];
       int cv[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const bool in = b0 + i < blocks;
-        pv[i] = in ? part[(long long)(b0 + i) * W + e] : 0.f;
-        cv[i] = in ? reinterpret_cast<const int*>(part)[(long long)(b0 + i) * W + E + e] : 0;
+        const int b = b0 + 8 * i;
+        pv[i] = b < blocks ? part[b * W + e] : 0.f;
+        cv[i] = b < blocks ? reinterpret_cast<const int*>(part)[b * W + E + e] : 0;
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) p += (double)pv[i], c += cv[i];
     }
-    counts[e] = c;
   }
-  if (e < 32) {
+  sp[slice][col] = p, sc[slice][col] = c;
+  if (rank == 0 && tid < 32) {
     int l = 0;
-    for (int b = e; b < blocks; b += 32) l += reinterpret_cast<const int*>(part)[(long long)b * W + 2 * E];
+    for (int b = tid; b < blocks; b += 32) l += reinterpret_cast<const int*>(part)[b * W + 2 * E];
     l = __reduce_add_sync(0xffffffffu, l);
-    if (e == 0) live_s = l;
+    if (tid == 0) live_s = l;
   }
-  double v = p * (double)c;
-  long long n = c;
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o), n += __shfl_xor_sync(0xffffffffu, n, o);
-  if ((e & 31) == 0) red[e >> 5] = v, reds[e >> 5] = n;
   __syncthreads();
-  if (e == 0) {
-    v = 0.0, n = 0;
-    for (int i = 0; i < (int)(blockDim.x >> 5); ++i) v += red[i], n += reds[i];
+  if (tid < 64) {
+#pragma unroll
+    for (int i = 1; i < 8; ++i) p += sp[i][tid], c += sc[i][tid];
+    if (mine) counts[e] = c;
+    double v = p * (double)c;
+    long long n = c;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o), n += __shfl_xor_sync(0xffffffffu, n, o);
+    if (tid == 32) sp[0][0] = v, sc[1][0] = (int)n, sc[2][0] = (int)(n >> 32);
+    named_bar_sync(1, 64);
+    if (tid == 0) {
+      v += sp[0][0], n += (long long)(((unsigned long long)(unsigned)sc[2][0] << 32) | (unsigned)sc[1][0]);
+      asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(mapa_shared(smem_u32(&rank_v[rank]), 0)), "d"(v) : "memory");
+      asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(mapa_shared(smem_u32(&rank_n[rank]), 0)), "l"(n) : "memory");
+    }
+  }
+  __syncwarp();
+  cluster_sync_all();
+  if (rank == 0 && tid == 0) {
+    double v = 0.0;
+    long long n = 0;
+    for (int i = 0; i < kBalanceRanks; ++i) v += rank_v[i], n += rank_n[i];
     const double live = live_s ? (double)live_s : 1.0, pairs = n ? (double)n : 1.0;
     *loss = (float)((double)E * v / (live * pairs));
     stats[0] = (float)(1.0 / pairs), stats[1] = (float)((double)E / live);
@@ -319,8 +342,8 @@ static bool vec_rows(const void* p, long long stride, int E, int size) {      //
   return ((uintptr_t)p % unit) == 0 && (stride * size) % unit == 0 && ((long long)E * size) % unit == 0;
 }
 static int balance_blocks(int tokens) {
-  const int want = (tokens + 7) / 8;
-  return want < 592 ? want : 592;
+  const int want = (tokens + kBalanceWarps - 1) / kBalanceWarps;
+  return want < 296 ? want : 296;
 }
 
 }  // namespace b200
@@ -393,13 +416,13 @@ int b200moe_balance_loss(const void* logits, int dtype, long long stride, int to
       const T* lp = (const T*)logits;
       void* args[] = {&lp, &stride, &tokens, &E, &ids, &k, &part};
       const void* fn = vec_rows(logits, stride, E, sizeof(T)) ? (const void*)k_balance_part<T, V, true> : (const void*)k_balance_part<T, V, false>;
-      return launch_kernel(fn, blocks, 256, 0, true, args, (cudaStream_t)stream);
+      return launch_kernel(fn, blocks, kBalanceWarps * 32, 0, true, args, (cudaStream_t)stream);
     });
   });
   if (rc) return rc;
   const float* cp = part;
   void* args[] = {&cp, &blocks, &E, &loss, &counts, &stats};
-  return launch_kernel((const void*)k_balance_sum, 1, (E + 31) & ~31, 0, true, args, (cudaStream_t)stream);
+  return launch_kernel((const void*)k_balance_sum, kBalanceRanks, 512, 0, true, args, (cudaStream_t)stream);
 }
 
 int b200moe_balance_backward(const float* grad_loss, const void* logits, int dtype, long long stride, int tokens, int E, const int* ids, int k, const int* counts,

@@ -34,6 +34,13 @@ __device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint32_t a_lo, uint32_t
       ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(pred), "n"(kDescHiSw128)
       : "memory");
 }
+__device__ __forceinline__ void umma2_f8(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate, uint32_t pred) {
+  asm volatile(
+      "{\n .reg .pred p, q;\n .reg .b64 a, b;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n mov.b64 a, {%1, %6};\n mov.b64 b, {%2, %6};\n"
+      " @q tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], a, b, %3, p;\n}\n"
+      ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(pred), "n"(kDescHiSw128)
+      : "memory");
+}
 // Instruction descriptor of kind::f8f6f4: fp32 accumulator (1 at bit 4), E4M3 operands (0), both K-major, N >> 3 at bit 17, M >> 4 at bit 24.
 __host__ __device__ constexpr uint32_t idesc_f8(int M, int N) { return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24); }
 
@@ -44,32 +51,88 @@ __device__ __forceinline__ void tma_load_2d_u32(uint32_t dst, const CUtensorMap*
       ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar), "r"(pred)
       : "memory");
 }
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+// The same for a CTA pair: the copy lands in this CTA's shared memory and its bytes count at a barrier of either CTA (a cluster address).
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar, uint32_t pred) {
+  asm volatile(
+      "{\n .reg .pred q;\n setp.ne.b32 q, %5, 0;\n"
+      " @q cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n}\n"
+      ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar), "r"(pred)
+      : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {      // a barrier of any CTA of the cluster
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// mbar_wait_warp for two barriers at once (one vote), what came before their arrivals in the whole cluster visible
+__device__ __forceinline__ bool mbar_wait_both(uint32_t bar0, uint32_t parity0, uint32_t bar1, uint32_t parity1, volatile int* abort_flag, uint32_t limit = (1u << 20)) {
+  for (uint32_t it = 0; it < limit; ++it) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p, q;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 q, [%3], %4;\n"
+        " and.pred p, p, q;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(bar0), "r"(parity0), "r"(bar1), "r"(parity1)
+        : "memory");
+    if (__all_sync(0xffffffffu, ok != 0)) return true;
+    if ((it & 63u) == 63u && __any_sync(0xffffffffu, *abort_flag != 0)) return false;
+  }
+  *abort_flag = 1;
+  return false;
+}
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
   return v;
 }
+__device__ __forceinline__ void tmem_ld_32x32b_x32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]),
+        "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+template <int C> __device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&r)[C]) {
+  if constexpr (C == 32) tmem_ld_32x32b_x32(taddr, r);
+  else tmem_ld_32x32b_x16(taddr, r);
+}
+// a pair of fp32 fma in one instruction, each rounded as fmaf
+__device__ __forceinline__ void fma2(float& a0, float& a1, uint32_t x0, uint32_t x1, float s0, float s1) {
+  asm("{\n .reg .b64 a, x, s;\n mov.b64 a, {%0, %1};\n mov.b64 x, {%2, %3};\n mov.b64 s, {%4, %5};\n fma.rn.f32x2 a, x, s, a;\n mov.b64 {%0, %1}, a;\n}\n"
+      : "+f"(a0), "+f"(a1) : "r"(x0), "r"(x1), "f"(s0), "f"(s1));
+}
+template <int R> __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R)); }
+template <int R> __device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R)); }
 
-template <int NT, bool kSwap> struct MmShape {
+template <int NT, bool kSwap, bool kPair> struct MmShape {
   static constexpr int kEpi = NT >= 128 ? 8 : 4;                  // epilogue warps: two per lane quadrant where a thread's columns would be more than 64 (128: kSwap false)
   static constexpr int kCols = NT / (kEpi / 4);                   // columns of a thread
-  static constexpr int kThreads = (kEpi + 3) * 32;
-  static constexpr int kStageBytes = 16384 + NT * 128;
+  static constexpr int kChunk = kCols < 32 ? kCols : 32;          // columns of a TMEM load
+  // 128 sums and 64 values in flight a thread: registers go from the other warps (a warpgroup of four, one idle) to the epilogue. A launch of 12 warps has
+  // 168 a thread: 8 * 216 + 4 * 72 = 12 * 168.
+  static constexpr bool kSplitRegs = kCols == 128;
+  static constexpr int kThreads = kSplitRegs ? 384 : (kEpi + 3) * 32;
+  static constexpr int kBRows = kPair ? NT / 2 : NT;              // rows of the B operand in this CTA's shared memory
+  static constexpr int kStageBytes = 16384 + kBRows * 128;
   static constexpr int kRed = kSwap ? NT * 128 * 4 : 0;           // sums of a split inner size
-  static constexpr int kStages = (200 * 1024 - kRed) / kStageBytes < 9 ? (200 * 1024 - kRed) / kStageBytes : 9;
+  static constexpr int kOut = kSwap ? 0 : kEpi * 2048;            // a warp's 32 rows x 64 bytes on their way out
+  static constexpr int kStages = (196 * 1024 - kRed) / kStageBytes < 9 ? (196 * 1024 - kRed) / kStageBytes : 9;
   static constexpr int kBufs = 512 / NT < 8 ? 512 / NT : 8;       // accumulators in TMEM
   static constexpr int kScaleRow = kSwap ? NT : 132;              // floats of a group's scales
-  static constexpr int kRows = kSwap ? NT : 128, kWeights = kSwap ? 128 : NT;      // of a tile
-  static constexpr int kSmem = 1024 + kStages * kStageBytes + kRed + kBufs * kScaleRow * 4 + 2 * (MM_MAXU + 2) * 4;
-  static_assert(kSmem <= 227 * 1024, "shared memory of a CTA");
+  static constexpr int kRows = kSwap ? NT : kPair ? 256 : 128, kWeights = kSwap ? 128 : NT;      // of a tile
+  static constexpr int kSmem = 1024 + kStages * kStageBytes + kRed + kOut + kBufs * kScaleRow * 4 + 2 * (MM_MAXU + 2) * 4;
+  static_assert(kSmem <= 226 * 1024, "shared memory of a CTA");
 };
 
 struct MmTile { int row0, row_end, expert, n0; };
 
 // The t-th tile: row tiles of a run and weight block side by side, so that neighbours share the weights.
-template <int NT, bool kSwap>
+template <int NT, bool kSwap, bool kPair>
 __device__ __forceinline__ MmTile mm_tile(const MatmulParams& p, const int* first, const int* off, int t) {
-  using S = MmShape<NT, kSwap>;
+  using S = MmShape<NT, kSwap, kPair>;
   int u = 0, begin = 0, end = p.M, e = 0;
   if (p.offsets) {
     int lo = 0, hi = p.U;                          // the last run whose first tile is at most t
@@ -89,24 +152,95 @@ template <int DT> __device__ __forceinline__ void put(void* out, long long i, fl
   else if constexpr (DT == DT_F16) reinterpret_cast<__half*>(out)[i] = __float2half_rn(v);
   else reinterpret_cast<float*>(out)[i] = v;
 }
-// n consecutive values (the whole count where vec: 16-byte stores) of a row
-template <int DT, int C> __device__ __forceinline__ void put_row(void* out, long long at, const float (&v)[C], int n, bool vec) {
-  if (vec && n >= C) {
-    if constexpr (DT == DT_F32) {
-      float4* o = reinterpret_cast<float4*>(reinterpret_cast<float*>(out) + at);
+// n values of a row, one at a time
+template <int DT, int C> __device__ __forceinline__ void put_some(void* out, long long at, const float (&v)[C], int n) {
 #pragma unroll
-      for (int i = 0; i < C / 4; ++i) o[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-    } else {
-      using T = std::conditional_t<DT == DT_BF16, __nv_bfloat16, __half>;
-      uint4* o = reinterpret_cast<uint4*>(reinterpret_cast<T*>(out) + at);
+  for (int i = 0; i < C; ++i)
+    if (i < n) put<DT>(out, at + i, v[i]);
+}
+// A warp's 32 rows x 128 columns (a row a thread) to the output, by way of 32 x 64 bytes of shared memory, so that a store instruction writes 64 bytes of
+// eight rows instead of 16 bytes of 32: a tile's stores took 5900 cycles without. 16-byte chunks are placed by (row >> 1) & 3, free of bank conflicts.
+template <int DT> __device__ __forceinline__ void put_rows(const MatmulParams& p, uint8_t* buf, const float (&acc)[128], int row0, int row_end, int n, int lane) {
+  constexpr int kSize = DT == DT_F32 ? 4 : 2, kStep = 64 / kSize;      // columns of a round
+  if (!p.vec) {
+    const int row = row0 + lane;
 #pragma unroll
-      for (int i = 0; i < C / 8; ++i)
-        o[i] = make_uint4(Elem<T>::pack(v[8 * i], v[8 * i + 1]), Elem<T>::pack(v[8 * i + 2], v[8 * i + 3]), Elem<T>::pack(v[8 * i + 4], v[8 * i + 5]), Elem<T>::pack(v[8 * i + 6], v[8 * i + 7]));
+    for (int i = 0; i < 128; ++i)
+      if (row < row_end && n + i < p.N) put<DT>(p.out, (long long)row * p.ldo + n + i, acc[i]);
+    return;
+  }
+#pragma unroll
+  for (int c0 = 0; c0 < 128; c0 += kStep) {
+    if (n + c0 >= p.N) break;
+    __syncwarp();
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      uint4 w;
+      const float* v = acc + c0 + q * kStep / 4;
+      if constexpr (DT == DT_F32) {
+        w = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+      } else {
+        using T = std::conditional_t<DT == DT_BF16, __nv_bfloat16, __half>;
+        w = make_uint4(Elem<T>::pack(v[0], v[1]), Elem<T>::pack(v[2], v[3]), Elem<T>::pack(v[4], v[5]), Elem<T>::pack(v[6], v[7]));
+      }
+      *reinterpret_cast<uint4*>(buf + lane * 64 + ((q ^ (lane >> 1 & 3)) << 4)) = w;
     }
-  } else {
+    __syncwarp();
 #pragma unroll
-    for (int i = 0; i < C; ++i)
-      if (i < n) put<DT>(out, at + i, v[i]);
+    for (int i = 0; i < 4; ++i) {
+      const int r = i * 8 + lane / 4, q = lane & 3, row = row0 + r, col = n + c0 + q * (kStep / 4);
+      const uint4 w = *reinterpret_cast<const uint4*>(buf + r * 64 + ((q ^ (r >> 1 & 3)) << 4));
+      if (row < row_end) {
+        uint8_t* o = reinterpret_cast<uint8_t*>(p.out) + ((long long)row * p.ldo + col) * kSize;
+        if (col + kStep / 4 <= p.N) {
+          *reinterpret_cast<uint4*>(o) = w;
+        } else {
+          const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int j = 0; j < 16 / kSize; ++j)
+            if (col + j < p.N) {
+              if constexpr (kSize == 4) reinterpret_cast<uint32_t*>(o)[j] = x[j];
+              else reinterpret_cast<uint16_t*>(o)[j] = (uint16_t)(x[j / 2] >> (16 * (j & 1)));
+            }
+        }
+      }
+    }
+  }
+}
+// This CTA's share of a tile whose inner size is split: 1 / kRanks of it, the sums of all ranks, added in rank order. A thread takes four weights of a row at a
+// time; all of its loads from the ranks' shared memory are in flight together.
+template <int NT, int kRanks>
+__device__ __forceinline__ void mm_add_ranks(const MatmulParams& p, const MmTile& tl, const float* red, int rank, int tid) {
+  using S = MmShape<NT, true, false>;
+  constexpr int kThreads = S::kEpi * 32, kItems = NT * 32 / kRanks, kEach = (kItems + kThreads - 1) / kThreads;
+  float4 v[kEach][kRanks];
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    const int i = tid + j * kThreads;
+    if (kItems % kThreads == 0 || i < kItems) {
+      const uint32_t mine = smem_u32(red) + (rank * kItems + i) * 16;
+#pragma unroll
+      for (int r = 0; r < kRanks; ++r) v[j][r] = ld_cluster_f32x4(mapa_shared(mine, r));
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    const int i = tid + j * kThreads, at4 = rank * kItems + i, row = tl.row0 + at4 / 32, n = tl.n0 + (at4 & 31) * 4;
+    if ((kItems % kThreads && i >= kItems) || row >= tl.row_end || n >= p.N) continue;
+    float o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int r = 0; r < kRanks; ++r) o[0] += v[j][r].x, o[1] += v[j][r].y, o[2] += v[j][r].z, o[3] += v[j][r].w;
+    const long long at = (long long)row * p.ldo + n;
+    if (p.out_dtype == DT_F32) {
+      if (p.vec && n + 4 <= p.N) *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + at) = make_float4(o[0], o[1], o[2], o[3]);
+      else put_some<DT_F32>(p.out, at, o, p.N - n);
+    } else if (p.out_dtype == DT_BF16) {
+      if (p.vec && n + 4 <= p.N) *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(p.out) + at) = make_uint2(Elem<__nv_bfloat16>::pack(o[0], o[1]), Elem<__nv_bfloat16>::pack(o[2], o[3]));
+      else put_some<DT_BF16>(p.out, at, o, p.N - n);
+    } else {
+      if (p.vec && n + 4 <= p.N) *reinterpret_cast<uint2*>(reinterpret_cast<__half*>(p.out) + at) = make_uint2(Elem<__half>::pack(o[0], o[1]), Elem<__half>::pack(o[2], o[3]));
+      else put_some<DT_F16>(p.out, at, o, p.N - n);
+    }
   }
 }
 __device__ __forceinline__ void zero_rows(const MatmulParams& p, int r0, int r1, int first, int step) {
@@ -122,17 +256,18 @@ __device__ __forceinline__ void zero_rows(const MatmulParams& p, int r0, int r1,
   }
 }
 
-template <int NT, bool kSwap>
-__global__ void __launch_bounds__(MmShape<NT, kSwap>::kThreads, 1)
+template <int NT, bool kSwap, bool kPair>
+__global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
     k_matmul_fp8(const __grid_constant__ CUtensorMap map_rows, const __grid_constant__ CUtensorMap map_weights, const __grid_constant__ MatmulParams p, int split) {
-  using S = MmShape<NT, kSwap>;
+  using S = MmShape<NT, kSwap, kPair>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   float* red = reinterpret_cast<float*>(smem + S::kStages * S::kStageBytes);      // [NT][128]
   float* scales = reinterpret_cast<float*>(smem + S::kStages * S::kStageBytes + S::kRed);
-  int* first = reinterpret_cast<int*>(scales + S::kBufs * S::kScaleRow);
+  uint8_t* outs = reinterpret_cast<uint8_t*>(scales + S::kBufs * S::kScaleRow);
+  int* first = reinterpret_cast<int*>(outs + S::kOut);
   int* off = first + MM_MAXU + 1;
-  __shared__ uint64_t full[S::kStages], empty[S::kStages], acc_full[S::kBufs], acc_empty[S::kBufs], drained;
+  __shared__ uint64_t full[S::kStages], empty[S::kStages], acc_full[S::kBufs], acc_empty[S::kBufs], scale_empty[S::kBufs], drained;
   __shared__ uint32_t tmem_base;
   __shared__ int abort_s, wsum[32];
   volatile int* abort_flag = &abort_s;
@@ -140,15 +275,15 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap>::kThreads, 1)
 
   if (tid == 0) {
     for (int i = 0; i < S::kStages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
-    for (int i = 0; i < S::kBufs; ++i) mbar_init(&acc_full[i], 2), mbar_init(&acc_empty[i], S::kEpi);
+    for (int i = 0; i < S::kBufs; ++i) mbar_init(&acc_full[i], 2), mbar_init(&acc_empty[i], kPair ? 2 * S::kEpi : S::kEpi), mbar_init(&scale_empty[i], S::kEpi);
     mbar_init(&drained, 1);
     abort_s = 0;
     fence_mbar_init();
     prefetch_tensormap(&map_rows), prefetch_tensormap(&map_weights);
   }
   if (warp == S::kEpi + 1) {
-    tmem_alloc(&tmem_base, S::kBufs * NT);
-    tmem_relinquish();
+    if constexpr (kPair) tmem_alloc2(&tmem_base, S::kBufs * NT), tmem_relinquish2();
+    else tmem_alloc(&tmem_base, S::kBufs * NT), tmem_relinquish();
   }
   grid_dependency_wait();
 
@@ -185,26 +320,38 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap>::kThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
+  if constexpr (kPair) cluster_sync_all();      // the peer's barriers and accumulators are there
   tc_fence_after();
   const uint32_t tb = tmem_base;
 
-  const int rank = split > 1 ? (int)cluster_ctarank() : 0;
-  const int t0 = blockIdx.x / split, t_step = gridDim.x / split;
-  const int kb0 = p.KB * rank / split, kb1 = p.KB * (rank + 1) / split;
+  const int ranks = kPair ? 2 : split;
+  const int rank = ranks > 1 ? (int)cluster_ctarank() : 0;
+  const int t0 = blockIdx.x / ranks, t_step = gridDim.x / ranks;
+  const int kb0 = kPair ? 0 : p.KB * rank / split, kb1 = kPair ? p.KB : p.KB * (rank + 1) / split;
+  const int crow = kPair ? rank * 128 : 0;      // this CTA's rows of a pair's tile
   bool dead = false;       // a wait ran out: the rest of the tiles is walked without work, so that the barriers of a cluster still meet
 
+  if (warp >= S::kEpi) {
+  if constexpr (S::kSplitRegs) regs_dec<72>();
   if (warp == S::kEpi) {                                             // ---- TMA producer
     const uint32_t el = elect_one();
     int st = 0, ph = 1, issued = 0;
     for (int t = t0; t < tiles; t += t_step) {
-      const MmTile tl = mm_tile<NT, kSwap>(p, first, off, t);
+      const MmTile tl = mm_tile<NT, kSwap, kPair>(p, first, off, t);
       for (int kb = kb0; kb < kb1 && !dead; ++kb) {
         if (!mbar_wait_warp(smem_u32(&empty[st]), ph, abort_flag)) { dead = true; break; }
         const uint32_t bar = smem_u32(&full[st]), sa = smem_u32(smem + st * S::kStageBytes);
         const int wrow = tl.expert * p.N + tl.n0;
-        mbar_expect_tx_u32(bar, S::kStageBytes, el);
-        tma_load_2d_u32(kSwap ? sa + 16384 : sa, &map_rows, kb * 128, tl.row0, bar, el);
-        tma_load_2d_u32(kSwap ? sa : sa + 16384, &map_weights, kb * 128, wrow, bar, el);
+        if constexpr (kPair) {      // each CTA brings its half of both operands; the bytes of both count at the leader's barrier
+          const uint32_t lead = mapa_shared(bar, 0);
+          mbar_expect_tx_u32(bar, 2 * S::kStageBytes, el & (rank == 0));
+          tma_load_2d_pair(sa, &map_rows, kb * 128, tl.row0 + crow, lead, el);
+          tma_load_2d_pair(sa + 16384, &map_weights, kb * 128, wrow + rank * S::kBRows, lead, el);
+        } else {
+          mbar_expect_tx_u32(bar, S::kStageBytes, el);
+          tma_load_2d_u32(kSwap ? sa + 16384 : sa, &map_rows, kb * 128, tl.row0, bar, el);
+          tma_load_2d_u32(kSwap ? sa : sa + 16384, &map_weights, kb * 128, wrow, bar, el);
+        }
         ++issued;
         if (++st == S::kStages) st = 0, ph ^= 1;
       }
@@ -212,38 +359,49 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap>::kThreads, 1)
     }
     if (dead) {      // copies in flight land before the CTA may end (with a limit)
       for (int i = issued > S::kStages ? issued - S::kStages : 0; i < issued; ++i)
-        for (int n = 0; n < 1 << 16 && !mbar_try_wait(&full[i % S::kStages], (i / S::kStages) & 1); ++n) {}
+        for (int n = 0; n < 1 << 16 && (!kPair || rank == 0) && !mbar_try_wait(&full[i % S::kStages], (i / S::kStages) & 1); ++n) {}
+      if (kPair)
+        for (int n = 0; n < 200; ++n) __nanosleep(1000);      // (a pair's second CTA has no barrier of its own copies)
     }
   } else if (warp == S::kEpi + 1) {                                  // ---- MMA issue
     const uint32_t el = elect_one();
-    constexpr uint32_t idesc = idesc_f8(128, NT);
+    constexpr uint32_t idesc = idesc_f8(kPair ? 256 : 128, NT);
     int st = 0, ph = 0, buf = 0, bph = 1;
     for (int t = t0; t < tiles; t += t_step) {
-      for (int kb = kb0; kb < kb1 && !dead; ++kb) {
-        if (!mbar_wait_warp(smem_u32(&acc_empty[buf]), bph, abort_flag) || !mbar_wait_warp(smem_u32(&full[st]), ph, abort_flag)) { dead = true; break; }
+      for (int kb = kb0; kb < kb1 && !dead && (!kPair || rank == 0); ++kb) {
+        if (!mbar_wait_both(smem_u32(&acc_empty[buf]), bph, smem_u32(&full[st]), ph, abort_flag)) { dead = true; break; }
         tc_fence_after();
         const uint32_t a = ((smem_u32(smem + st * S::kStageBytes) >> 4) & 0x3fff) | kDescLoSw128, b = a + (16384 >> 4);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) umma_f8(tb + buf * NT, a + 2 * j, b + 2 * j, idesc, j != 0, el);
-        umma_commit_u32(smem_u32(&empty[st]), el);
-        umma_commit_u32(smem_u32(&acc_full[buf]), el);
+        for (int j = 0; j < 4; ++j) {
+          if constexpr (kPair) umma2_f8(tb + buf * NT, a + 2 * j, b + 2 * j, idesc, j != 0, el);
+          else umma_f8(tb + buf * NT, a + 2 * j, b + 2 * j, idesc, j != 0, el);
+        }
+        if constexpr (kPair) {
+          umma2_commit_p(&empty[st], 3, el);
+          umma2_commit_p(&acc_full[buf], 3, el);
+        } else {
+          umma_commit_u32(smem_u32(&empty[st]), el);
+          umma_commit_u32(smem_u32(&acc_full[buf]), el);
+        }
         if (++st == S::kStages) st = 0, ph ^= 1;
         if (++buf == S::kBufs) buf = 0, bph ^= 1;
       }
       if (split > 1) __syncwarp(), cluster_sync_all(), cluster_sync_all();
     }
     if (dead) {
-      umma_commit_u32(smem_u32(&drained), el);
-      for (int n = 0; n < 1 << 16 && !mbar_try_wait(&drained, 0); ++n) {}
+      if constexpr (kPair) umma2_commit_p(&drained, 1, el & (rank == 0));
+      else umma_commit_u32(smem_u32(&drained), el);
+      for (int n = 0; n < 1 << 16 && (!kPair || rank == 0) && !mbar_try_wait(&drained, 0); ++n) {}
     }
   } else if (warp == S::kEpi + 2) {                                  // ---- scales: four groups ahead in registers, then a slot beside each accumulator
-    constexpr int R = (S::kRows + 31) / 32;
+    constexpr int kHere = kSwap ? NT : 128, R = (kHere + 31) / 32;
     int buf = 0, bph = 1;
     for (int t = t0; t < tiles; t += t_step) {
-      const MmTile tl = mm_tile<NT, kSwap>(p, first, off, t);
+      const MmTile tl = mm_tile<NT, kSwap, kPair>(p, first, off, t);
       const float* ra[R];
 #pragma unroll
-      for (int i = 0; i < R; ++i) ra[i] = p.sa + (long long)min(tl.row0 + lane + 32 * i, p.M - 1) * p.KB;
+      for (int i = 0; i < R; ++i) ra[i] = p.sa + (long long)min(tl.row0 + crow + lane + 32 * i, p.M - 1) * p.KB;
       const int nb = tl.n0 / 128 + (kSwap ? 0 : lane & 1);
       const float* rb = p.sb + ((long long)tl.expert * p.NB + min(nb, p.NB - 1)) * p.KB;
       float va[4][R], vb[4];
@@ -269,11 +427,11 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap>::kThreads, 1)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           if (kb + j >= kb1) break;
-          if (!mbar_wait_warp(smem_u32(&acc_empty[buf]), bph, abort_flag)) { dead = true; break; }
+          if (!mbar_wait_warp(smem_u32(&scale_empty[buf]), bph, abort_flag)) { dead = true; break; }
           float* s = scales + buf * S::kScaleRow;
 #pragma unroll
           for (int i = 0; i < R; ++i)
-            if (lane + 32 * i < S::kRows) s[lane + 32 * i] = kSwap ? ca[j][i] * cb[j] : ca[j][i];
+            if (lane + 32 * i < kHere) s[lane + 32 * i] = kSwap ? ca[j][i] * cb[j] : ca[j][i];
           if (!kSwap && lane < 2) s[128 + lane] = cb[j];
           __syncwarp();
           if (lane == 0) mbar_arrive(&acc_full[buf]);
@@ -282,12 +440,14 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap>::kThreads, 1)
       }
       if (split > 1) __syncwarp(), cluster_sync_all(), cluster_sync_all();
     }
+  }
   } else {                                                           // ---- epilogue
+    if constexpr (S::kSplitRegs) regs_inc<216>();
     const int quad = warp & 3, half = warp >> 2, col0 = half * S::kCols;
     const int l = quad * 32 + lane;                                  // accumulator lane
     int buf = 0, ph = 0;
     for (int t = t0; t < tiles; t += t_step) {
-      const MmTile tl = mm_tile<NT, kSwap>(p, first, off, t);
+      const MmTile tl = mm_tile<NT, kSwap, kPair>(p, first, off, t);
       float acc[S::kCols];
 #pragma unroll
       for (int i = 0; i < S::kCols; ++i) acc[i] = 0.f;
@@ -296,39 +456,45 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap>::kThreads, 1)
         tc_fence_after();
         const float* s = scales + buf * S::kScaleRow;
         const uint32_t taddr = tb + buf * NT + col0 + ((uint32_t)(quad * 32) << 16);
+        uint32_t v[2][S::kChunk];
+        tmem_ld_cols<S::kChunk>(taddr, v[0]);
         const float sr = kSwap ? 0.f : s[l] * s[128 + half];
-        uint32_t v[2][16];
-        tmem_ld_32x32b_x16(taddr, v[0]);
 #pragma unroll
-        for (int c = 0; c < S::kCols / 16; ++c) {
+        for (int c = 0; c < S::kCols / S::kChunk; ++c) {
           tmem_ld_wait();
-          if (c + 1 < S::kCols / 16) tmem_ld_32x32b_x16(taddr + 16 * (c + 1), v[(c + 1) & 1]);
-#pragma unroll
-          for (int i = 0; i < 16; i += 4) {
-            if constexpr (kSwap) {
-              const float4 sc = *reinterpret_cast<const float4*>(s + col0 + c * 16 + i);
-              acc[c * 16 + i] = fmaf(__uint_as_float(v[c & 1][i]), sc.x, acc[c * 16 + i]);
-              acc[c * 16 + i + 1] = fmaf(__uint_as_float(v[c & 1][i + 1]), sc.y, acc[c * 16 + i + 1]);
-              acc[c * 16 + i + 2] = fmaf(__uint_as_float(v[c & 1][i + 2]), sc.z, acc[c * 16 + i + 2]);
-              acc[c * 16 + i + 3] = fmaf(__uint_as_float(v[c & 1][i + 3]), sc.w, acc[c * 16 + i + 3]);
-            } else {
-#pragma unroll
-              for (int j = 0; j < 4; ++j) acc[c * 16 + i + j] = fmaf(__uint_as_float(v[c & 1][i + j]), sr, acc[c * 16 + i + j]);
+          if (c + 1 < S::kCols / S::kChunk) {
+            tmem_ld_cols<S::kChunk>(taddr + S::kChunk * (c + 1), v[(c + 1) & 1]);
+          } else {      // all of it is in registers: the tensor core may have the accumulator back
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+              if constexpr (kPair) mbar_arrive_cluster(mapa_shared(smem_u32(&acc_empty[buf]), 0));
+              else mbar_arrive(&acc_empty[buf]);
+              if (!kSwap) mbar_arrive(&scale_empty[buf]);
             }
           }
+#pragma unroll
+          for (int i = 0; i < S::kChunk; i += 4) {
+            float* o = acc + c * S::kChunk + i;
+            const uint32_t* x = v[c & 1] + i;
+            float4 sc = make_float4(sr, sr, sr, sr);
+            if constexpr (kSwap) sc = *reinterpret_cast<const float4*>(s + col0 + c * S::kChunk + i);
+            fma2(o[0], o[1], x[0], x[1], sc.x, sc.y);
+            fma2(o[2], o[3], x[2], x[3], sc.z, sc.w);
+          }
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&acc_empty[buf]);
+        if constexpr (kSwap) {      // (the slot's scales are read up to here)
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&scale_empty[buf]);
+        }
         if (++buf == S::kBufs) buf = 0, ph ^= 1;
       }
       if constexpr (!kSwap) {
-        const int row = tl.row0 + l, n = tl.n0 + col0;
-        if (!dead && row < tl.row_end && n < p.N) {
-          const long long at = (long long)row * p.ldo + n;
-          if (p.out_dtype == DT_BF16) put_row<DT_BF16>(p.out, at, acc, p.N - n, p.vec);
-          else if (p.out_dtype == DT_F16) put_row<DT_F16>(p.out, at, acc, p.N - n, p.vec);
-          else put_row<DT_F32>(p.out, at, acc, p.N - n, p.vec);
+        if (!dead) {
+          const int row0 = tl.row0 + crow + quad * 32, n = tl.n0 + col0;
+          if (p.out_dtype == DT_BF16) put_rows<DT_BF16>(p, outs + warp * 2048, acc, row0, tl.row_end, n, lane);
+          else if (p.out_dtype == DT_F16) put_rows<DT_F16>(p, outs + warp * 2048, acc, row0, tl.row_end, n, lane);
+          else put_rows<DT_F32>(p, outs + warp * 2048, acc, row0, tl.row_end, n, lane);
         }
       } else {
         if (split == 1) {
@@ -351,17 +517,9 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap>::kThreads, 1)
           __syncwarp();
           cluster_sync_all();
           if (!dead) {
-            for (int i = tid + rank * S::kEpi * 32; i < NT * 128; i += split * S::kEpi * 32) {
-              const int row = tl.row0 + i / 128, n = tl.n0 + (i & 127);
-              if (row >= tl.row_end || n >= p.N) continue;
-              float v = 0.f;
-              const uint32_t mine = smem_u32(red + i);
-              for (int r = 0; r < split; ++r) v += ld_cluster_f32(mapa_shared(mine, r));
-              const long long at = (long long)row * p.ldo + n;
-              if (p.out_dtype == DT_BF16) put<DT_BF16>(p.out, at, v);
-              else if (p.out_dtype == DT_F16) put<DT_F16>(p.out, at, v);
-              else put<DT_F32>(p.out, at, v);
-            }
+            if (split == 2) mm_add_ranks<NT, 2>(p, tl, red, rank, tid);
+            else if (split == 4) mm_add_ranks<NT, 4>(p, tl, red, rank, tid);
+            else mm_add_ranks<NT, 8>(p, tl, red, rank, tid);
           }
           __syncwarp();
           cluster_sync_all();      // the peers' sums stay until everybody has read them
@@ -381,7 +539,12 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap>::kThreads, 1)
   if (dead) atomicExch(&g_matmul_fp8_status, 1);
   tc_fence_before();
   __syncthreads();
-  if (warp == S::kEpi + 1) tmem_dealloc(tb, S::kBufs * NT);
+  if constexpr (kPair) {
+    cluster_sync_all();      // nobody frees or leaves while the pair's work may still reach it
+    if (warp == S::kEpi + 1) tmem_dealloc2(tb, S::kBufs * NT);
+  } else {
+    if (warp == S::kEpi + 1) tmem_dealloc(tb, S::kBufs * NT);
+  }
 }
 
 static PFN_cuTensorMapEncodeTiled_v12000 map_encoder() {
@@ -411,23 +574,24 @@ static int sm_count() {
   return n;
 }
 
-template <int NT, bool kSwap>
+template <int NT, bool kSwap, bool kPair>
 static int launch_matmul(const MatmulParams& p, const void* a, long long lda, const void* w, long long ldw, long long tiles, int split, int sms, cudaStream_t st) {
-  using S = MmShape<NT, kSwap>;
+  using S = MmShape<NT, kSwap, kPair>;
   CUtensorMap rows, weights;
-  if (int rc = codes_map(&rows, a, p.M, p.K, lda, S::kRows)) return rc;
-  if (int rc = codes_map(&weights, w, (long long)p.E * p.N, p.K, ldw, S::kWeights)) return rc;
-  const void* fn = (const void*)k_matmul_fp8<NT, kSwap>;
+  if (int rc = codes_map(&rows, a, p.M, p.K, lda, kSwap ? NT : 128)) return rc;
+  if (int rc = codes_map(&weights, w, (long long)p.E * p.N, p.K, ldw, kSwap ? 128 : S::kBRows)) return rc;
+  const void* fn = (const void*)k_matmul_fp8<NT, kSwap, kPair>;
   B200_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
-  const long long most = sms / split;
+  const int ranks = kPair ? 2 : split;
+  const long long most = sms / ranks;
   const int clusters = (int)(tiles < most ? (tiles > 0 ? tiles : 1) : most);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(clusters * split), cfg.blockDim = dim3(S::kThreads), cfg.dynamicSmemBytes = S::kSmem, cfg.stream = st;
+  cfg.gridDim = dim3(clusters * ranks), cfg.blockDim = dim3(S::kThreads), cfg.dynamicSmemBytes = S::kSmem, cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization, attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = split, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr, cfg.numAttrs = split > 1 ? 2 : 1;
+  attr[1].val.clusterDim.x = ranks, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr, cfg.numAttrs = ranks > 1 ? 2 : 1;
   MatmulParams q = p;
   void* args[] = {&rows, &weights, &q, &split};
   B200_CUDA_TRY(cudaLaunchKernelExC(&cfg, fn, args));
@@ -441,16 +605,17 @@ static int matmul(const MatmulParams& p, const void* a, long long lda, const voi
   if (sms <= 0) return B200MOE_ERR_DEVICE;
   const long long runs = p.offsets ? (p.U < p.M ? p.U : p.M) : 1, mean = p.M / runs;
   const auto tiles = [&](int r, int c) { return (p.M / r + (p.offsets ? runs : (p.M % r != 0))) * ((p.N + c - 1) / c); };      // (at most)
-  if (mean >= 96 && tiles(128, 256) >= sms / 2) return launch_matmul<256, false>(p, a, lda, w, ldw, tiles(128, 256), 1, sms, st);
+  if (mean >= 256 && tiles(256, 256) >= sms / 2) return launch_matmul<256, false, true>(p, a, lda, w, ldw, tiles(256, 256), 1, sms, st);
+  if (mean >= 96 && tiles(128, 256) >= sms / 2) return launch_matmul<256, false, false>(p, a, lda, w, ldw, tiles(128, 256), 1, sms, st);
   const int nt = mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 64 ? 64 : 128;
   const long long n = tiles(nt, 128);
   int split = 1;
   while (split < 8 && n * split * 2 <= sms && p.KB >= split * 4) split *= 2;
   switch (nt) {
-    case 16: return launch_matmul<16, true>(p, a, lda, w, ldw, n, split, sms, st);
-    case 32: return launch_matmul<32, true>(p, a, lda, w, ldw, n, split, sms, st);
-    case 64: return launch_matmul<64, true>(p, a, lda, w, ldw, n, split, sms, st);
-    default: return launch_matmul<128, true>(p, a, lda, w, ldw, n, split, sms, st);
+    case 16: return launch_matmul<16, true, false>(p, a, lda, w, ldw, n, split, sms, st);
+    case 32: return launch_matmul<32, true, false>(p, a, lda, w, ldw, n, split, sms, st);
+    case 64: return launch_matmul<64, true, false>(p, a, lda, w, ldw, n, split, sms, st);
+    default: return launch_matmul<128, true, false>(p, a, lda, w, ldw, n, split, sms, st);
   }
 }
 

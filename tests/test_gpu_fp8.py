@@ -158,7 +158,7 @@ def operands(m, n, k, seed=0):
 
 
 SIZES = [(1, 1, 1), (1, 4096, 4096), (1, 128, 128), (2, 16, 16), (3, 130, 200), (16, 1536, 2048), (17, 300, 384), (32, 2816, 704), (33, 257, 100), (64, 64, 8192), (65, 129, 640),
-         (100, 4096, 130), (128, 1408, 2816), (129, 100, 512), (200, 2048, 256), (333, 2816, 704), (500, 5001, 300), (1000, 4100, 272), (1024, 4096, 1024), (1300, 7000, 129)]
+         (100, 4096, 130), (128, 1408, 2816), (129, 100, 512), (200, 2048, 256), (333, 2816, 704), (500, 5001, 300), (1000, 4100, 272), (1024, 4096, 1024), (1300, 7000, 129), (2100, 2570, 640), (2048, 2560, 256)]
 
 
 @pytest.mark.parametrize("m,n,k", SIZES)
@@ -244,7 +244,7 @@ def runs_of(counts):
 
 
 @pytest.mark.parametrize("counts,n,k", [([1], 64, 128), ([1, 0, 2, 1], 1536, 256), ([5, 17, 0, 1, 40], 300, 704), ([200, 3, 129, 0, 1], 257, 300), ([0, 0, 0], 64, 64),
-                                        ([16] * 40, 704, 512), ([130, 1, 500, 127, 128, 0, 300, 90], 1408, 640), ([1500], 200, 384), ([2] * 300, 48, 160)])
+                                        ([16] * 40, 704, 512), ([130, 1, 500, 127, 128, 0, 300, 90], 1408, 640), ([1500], 200, 384), ([2] * 300, 48, 160), ([600, 255, 1, 900, 0, 513], 1400, 300)])
 def test_experts(counts, n, k):
     import sm120fp4_b200 as pkg
     e = len(counts) + 2
