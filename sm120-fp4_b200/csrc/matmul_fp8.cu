@@ -59,8 +59,18 @@ __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap
       ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar), "r"(pred)
       : "memory");
 }
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {      // a barrier of any CTA of the cluster
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+// Arrivals of one lane (pred) without a branch. The one at a barrier of any CTA of the cluster orders no memory: what it hands over is TMEM, ordered by the tcgen05
+// fences, and with cluster-wide release it held the epilogue up for 900 cycles.
+__device__ __forceinline__ void mbar_arrive_cluster_p(uint32_t bar, uint32_t pred) {
+  asm volatile("{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n @q mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];\n}\n" ::"r"(bar), "r"(pred) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_p(uint32_t bar, uint32_t pred) {
+  asm volatile("{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n @q mbarrier.arrive.shared::cta.b64 _, [%0];\n}\n" ::"r"(bar), "r"(pred) : "memory");
+}
+__device__ __forceinline__ bool mbar_ready(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  return __all_sync(0xffffffffu, ok != 0);
 }
 // mbar_wait_warp for two barriers at once (one vote), what came before their arrivals in the whole cluster visible
 __device__ __forceinline__ bool mbar_wait_both(uint32_t bar0, uint32_t parity0, uint32_t bar1, uint32_t parity1, volatile int* abort_flag, uint32_t limit = (1u << 20)) {
@@ -107,19 +117,23 @@ __device__ __forceinline__ void fma2(float& a0, float& a1, uint32_t x0, uint32_t
 template <int R> __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R)); }
 template <int R> __device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R)); }
 
+constexpr int kOutRow = 256 + 16;                 // bytes from a row to the next on its way out of a pair's tile: eight lanes' 16-byte stores meet all banks
+
 template <int NT, bool kSwap, bool kPair> struct MmShape {
   static constexpr int kEpi = NT >= 128 ? 8 : 4;                  // epilogue warps: two per lane quadrant where a thread's columns would be more than 64 (128: kSwap false)
   static constexpr int kCols = NT / (kEpi / 4);                   // columns of a thread
   static constexpr int kChunk = kCols < 32 ? kCols : 32;          // columns of a TMEM load
   // 128 sums and 64 values in flight a thread: registers go from the other warps (a warpgroup of four, one idle) to the epilogue. A launch of 12 warps has
-  // 168 a thread: 8 * 216 + 4 * 72 = 12 * 168.
+  // 168 a thread: 8 * 184 + 4 * 136 = 12 * 168.
   static constexpr bool kSplitRegs = kCols == 128;
   static constexpr int kThreads = kSplitRegs ? 384 : (kEpi + 3) * 32;
   static constexpr int kBRows = kPair ? NT / 2 : NT;              // rows of the B operand in this CTA's shared memory
   static constexpr int kStageBytes = 16384 + kBRows * 128;
   static constexpr int kRed = kSwap ? NT * 128 * 4 : 0;           // sums of a split inner size
-  static constexpr int kOut = kSwap ? 0 : kEpi * 2048;            // a warp's 32 rows x 64 bytes on their way out
-  static constexpr int kStages = (196 * 1024 - kRed) / kStageBytes < 9 ? (196 * 1024 - kRed) / kStageBytes : 9;
+  static constexpr int kOutWarp = kSwap ? 0 : kPair ? 32 * kOutRow : 2048;      // a warp's sums on their way out: 32 rows x 256 (64) bytes
+  static constexpr int kOut = kEpi * kOutWarp;
+  static constexpr int kRing = 196 * 1024 - kRed - (kPair ? kOut : 0);
+  static constexpr int kStages = kRing / kStageBytes < 9 ? kRing / kStageBytes : 9;
   static constexpr int kBufs = 512 / NT < 8 ? 512 / NT : 8;       // accumulators in TMEM
   static constexpr int kScaleRow = kSwap ? NT : 132;              // floats of a group's scales
   static constexpr int kRows = kSwap ? NT : kPair ? 256 : 128, kWeights = kSwap ? 128 : NT;      // of a tile
@@ -160,7 +174,9 @@ template <int DT, int C> __device__ __forceinline__ void put_some(void* out, lon
 }
 // A warp's 32 rows x 128 columns (a row a thread) to the output, by way of 32 x 64 bytes of shared memory, so that a store instruction writes 64 bytes of
 // eight rows instead of 16 bytes of 32: a tile's stores took 5900 cycles without. 16-byte chunks are placed by (row >> 1) & 3, free of bank conflicts.
-template <int DT> __device__ __forceinline__ void put_rows(const MatmulParams& p, uint8_t* buf, const float (&acc)[128], int row0, int row_end, int n, int lane) {
+// kAsync: 32 x 256 bytes of shared memory, a bulk copy for each row (128 columns of 16 bits, 64 of 32 at a time), which the next tile's math does not wait for: all
+// SMs end their tiles at about the same time, and 4100 cycles passed until L2 had taken the stores.
+template <int DT, bool kAsync> __device__ __forceinline__ void put_rows(const MatmulParams& p, uint8_t* buf, const float (&acc)[128], int row0, int row_end, int n, int lane) {
   constexpr int kSize = DT == DT_F32 ? 4 : 2, kStep = 64 / kSize;      // columns of a round
   if (!p.vec) {
     const int row = row0 + lane;
@@ -169,6 +185,48 @@ template <int DT> __device__ __forceinline__ void put_rows(const MatmulParams& p
       if (row < row_end && n + i < p.N) put<DT>(p.out, (long long)row * p.ldo + n + i, acc[i]);
     return;
   }
+  if constexpr (kAsync) {
+    constexpr int kCols = 256 / kSize;
+    const int row = row0 + lane;
+    uint8_t *mine = buf + lane * kOutRow, *o = reinterpret_cast<uint8_t*>(p.out) + ((long long)row * p.ldo + n) * kSize;
+#pragma unroll
+    for (int c0 = 0; c0 < 128; c0 += kCols) {
+      const int bytes = min(256, (p.N - n - c0) * kSize);
+      if (bytes <= 0) break;
+      asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");      // the row's last copy has left
+#pragma unroll
+      for (int q = 0; q < 16; ++q) {
+        uint4 w;
+        const float* v = acc + c0 + q * 16 / kSize;
+        if constexpr (DT == DT_F32) {
+          w = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+        } else {
+          using T = std::conditional_t<DT == DT_BF16, __nv_bfloat16, __half>;
+          w = make_uint4(Elem<T>::pack(v[0], v[1]), Elem<T>::pack(v[2], v[3]), Elem<T>::pack(v[4], v[5]), Elem<T>::pack(v[6], v[7]));
+        }
+        *reinterpret_cast<uint4*>(mine + q * 16) = w;
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      const int whole = bytes & ~15;
+      if (row < row_end) {
+        if (whole)
+          asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;\n cp.async.bulk.commit_group;" ::"l"(o + c0 * kSize), "r"(smem_u32(mine)), "r"(whole) : "memory");
+        for (int i = whole; i < bytes; i += 2) *reinterpret_cast<uint16_t*>(o + c0 * kSize + i) = *reinterpret_cast<const uint16_t*>(mine + i);
+      }
+    }
+    return;
+  }
+  uint8_t* o[4];      // rows i * 8 + lane / 4
+  bool row_ok[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = row0 + i * 8 + lane / 4;
+    row_ok[i] = row < row_end;
+    o[i] = reinterpret_cast<uint8_t*>(p.out) + ((long long)row * p.ldo + n) * kSize + (lane & 3) * 16;
+  }
+  const int left = (p.N - n) * kSize - (lane & 3) * 16;      // bytes of a row from this lane's first chunk on
+  uint8_t *put_at = buf + lane * 64, *get_at = buf + (lane / 4) * 64 + (((lane & 3) ^ (lane >> 3 & 3)) << 4);
+  const int turn = (lane >> 1 & 3) << 4;
 #pragma unroll
   for (int c0 = 0; c0 < 128; c0 += kStep) {
     if (n + c0 >= p.N) break;
@@ -183,26 +241,23 @@ template <int DT> __device__ __forceinline__ void put_rows(const MatmulParams& p
         using T = std::conditional_t<DT == DT_BF16, __nv_bfloat16, __half>;
         w = make_uint4(Elem<T>::pack(v[0], v[1]), Elem<T>::pack(v[2], v[3]), Elem<T>::pack(v[4], v[5]), Elem<T>::pack(v[6], v[7]));
       }
-      *reinterpret_cast<uint4*>(buf + lane * 64 + ((q ^ (lane >> 1 & 3)) << 4)) = w;
+      *reinterpret_cast<uint4*>(put_at + ((q << 4) ^ turn)) = w;
     }
     __syncwarp();
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = i * 8 + lane / 4, q = lane & 3, row = row0 + r, col = n + c0 + q * (kStep / 4);
-      const uint4 w = *reinterpret_cast<const uint4*>(buf + r * 64 + ((q ^ (r >> 1 & 3)) << 4));
-      if (row < row_end) {
-        uint8_t* o = reinterpret_cast<uint8_t*>(p.out) + ((long long)row * p.ldo + col) * kSize;
-        if (col + kStep / 4 <= p.N) {
-          *reinterpret_cast<uint4*>(o) = w;
-        } else {
-          const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+    for (int i = 0; i < 4; ++i) {      // row r = i * 8 + lane / 4: its chunks are turned by (r >> 1) & 3 = (lane >> 3) & 3
+      const uint4 w = *reinterpret_cast<const uint4*>(get_at + i * 512);
+      if (!row_ok[i]) continue;
+      if (left >= c0 * kSize + 16) {
+        *reinterpret_cast<uint4*>(o[i] + c0 * kSize) = w;
+      } else {
+        const uint32_t x[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-          for (int j = 0; j < 16 / kSize; ++j)
-            if (col + j < p.N) {
-              if constexpr (kSize == 4) reinterpret_cast<uint32_t*>(o)[j] = x[j];
-              else reinterpret_cast<uint16_t*>(o)[j] = (uint16_t)(x[j / 2] >> (16 * (j & 1)));
-            }
-        }
+        for (int j = 0; j < 16 / kSize; ++j)
+          if (left >= c0 * kSize + (j + 1) * kSize) {
+            if constexpr (kSize == 4) reinterpret_cast<uint32_t*>(o[i] + c0 * kSize)[j] = x[j];
+            else reinterpret_cast<uint16_t*>(o[i] + c0 * kSize)[j] = (uint16_t)(x[j / 2] >> (16 * (j & 1)));
+          }
       }
     }
   }
@@ -332,7 +387,7 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
   bool dead = false;       // a wait ran out: the rest of the tiles is walked without work, so that the barriers of a cluster still meet
 
   if (warp >= S::kEpi) {
-  if constexpr (S::kSplitRegs) regs_dec<72>();
+  if constexpr (S::kSplitRegs) regs_dec<136>();
   if (warp == S::kEpi) {                                             // ---- TMA producer
     const uint32_t el = elect_one();
     int st = 0, ph = 1, issued = 0;
@@ -442,9 +497,10 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
     }
   }
   } else {                                                           // ---- epilogue
-    if constexpr (S::kSplitRegs) regs_inc<216>();
+    if constexpr (S::kSplitRegs) regs_inc<184>();
     const int quad = warp & 3, half = warp >> 2, col0 = half * S::kCols;
     const int l = quad * 32 + lane;                                  // accumulator lane
+    const uint32_t lead_empty = mapa_shared(smem_u32(&acc_empty[0]), 0);
     int buf = 0, ph = 0;
     for (int t = t0; t < tiles; t += t_step) {
       const MmTile tl = mm_tile<NT, kSwap, kPair>(p, first, off, t);
@@ -452,7 +508,7 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
 #pragma unroll
       for (int i = 0; i < S::kCols; ++i) acc[i] = 0.f;
       for (int kb = kb0; kb < kb1 && !dead; ++kb) {
-        if (!mbar_wait_warp(smem_u32(&acc_full[buf]), ph, abort_flag)) { dead = true; break; }
+        if (!mbar_ready(smem_u32(&acc_full[buf]), ph) && !mbar_wait_warp(smem_u32(&acc_full[buf]), ph, abort_flag)) { dead = true; break; }
         tc_fence_after();
         const float* s = scales + buf * S::kScaleRow;
         const uint32_t taddr = tb + buf * NT + col0 + ((uint32_t)(quad * 32) << 16);
@@ -467,11 +523,9 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
           } else {      // all of it is in registers: the tensor core may have the accumulator back
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) {
-              if constexpr (kPair) mbar_arrive_cluster(mapa_shared(smem_u32(&acc_empty[buf]), 0));
-              else mbar_arrive(&acc_empty[buf]);
-              if (!kSwap) mbar_arrive(&scale_empty[buf]);
-            }
+            if constexpr (kPair) mbar_arrive_cluster_p(lead_empty + buf * 8, lane == 0);
+            else mbar_arrive_p(smem_u32(&acc_empty[buf]), lane == 0);
+            if (!kSwap) mbar_arrive_p(smem_u32(&scale_empty[buf]), lane == 0);
           }
 #pragma unroll
           for (int i = 0; i < S::kChunk; i += 4) {
@@ -485,16 +539,17 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
         }
         if constexpr (kSwap) {      // (the slot's scales are read up to here)
           __syncwarp();
-          if (lane == 0) mbar_arrive(&scale_empty[buf]);
+          mbar_arrive_p(smem_u32(&scale_empty[buf]), lane == 0);
         }
         if (++buf == S::kBufs) buf = 0, ph ^= 1;
       }
       if constexpr (!kSwap) {
         if (!dead) {
           const int row0 = tl.row0 + crow + quad * 32, n = tl.n0 + col0;
-          if (p.out_dtype == DT_BF16) put_rows<DT_BF16>(p, outs + warp * 2048, acc, row0, tl.row_end, n, lane);
-          else if (p.out_dtype == DT_F16) put_rows<DT_F16>(p, outs + warp * 2048, acc, row0, tl.row_end, n, lane);
-          else put_rows<DT_F32>(p, outs + warp * 2048, acc, row0, tl.row_end, n, lane);
+          uint8_t* buf = outs + warp * S::kOutWarp;
+          if (p.out_dtype == DT_BF16) put_rows<DT_BF16, kPair>(p, buf, acc, row0, tl.row_end, n, lane);
+          else if (p.out_dtype == DT_F16) put_rows<DT_F16, kPair>(p, buf, acc, row0, tl.row_end, n, lane);
+          else put_rows<DT_F32, kPair>(p, buf, acc, row0, tl.row_end, n, lane);
         }
       } else {
         if (split == 1) {
@@ -526,6 +581,7 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
         }
       }
     }
+    if constexpr (kPair) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");      // shared memory stays until the copies have read it
     if (p.offsets && p.zero_rest) {      // rows outside every run, and of experts that are not there
       const int step = gridDim.x * S::kEpi * 32, me = blockIdx.x * S::kEpi * 32 + tid;
       for (int u = 0; u < p.U; ++u) {
