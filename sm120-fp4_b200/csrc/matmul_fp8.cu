@@ -143,6 +143,25 @@ template <int NT, bool kSwap, bool kPair> struct MmShape {
 
 struct MmTile { int row0, row_end, expert, n0; };
 
+// Rounds of the workers (CTAs, or pairs): in every full round a tile each; the tiles left over are cut along the inner size into as many parts as leave
+// no worker without one, up to the cluster (parts of a tile are neighbours in a cluster), with two groups at least in a part.
+struct MmRounds {
+  int full, rest, parts;
+  __device__ __forceinline__ MmRounds(int tiles, int workers, int cluster, int KB) : full(tiles / workers), rest(tiles - tiles / workers * workers), parts(cluster) {
+    while (parts > 1 && (rest * parts > workers || KB < 2 * parts)) parts >>= 1;
+  }
+  __device__ __forceinline__ int count() const { return full + (rest > 0); }
+  __device__ __forceinline__ bool shared(int i) const { return i == full && parts > 1; }
+  // tile of round i (-1: none) and its groups
+  __device__ __forceinline__ int tile(int i, int worker, int workers, int KB, int& kb0, int& kb1) const {
+    kb0 = 0, kb1 = KB;
+    if (i < full) return i * workers + worker;
+    const int j = worker / parts, r = worker - j * parts;
+    kb0 = (int)((long long)KB * r / parts), kb1 = (int)((long long)KB * (r + 1) / parts);
+    return j < rest ? full * workers + j : -1;
+  }
+};
+
 // The t-th tile: row tiles of a run and weight block side by side, so that neighbours share the weights.
 template <int NT, bool kSwap, bool kPair>
 __device__ __forceinline__ MmTile mm_tile(const MatmulParams& p, const int* first, const int* off, int t) {
@@ -265,9 +284,10 @@ template <int DT, bool kAsync> __device__ __forceinline__ void put_rows(const Ma
 // This CTA's share of a tile whose inner size is split: 1 / kRanks of it, the sums of all ranks, added in rank order. A thread takes four weights of a row at a
 // time; all of its loads from the ranks' shared memory are in flight together.
 template <int NT, int kRanks>
-__device__ __forceinline__ void mm_add_ranks(const MatmulParams& p, const MmTile& tl, const float* red, int rank, int tid) {
+__device__ __forceinline__ void mm_add_ranks(const MatmulParams& p, const MmTile& tl, const float* red, int cluster_rank, int tid) {
   using S = MmShape<NT, true, false>;
   constexpr int kThreads = S::kEpi * 32, kItems = NT * 32 / kRanks, kEach = (kItems + kThreads - 1) / kThreads;
+  const int base = cluster_rank & ~(kRanks - 1), rank = cluster_rank - base;
   float4 v[kEach][kRanks];
 #pragma unroll
   for (int j = 0; j < kEach; ++j) {
@@ -275,7 +295,7 @@ __device__ __forceinline__ void mm_add_ranks(const MatmulParams& p, const MmTile
     if (kItems % kThreads == 0 || i < kItems) {
       const uint32_t mine = smem_u32(red) + (rank * kItems + i) * 16;
 #pragma unroll
-      for (int r = 0; r < kRanks; ++r) v[j][r] = ld_cluster_f32x4(mapa_shared(mine, r));
+      for (int r = 0; r < kRanks; ++r) v[j][r] = ld_cluster_f32x4(mapa_shared(mine, base + r));
     }
   }
 #pragma unroll
@@ -313,7 +333,7 @@ __device__ __forceinline__ void zero_rows(const MatmulParams& p, int r0, int r1,
 
 template <int NT, bool kSwap, bool kPair>
 __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
-    k_matmul_fp8(const __grid_constant__ CUtensorMap map_rows, const __grid_constant__ CUtensorMap map_weights, const __grid_constant__ MatmulParams p, int split) {
+    k_matmul_fp8(const __grid_constant__ CUtensorMap map_rows, const __grid_constant__ CUtensorMap map_weights, const __grid_constant__ MatmulParams p, int cluster) {
   using S = MmShape<NT, kSwap, kPair>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -324,7 +344,7 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
   int* off = first + MM_MAXU + 1;
   __shared__ uint64_t full[S::kStages], empty[S::kStages], acc_full[S::kBufs], acc_empty[S::kBufs], scale_empty[S::kBufs], drained;
   __shared__ uint32_t tmem_base;
-  __shared__ int abort_s, wsum[32];
+  __shared__ int abort_s, unknown_s, wsum[32];
   volatile int* abort_flag = &abort_s;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
@@ -332,7 +352,7 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
     for (int i = 0; i < S::kStages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
     for (int i = 0; i < S::kBufs; ++i) mbar_init(&acc_full[i], 2), mbar_init(&acc_empty[i], kPair ? 2 * S::kEpi : S::kEpi), mbar_init(&scale_empty[i], S::kEpi);
     mbar_init(&drained, 1);
-    abort_s = 0;
+    abort_s = 0, unknown_s = 0;
     fence_mbar_init();
     prefetch_tensormap(&map_rows), prefetch_tensormap(&map_weights);
   }
@@ -341,6 +361,7 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
     else tmem_alloc(&tmem_base, S::kBufs * NT), tmem_relinquish();
   }
   grid_dependency_wait();
+  grid_launch_dependents();      // (the next kernel's CTAs set themselves up as this one's leave, and wait for all of it)
 
   // The plan: first tile of each run. Offsets are held to 0..M and to their order, runs of an expert that is not there have no tiles.
   int tiles;
@@ -353,7 +374,9 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
     for (int u = u0; u < u1; ++u) {
       const int e = p.experts[u];
       first[u] = n;
-      if (e >= 0 && e < p.E) n += (max(off[u + 1] - off[u], 0) + S::kRows - 1) / S::kRows * ntn;
+      const int rows = max(off[u + 1] - off[u], 0);
+      if (e >= 0 && e < p.E) n += (rows + S::kRows - 1) / S::kRows * ntn;
+      else if (rows) unknown_s = 1;
     }
     int incl = n;
 #pragma unroll
@@ -379,10 +402,9 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
   tc_fence_after();
   const uint32_t tb = tmem_base;
 
-  const int ranks = kPair ? 2 : split;
-  const int rank = ranks > 1 ? (int)cluster_ctarank() : 0;
-  const int t0 = blockIdx.x / ranks, t_step = gridDim.x / ranks;
-  const int kb0 = kPair ? 0 : p.KB * rank / split, kb1 = kPair ? p.KB : p.KB * (rank + 1) / split;
+  const int rank = kPair || cluster > 1 ? (int)cluster_ctarank() : 0;
+  const int worker = kPair ? blockIdx.x / 2 : blockIdx.x, workers = kPair ? gridDim.x / 2 : gridDim.x;
+  const MmRounds rounds(tiles, workers, kSwap ? cluster : 1, p.KB);
   const int crow = kPair ? rank * 128 : 0;      // this CTA's rows of a pair's tile
   bool dead = false;       // a wait ran out: the rest of the tiles is walked without work, so that the barriers of a cluster still meet
 
@@ -391,8 +413,11 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
   if (warp == S::kEpi) {                                             // ---- TMA producer
     const uint32_t el = elect_one();
     int st = 0, ph = 1, issued = 0;
-    for (int t = t0; t < tiles; t += t_step) {
-      const MmTile tl = mm_tile<NT, kSwap, kPair>(p, first, off, t);
+    for (int i = 0; i < rounds.count(); ++i) {
+      int kb0, kb1;
+      const int t = rounds.tile(i, worker, workers, p.KB, kb0, kb1);
+      if (t < 0) kb1 = kb0;
+      const MmTile tl = mm_tile<NT, kSwap, kPair>(p, first, off, t < 0 ? 0 : t);
       for (int kb = kb0; kb < kb1 && !dead; ++kb) {
         if (!mbar_wait_warp(smem_u32(&empty[st]), ph, abort_flag)) { dead = true; break; }
         const uint32_t bar = smem_u32(&full[st]), sa = smem_u32(smem + st * S::kStageBytes);
@@ -410,7 +435,13 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
         ++issued;
         if (++st == S::kStages) st = 0, ph ^= 1;
       }
-      if (split > 1) __syncwarp(), cluster_sync_all(), cluster_sync_all();
+      if (rounds.shared(i)) __syncwarp(), cluster_sync_all(), cluster_sync_all();
+    }
+    // The tensor core's word that it has read a slot goes to this CTA's barriers (from the leader, in a pair): all of it arrives before the CTA may end, or it
+    // would reach the barriers of the CTA that comes after it.
+    for (int i = 0; i < S::kStages && !dead; ++i) {
+      if (!mbar_wait_warp(smem_u32(&empty[st]), ph, abort_flag)) dead = true;
+      if (++st == S::kStages) st = 0, ph ^= 1;
     }
     if (dead) {      // copies in flight land before the CTA may end (with a limit)
       for (int i = issued > S::kStages ? issued - S::kStages : 0; i < issued; ++i)
@@ -422,7 +453,9 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
     const uint32_t el = elect_one();
     constexpr uint32_t idesc = idesc_f8(kPair ? 256 : 128, NT);
     int st = 0, ph = 0, buf = 0, bph = 1;
-    for (int t = t0; t < tiles; t += t_step) {
+    for (int i = 0; i < rounds.count(); ++i) {
+      int kb0, kb1;
+      if (rounds.tile(i, worker, workers, p.KB, kb0, kb1) < 0) kb1 = kb0;
       for (int kb = kb0; kb < kb1 && !dead && (!kPair || rank == 0); ++kb) {
         if (!mbar_wait_both(smem_u32(&acc_empty[buf]), bph, smem_u32(&full[st]), ph, abort_flag)) { dead = true; break; }
         tc_fence_after();
@@ -442,7 +475,7 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
         if (++st == S::kStages) st = 0, ph ^= 1;
         if (++buf == S::kBufs) buf = 0, bph ^= 1;
       }
-      if (split > 1) __syncwarp(), cluster_sync_all(), cluster_sync_all();
+      if (rounds.shared(i)) __syncwarp(), cluster_sync_all(), cluster_sync_all();
     }
     if (dead) {
       if constexpr (kPair) umma2_commit_p(&drained, 1, el & (rank == 0));
@@ -452,8 +485,11 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
   } else if (warp == S::kEpi + 2) {                                  // ---- scales: four groups ahead in registers, then a slot beside each accumulator
     constexpr int kHere = kSwap ? NT : 128, R = (kHere + 31) / 32;
     int buf = 0, bph = 1;
-    for (int t = t0; t < tiles; t += t_step) {
-      const MmTile tl = mm_tile<NT, kSwap, kPair>(p, first, off, t);
+    for (int i = 0; i < rounds.count(); ++i) {
+      int kb0, kb1;
+      const int t = rounds.tile(i, worker, workers, p.KB, kb0, kb1);
+      if (t < 0) kb1 = kb0;
+      const MmTile tl = mm_tile<NT, kSwap, kPair>(p, first, off, t < 0 ? 0 : t);
       const float* ra[R];
 #pragma unroll
       for (int i = 0; i < R; ++i) ra[i] = p.sa + (long long)min(tl.row0 + crow + lane + 32 * i, p.M - 1) * p.KB;
@@ -469,7 +505,7 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
           vb[j] = __ldg(rb + g);
         }
       };
-      if (!dead) fetch(kb0);
+      if (!dead && kb0 < kb1) fetch(kb0);
       for (int kb = kb0; kb < kb1 && !dead; kb += 4) {
         float ca[4][R], cb[4];
 #pragma unroll
@@ -493,7 +529,7 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
           if (++buf == S::kBufs) buf = 0, bph ^= 1;
         }
       }
-      if (split > 1) __syncwarp(), cluster_sync_all(), cluster_sync_all();
+      if (rounds.shared(i)) __syncwarp(), cluster_sync_all(), cluster_sync_all();
     }
   }
   } else {                                                           // ---- epilogue
@@ -502,11 +538,14 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
     const int l = quad * 32 + lane;                                  // accumulator lane
     const uint32_t lead_empty = mapa_shared(smem_u32(&acc_empty[0]), 0);
     int buf = 0, ph = 0;
-    for (int t = t0; t < tiles; t += t_step) {
-      const MmTile tl = mm_tile<NT, kSwap, kPair>(p, first, off, t);
+    for (int i = 0; i < rounds.count(); ++i) {
+      int kb0, kb1;
+      const int t = rounds.tile(i, worker, workers, p.KB, kb0, kb1);
+      if (t < 0) kb1 = kb0;
+      const MmTile tl = mm_tile<NT, kSwap, kPair>(p, first, off, t < 0 ? 0 : t);
       float acc[S::kCols];
 #pragma unroll
-      for (int i = 0; i < S::kCols; ++i) acc[i] = 0.f;
+      for (int j = 0; j < S::kCols; ++j) acc[j] = 0.f;
       for (int kb = kb0; kb < kb1 && !dead; ++kb) {
         if (!mbar_ready(smem_u32(&acc_full[buf]), ph) && !mbar_wait_warp(smem_u32(&acc_full[buf]), ph, abort_flag)) { dead = true; break; }
         tc_fence_after();
@@ -544,7 +583,7 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
         if (++buf == S::kBufs) buf = 0, ph ^= 1;
       }
       if constexpr (!kSwap) {
-        if (!dead) {
+        if (!dead && t >= 0) {
           const int row0 = tl.row0 + crow + quad * 32, n = tl.n0 + col0;
           uint8_t* buf = outs + warp * S::kOutWarp;
           if (p.out_dtype == DT_BF16) put_rows<DT_BF16, kPair>(p, buf, acc, row0, tl.row_end, n, lane);
@@ -552,28 +591,28 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
           else put_rows<DT_F32, kPair>(p, buf, acc, row0, tl.row_end, n, lane);
         }
       } else {
-        if (split == 1) {
+        if (!rounds.shared(i)) {
           const int n = tl.n0 + l;
-          if (!dead && n < p.N) {
+          if (!dead && t >= 0 && n < p.N) {
 #pragma unroll
-            for (int i = 0; i < S::kCols; ++i) {
-              const int row = tl.row0 + col0 + i;
+            for (int j = 0; j < S::kCols; ++j) {
+              const int row = tl.row0 + col0 + j;
               if (row < tl.row_end) {
                 const long long at = (long long)row * p.ldo + n;
-                if (p.out_dtype == DT_BF16) put<DT_BF16>(p.out, at, acc[i]);
-                else if (p.out_dtype == DT_F16) put<DT_F16>(p.out, at, acc[i]);
-                else put<DT_F32>(p.out, at, acc[i]);
+                if (p.out_dtype == DT_BF16) put<DT_BF16>(p.out, at, acc[j]);
+                else if (p.out_dtype == DT_F16) put<DT_F16>(p.out, at, acc[j]);
+                else put<DT_F32>(p.out, at, acc[j]);
               }
             }
           }
         } else {
 #pragma unroll
-          for (int i = 0; i < S::kCols; ++i) red[(col0 + i) * 128 + l] = acc[i];
+          for (int j = 0; j < S::kCols; ++j) red[(col0 + j) * 128 + l] = acc[j];
           __syncwarp();
           cluster_sync_all();
-          if (!dead) {
-            if (split == 2) mm_add_ranks<NT, 2>(p, tl, red, rank, tid);
-            else if (split == 4) mm_add_ranks<NT, 4>(p, tl, red, rank, tid);
+          if (!dead && t >= 0) {
+            if (rounds.parts == 2) mm_add_ranks<NT, 2>(p, tl, red, rank, tid);
+            else if (rounds.parts == 4) mm_add_ranks<NT, 4>(p, tl, red, rank, tid);
             else mm_add_ranks<NT, 8>(p, tl, red, rank, tid);
           }
           __syncwarp();
@@ -584,10 +623,11 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
     if constexpr (kPair) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");      // shared memory stays until the copies have read it
     if (p.offsets && p.zero_rest) {      // rows outside every run, and of experts that are not there
       const int step = gridDim.x * S::kEpi * 32, me = blockIdx.x * S::kEpi * 32 + tid;
-      for (int u = 0; u < p.U; ++u) {
-        const int e = p.experts[u];
-        if (e < 0 || e >= p.E) zero_rows(p, off[u], off[u + 1], me, step);
-      }
+      if (unknown_s)
+        for (int u = 0; u < p.U; ++u) {
+          const int e = p.experts[u];
+          if (e < 0 || e >= p.E) zero_rows(p, off[u], off[u + 1], me, step);
+        }
       if (off[0] > 0) zero_rows(p, 0, off[0], me, step);
       zero_rows(p, off[p.U], p.M, me, step);
     }
@@ -631,14 +671,14 @@ static int sm_count() {
 }
 
 template <int NT, bool kSwap, bool kPair>
-static int launch_matmul(const MatmulParams& p, const void* a, long long lda, const void* w, long long ldw, long long tiles, int split, int sms, cudaStream_t st) {
+static int launch_matmul(const MatmulParams& p, const void* a, long long lda, const void* w, long long ldw, long long tiles, int cluster, int sms, cudaStream_t st) {
   using S = MmShape<NT, kSwap, kPair>;
   CUtensorMap rows, weights;
   if (int rc = codes_map(&rows, a, p.M, p.K, lda, kSwap ? NT : 128)) return rc;
   if (int rc = codes_map(&weights, w, (long long)p.E * p.N, p.K, ldw, kSwap ? 128 : S::kBRows)) return rc;
   const void* fn = (const void*)k_matmul_fp8<NT, kSwap, kPair>;
   B200_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
-  const int ranks = kPair ? 2 : split;
+  const int ranks = kPair ? 2 : cluster;
   const long long most = sms / ranks;
   const int clusters = (int)(tiles < most ? (tiles > 0 ? tiles : 1) : most);
   cudaLaunchConfig_t cfg = {};
@@ -649,13 +689,13 @@ static int launch_matmul(const MatmulParams& p, const void* a, long long lda, co
   attr[1].val.clusterDim.x = ranks, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr, cfg.numAttrs = ranks > 1 ? 2 : 1;
   MatmulParams q = p;
-  void* args[] = {&rows, &weights, &q, &split};
+  void* args[] = {&rows, &weights, &q, &cluster};
   B200_CUDA_TRY(cudaLaunchKernelExC(&cfg, fn, args));
   return B200MOE_OK;
 }
 
 // Which form: rows on the lanes (128 x 256 tiles) where a run of rows fills them and the tiles fill the SMs, otherwise weights on the lanes with
-// the rows' tile that a run needs; there the inner size is split while SMs are idle and a CTA keeps two groups.
+// the rows' tile that a run needs, and clusters large enough to give every SM a part of the tiles that there are (two for the tiles of the last round).
 static int matmul(const MatmulParams& p, const void* a, long long lda, const void* w, long long ldw, cudaStream_t st) {
   const int sms = sm_count();
   if (sms <= 0) return B200MOE_ERR_DEVICE;
@@ -665,13 +705,13 @@ static int matmul(const MatmulParams& p, const void* a, long long lda, const voi
   if (mean >= 96 && tiles(128, 256) >= sms / 2) return launch_matmul<256, false, false>(p, a, lda, w, ldw, tiles(128, 256), 1, sms, st);
   const int nt = mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 64 ? 64 : 128;
   const long long n = tiles(nt, 128);
-  int split = 1;
-  while (split < 8 && n * split * 2 <= sms && p.KB >= split * 4) split *= 2;
+  int cluster = 2;
+  while (cluster < 8 && n * cluster * 2 <= sms && p.KB >= cluster * 4) cluster *= 2;
   switch (nt) {
-    case 16: return launch_matmul<16, true, false>(p, a, lda, w, ldw, n, split, sms, st);
-    case 32: return launch_matmul<32, true, false>(p, a, lda, w, ldw, n, split, sms, st);
-    case 64: return launch_matmul<64, true, false>(p, a, lda, w, ldw, n, split, sms, st);
-    default: return launch_matmul<128, true, false>(p, a, lda, w, ldw, n, split, sms, st);
+    case 16: return launch_matmul<16, true, false>(p, a, lda, w, ldw, n, cluster, sms, st);
+    case 32: return launch_matmul<32, true, false>(p, a, lda, w, ldw, n, cluster, sms, st);
+    case 64: return launch_matmul<64, true, false>(p, a, lda, w, ldw, n, cluster, sms, st);
+    default: return launch_matmul<128, true, false>(p, a, lda, w, ldw, n, cluster, sms, st);
   }
 }
 

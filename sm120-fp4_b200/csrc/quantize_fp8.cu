@@ -16,6 +16,7 @@ __global__ void __launch_bounds__(256) k_quantize_fp8_rows(const T* __restrict__
   const int KB = (K + 127) >> 7;
   const long long units = (long long)rows * KB;
   grid_dependency_wait();
+  grid_launch_dependents();
   for (long long u = (long long)blockIdx.x * 32 + (threadIdx.x >> 3); u < ((units + 3) & ~3ll); u += (long long)gridDim.x * 32) {   // (whole warps: four units each)
     const bool in = u < units;
     const int row = in ? (int)(u / KB) : 0, g = in ? (int)(u - (long long)row * KB) : 0;
@@ -56,6 +57,7 @@ __global__ void __launch_bounds__(256) k_quantize_fp8_rows_any(const T* __restri
   const int lane = threadIdx.x & 31, KB = (K + 127) >> 7;
   const long long units = (long long)rows * KB;
   grid_dependency_wait();
+  grid_launch_dependents();
   for (long long u = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); u < units; u += (long long)gridDim.x * 8) {
     const int row = (int)(u / KB), g = (int)(u - (long long)row * KB);
     const int src = src_row ? src_row[row] : row;
@@ -91,6 +93,7 @@ __global__ void __launch_bounds__(Elem<T>::kSize == 2 ? 256 : 512) k_quantize_fp
   const int c = kb * 128 + (threadIdx.x % kLanes) * kPer, r0 = nb * 128 + threadIdx.x / kLanes;
   const T* src = w + e * N * K + c;
   grid_dependency_wait();
+  grid_launch_dependents();
   uint4 d[kSteps];
 #pragma unroll
   for (int i = 0; i < kSteps; ++i) {
