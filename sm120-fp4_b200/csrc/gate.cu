@@ -101,7 +101,6 @@ __global__ void __launch_bounds__(256) k_gate(const T* __restrict__ logits, long
                                               int* __restrict__ ids) {
   const int lane = threadIdx.x & 31;
   grid_dependency_wait();
-  grid_launch_dependents();
   const int t = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   if (t >= tokens) return;
   float x[V];
@@ -150,7 +149,6 @@ __global__ void __launch_bounds__(256) k_gate_backward(const float* __restrict__
                                                        const T* __restrict__ logits, long long stride, int tokens, int E, int k, int renorm, T* __restrict__ out) {
   const int lane = threadIdx.x & 31;
   grid_dependency_wait();
-  grid_launch_dependents();
   const int t = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   if (t >= tokens) return;
   int e = -1;
@@ -196,7 +194,6 @@ __global__ void __launch_bounds__(kBalanceWarps * 32) k_balance_part(const T* __
   if (threadIdx.x == 0) live_n = 0;
   __syncthreads();
   grid_dependency_wait();
-  grid_launch_dependents();
   float acc[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) acc[j] = 0.f;
@@ -242,7 +239,6 @@ __global__ void __cluster_dims__(kBalanceRanks, 1, 1) __launch_bounds__(512)
   const int per = (E + kBalanceRanks - 1) / kBalanceRanks, e = rank * per + col;
   const long long W = balance_words(E);
   grid_dependency_wait();
-  grid_launch_dependents();
   double p = 0.0;
   int c = 0;
   const bool mine = col < per && e < E;
@@ -302,7 +298,6 @@ __global__ void __launch_bounds__(256) k_balance_backward(const float* __restric
                                                           T* __restrict__ out) {
   const int lane = threadIdx.x & 31;
   grid_dependency_wait();
-  grid_launch_dependents();
   const float inv = stats[0], c = *grad * stats[1];
   float f[V];
 #pragma unroll

@@ -72,6 +72,18 @@ __device__ __forceinline__ bool mbar_ready(uint32_t bar, uint32_t parity) {
   asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
   return __all_sync(0xffffffffu, ok != 0);
 }
+// mbar_wait_warp with a barrier of its own for each lane that is not done
+__device__ __forceinline__ bool mbar_wait_lanes(uint32_t bar, uint32_t parity, bool done, volatile int* abort_flag, uint32_t limit = (1u << 20)) {
+  for (uint32_t it = 0; it < limit; ++it) {
+    uint32_t ok = 1;
+    if (!done)
+      asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    if (__all_sync(0xffffffffu, ok != 0)) return true;
+    if ((it & 63u) == 63u && __any_sync(0xffffffffu, *abort_flag != 0)) return false;
+  }
+  *abort_flag = 1;
+  return false;
+}
 // mbar_wait_warp for two barriers at once (one vote), what came before their arrivals in the whole cluster visible
 __device__ __forceinline__ bool mbar_wait_both(uint32_t bar0, uint32_t parity0, uint32_t bar1, uint32_t parity1, volatile int* abort_flag, uint32_t limit = (1u << 20)) {
   for (uint32_t it = 0; it < limit; ++it) {
@@ -123,8 +135,10 @@ template <int NT, bool kSwap, bool kPair> struct MmShape {
   static constexpr int kEpi = NT >= 128 ? 8 : 4;                  // epilogue warps: two per lane quadrant where a thread's columns would be more than 64 (128: kSwap false)
   static constexpr int kCols = NT / (kEpi / 4);                   // columns of a thread
   static constexpr int kChunk = kCols < 32 ? kCols : 32;          // columns of a TMEM load
-  // 128 sums and 64 values in flight a thread: registers go from the other warps (a warpgroup of four, one idle) to the epilogue. A launch of 12 warps has
-  // 168 a thread: 8 * 184 + 4 * 136 = 12 * 168.
+  // 128 sums and 64 values in flight a thread: registers go from the other warps (a warpgroup of four, one idle) to the epilogue's eight. A launch of 12 warps has
+  // 168 a thread: 8 * kEpiRegs + 4 * (504 - 2 * kEpiRegs) = 12 * 168. Both shares are those with which ptxas spills nothing (192 / 120 spilled and took 148
+  // instead of 126 us at 8192 x 4096 x 4096).
+  static constexpr int kEpiRegs = kPair ? 176 : 184;
   static constexpr bool kSplitRegs = kCols == 128;
   static constexpr int kThreads = kSplitRegs ? 384 : (kEpi + 3) * 32;
   static constexpr int kBRows = kPair ? NT / 2 : NT;              // rows of the B operand in this CTA's shared memory
@@ -143,22 +157,36 @@ template <int NT, bool kSwap, bool kPair> struct MmShape {
 
 struct MmTile { int row0, row_end, expert, n0; };
 
-// Rounds of the workers (CTAs, or pairs): in every full round a tile each; the tiles left over are cut along the inner size into as many parts as leave
-// no worker without one, up to the cluster (parts of a tile are neighbours in a cluster), with two groups at least in a part.
-struct MmRounds {
-  int full, rest, parts;
-  __device__ __forceinline__ MmRounds(int tiles, int workers, int cluster, int KB) : full(tiles / workers), rest(tiles - tiles / workers * workers), parts(cluster) {
-    while (parts > 1 && (rest * parts > workers || KB < 2 * parts)) parts >>= 1;
+// Rounds of a worker (a CTA, or a pair): a tile each. kParts: the tiles that are left for the last round are cut along the inner size into as many parts as leave no
+// worker without one, up to the cluster (parts of a tile are neighbours in a cluster), with two groups at least in a part; every worker has that round.
+template <bool kParts> struct MmRounds {
+  int tiles, worker, workers, KB, full = 0, rest = 0, log_parts = 0;
+  __device__ __forceinline__ MmRounds(int tiles, int worker, int workers, int KB, int cluster) : tiles(tiles), worker(worker), workers(workers), KB(KB) {
+    if constexpr (kParts) {
+      full = tiles / workers, rest = tiles - full * workers, log_parts = 31 - __clz(cluster);
+      while (log_parts > 0 && ((rest << log_parts) > workers || KB < (2 << log_parts))) --log_parts;
+    }
   }
-  __device__ __forceinline__ int count() const { return full + (rest > 0); }
-  __device__ __forceinline__ bool shared(int i) const { return i == full && parts > 1; }
+  __device__ __forceinline__ bool has(int i) const {
+    if constexpr (kParts) return i < full + (rest > 0);
+    else return i * workers + worker < tiles;
+  }
+  __device__ __forceinline__ bool shared(int i) const { return kParts && i == full && log_parts > 0; }
   // tile of round i (-1: none) and its groups
-  __device__ __forceinline__ int tile(int i, int worker, int workers, int KB, int& kb0, int& kb1) const {
+  __device__ __forceinline__ int tile(int i, int& kb0, int& kb1) const {
     kb0 = 0, kb1 = KB;
-    if (i < full) return i * workers + worker;
-    const int j = worker / parts, r = worker - j * parts;
-    kb0 = (int)((long long)KB * r / parts), kb1 = (int)((long long)KB * (r + 1) / parts);
-    return j < rest ? full * workers + j : -1;
+    if constexpr (kParts) {
+      if (i == full) {
+        const int j = worker >> log_parts, r = worker & ((1 << log_parts) - 1);
+        kb0 = (KB * r) >> log_parts, kb1 = (KB * (r + 1)) >> log_parts;      // (KB < 2^24, at most 8 parts)
+        if (j >= rest) {
+          kb1 = kb0;
+          return -1;
+        }
+        return full * workers + j;
+      }
+    }
+    return i * workers + worker;
   }
 };
 
@@ -404,20 +432,19 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
 
   const int rank = kPair || cluster > 1 ? (int)cluster_ctarank() : 0;
   const int worker = kPair ? blockIdx.x / 2 : blockIdx.x, workers = kPair ? gridDim.x / 2 : gridDim.x;
-  const MmRounds rounds(tiles, workers, kSwap ? cluster : 1, p.KB);
+  const MmRounds<kSwap> rounds(tiles, worker, workers, p.KB, cluster);
   const int crow = kPair ? rank * 128 : 0;      // this CTA's rows of a pair's tile
   bool dead = false;       // a wait ran out: the rest of the tiles is walked without work, so that the barriers of a cluster still meet
 
   if (warp >= S::kEpi) {
-  if constexpr (S::kSplitRegs) regs_dec<136>();
+  if constexpr (S::kSplitRegs) regs_dec<504 - 2 * S::kEpiRegs>();
   if (warp == S::kEpi) {                                             // ---- TMA producer
     const uint32_t el = elect_one();
     int st = 0, ph = 1, issued = 0;
-    for (int i = 0; i < rounds.count(); ++i) {
+    for (int i = 0; rounds.has(i); ++i) {
       int kb0, kb1;
-      const int t = rounds.tile(i, worker, workers, p.KB, kb0, kb1);
-      if (t < 0) kb1 = kb0;
-      const MmTile tl = mm_tile<NT, kSwap, kPair>(p, first, off, t < 0 ? 0 : t);
+      const int t = rounds.tile(i, kb0, kb1);
+      const MmTile tl = mm_tile<NT, kSwap, kPair>(p, first, off, kSwap && t < 0 ? 0 : t);
       for (int kb = kb0; kb < kb1 && !dead; ++kb) {
         if (!mbar_wait_warp(smem_u32(&empty[st]), ph, abort_flag)) { dead = true; break; }
         const uint32_t bar = smem_u32(&full[st]), sa = smem_u32(smem + st * S::kStageBytes);
@@ -439,10 +466,7 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
     }
     // The tensor core's word that it has read a slot goes to this CTA's barriers (from the leader, in a pair): all of it arrives before the CTA may end, or it
     // would reach the barriers of the CTA that comes after it.
-    for (int i = 0; i < S::kStages && !dead; ++i) {
-      if (!mbar_wait_warp(smem_u32(&empty[st]), ph, abort_flag)) dead = true;
-      if (++st == S::kStages) st = 0, ph ^= 1;
-    }
+    if (!dead && !mbar_wait_lanes(smem_u32(&empty[lane < S::kStages ? lane : 0]), lane < st ? ph ^ 1 : ph, lane >= S::kStages, abort_flag)) dead = true;
     if (dead) {      // copies in flight land before the CTA may end (with a limit)
       for (int i = issued > S::kStages ? issued - S::kStages : 0; i < issued; ++i)
         for (int n = 0; n < 1 << 16 && (!kPair || rank == 0) && !mbar_try_wait(&full[i % S::kStages], (i / S::kStages) & 1); ++n) {}
@@ -453,9 +477,9 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
     const uint32_t el = elect_one();
     constexpr uint32_t idesc = idesc_f8(kPair ? 256 : 128, NT);
     int st = 0, ph = 0, buf = 0, bph = 1;
-    for (int i = 0; i < rounds.count(); ++i) {
+    for (int i = 0; rounds.has(i); ++i) {
       int kb0, kb1;
-      if (rounds.tile(i, worker, workers, p.KB, kb0, kb1) < 0) kb1 = kb0;
+      rounds.tile(i, kb0, kb1);
       for (int kb = kb0; kb < kb1 && !dead && (!kPair || rank == 0); ++kb) {
         if (!mbar_wait_both(smem_u32(&acc_empty[buf]), bph, smem_u32(&full[st]), ph, abort_flag)) { dead = true; break; }
         tc_fence_after();
@@ -485,11 +509,10 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
   } else if (warp == S::kEpi + 2) {                                  // ---- scales: four groups ahead in registers, then a slot beside each accumulator
     constexpr int kHere = kSwap ? NT : 128, R = (kHere + 31) / 32;
     int buf = 0, bph = 1;
-    for (int i = 0; i < rounds.count(); ++i) {
+    for (int i = 0; rounds.has(i); ++i) {
       int kb0, kb1;
-      const int t = rounds.tile(i, worker, workers, p.KB, kb0, kb1);
-      if (t < 0) kb1 = kb0;
-      const MmTile tl = mm_tile<NT, kSwap, kPair>(p, first, off, t < 0 ? 0 : t);
+      const int t = rounds.tile(i, kb0, kb1);
+      const MmTile tl = mm_tile<NT, kSwap, kPair>(p, first, off, kSwap && t < 0 ? 0 : t);
       const float* ra[R];
 #pragma unroll
       for (int i = 0; i < R; ++i) ra[i] = p.sa + (long long)min(tl.row0 + crow + lane + 32 * i, p.M - 1) * p.KB;
@@ -533,16 +556,15 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
     }
   }
   } else {                                                           // ---- epilogue
-    if constexpr (S::kSplitRegs) regs_inc<184>();
+    if constexpr (S::kSplitRegs) regs_inc<S::kEpiRegs>();
     const int quad = warp & 3, half = warp >> 2, col0 = half * S::kCols;
     const int l = quad * 32 + lane;                                  // accumulator lane
     const uint32_t lead_empty = mapa_shared(smem_u32(&acc_empty[0]), 0);
     int buf = 0, ph = 0;
-    for (int i = 0; i < rounds.count(); ++i) {
+    for (int i = 0; rounds.has(i); ++i) {
       int kb0, kb1;
-      const int t = rounds.tile(i, worker, workers, p.KB, kb0, kb1);
-      if (t < 0) kb1 = kb0;
-      const MmTile tl = mm_tile<NT, kSwap, kPair>(p, first, off, t < 0 ? 0 : t);
+      const int t = rounds.tile(i, kb0, kb1);
+      const MmTile tl = mm_tile<NT, kSwap, kPair>(p, first, off, kSwap && t < 0 ? 0 : t);
       float acc[S::kCols];
 #pragma unroll
       for (int j = 0; j < S::kCols; ++j) acc[j] = 0.f;
@@ -583,7 +605,7 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
         if (++buf == S::kBufs) buf = 0, ph ^= 1;
       }
       if constexpr (!kSwap) {
-        if (!dead && t >= 0) {
+        if (!dead) {
           const int row0 = tl.row0 + crow + quad * 32, n = tl.n0 + col0;
           uint8_t* buf = outs + warp * S::kOutWarp;
           if (p.out_dtype == DT_BF16) put_rows<DT_BF16, kPair>(p, buf, acc, row0, tl.row_end, n, lane);
@@ -611,8 +633,8 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
           __syncwarp();
           cluster_sync_all();
           if (!dead && t >= 0) {
-            if (rounds.parts == 2) mm_add_ranks<NT, 2>(p, tl, red, rank, tid);
-            else if (rounds.parts == 4) mm_add_ranks<NT, 4>(p, tl, red, rank, tid);
+            if (rounds.log_parts == 1) mm_add_ranks<NT, 2>(p, tl, red, rank, tid);
+            else if (rounds.log_parts == 2) mm_add_ranks<NT, 4>(p, tl, red, rank, tid);
             else mm_add_ranks<NT, 8>(p, tl, red, rank, tid);
           }
           __syncwarp();
