@@ -286,10 +286,12 @@ int b200moe_balance_backward(const float* grad_loss, const void* logits, int dty
 /* ---- FP8 (E4M3) with fp32 scales per 128 values, for the matrices of a model that are not NVFP4 (no counterpart in the reference).
  * scale = fl(max(max|x|, 1e-12) / 448), code = e4m3(fl(x * fl(448 / max))), to nearest, ties to even; a value stands for code * scale.
  * quantize_fp8: x [x_rows, K] (dtype as above, rows x_stride elements apart) -> codes u8 [rows, K] with rows codes_stride bytes apart, scales f32 [rows,
- * ceil(K/128)]: one per 128 values of a row. Row r is source row src_row[r] (null: r, and rows == x_rows); one outside 0..x_rows-1 gives zero codes and scales.
+ * ceil(K/128)]: one per 128 values of a row. Row r is source row src_row[r] (null: r, and rows == x_rows); one outside 0..x_rows-1 gives zero codes and scales. The
+ * workspace is for calls with src_row (null where the size is 0) and holds nothing between calls.
  * quantize_fp8_blocks: w [E, N, K] contiguous -> codes u8 [E, N, K] (rows codes_stride bytes apart), scales f32 [E, ceil(N/128), ceil(K/128)]: one per 128x128. */
+long long b200moe_quantize_fp8_workspace_bytes(int x_rows, int rows, int K);
 int b200moe_quantize_fp8(const void* x, int dtype, long long x_stride, int x_rows, const int* src_row, int rows, int K, void* codes, long long codes_stride,
-                         float* scales, void* stream);
+                         float* scales, void* workspace, long long workspace_bytes, void* stream);
 int b200moe_quantize_fp8_blocks(const void* w, int dtype, int E, int N, int K, void* codes, long long codes_stride, float* scales, void* stream);
 /* matmul_fp8: out [M, N] (out_dtype as above, rows out_stride elements apart) = a x w^T of such codes: a u8 [M, K] with a_scales f32 [M, ceil(K/128)], w u8
  * [N, K] with w_scales f32 [ceil(N/128), ceil(K/128)]. Codes start on 16 bytes and their row strides (bytes) are multiples of 16; M, N, K are any sizes.

@@ -84,7 +84,8 @@ SIGNATURES = {
     "b200moe_balance_workspace_bytes": (_LL, [_I, _I]),
     "b200moe_balance_loss": (_I, [_P, _I, _LL, _I, _I, _P, _I, _P, _P, _P, _P, _LL, _P]),
     "b200moe_balance_backward": (_I, [_P, _P, _I, _LL, _I, _I, _P, _I, _P, _P, _P, _P]),
-    "b200moe_quantize_fp8": (_I, [_P, _I, _LL, _I, _P, _I, _I, _P, _LL, _P, _P]),
+    "b200moe_quantize_fp8_workspace_bytes": (_LL, [_I, _I, _I]),
+    "b200moe_quantize_fp8": (_I, [_P, _I, _LL, _I, _P, _I, _I, _P, _LL, _P, _P, _LL, _P]),
     "b200moe_quantize_fp8_blocks": (_I, [_P, _I, _I, _I, _I, _P, _LL, _P, _P]),
     "b200moe_matmul_fp8": (_I, [_P, _LL, _P, _P, _LL, _P, _I, _I, _I, _P, _I, _LL, _P]),
     "b200moe_matmul_fp8_experts": (_I, [_P, _LL, _P, _I, _P, _LL, _P, _I, _P, _P, _I, _I, _I, _P, _I, _LL, _I, _P]),
@@ -142,7 +143,7 @@ def host():
         if module is not NO_HOST:
             module.bind(*(C.cast(f, C.c_void_p).value for f in (h.b200moe_quantize_nvfp4_own_scale, h.b200moe_quantize_nvfp4)), ONE_CLUSTER)
             module.bind_ops(*(C.cast(f, C.c_void_p).value for f in (
-                h.b200moe_gate, h.b200moe_gate_backward, h.b200moe_balance_workspace_bytes, h.b200moe_balance_loss, h.b200moe_balance_backward, h.b200moe_quantize_fp8,
+                h.b200moe_gate, h.b200moe_gate_backward, h.b200moe_balance_workspace_bytes, h.b200moe_balance_loss, h.b200moe_balance_backward, h.b200moe_quantize_fp8_workspace_bytes, h.b200moe_quantize_fp8,
                 h.b200moe_matmul_fp8, h.b200moe_matmul_fp8_experts, h.b200moe_error_string)))
         _host = module
     return _host

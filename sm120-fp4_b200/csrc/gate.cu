@@ -64,24 +64,39 @@ __device__ __forceinline__ float warp_sum(float v) {
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-__device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
+__device__ __forceinline__ float warp_max(float v) {      // NaN where a lane has one
+  float m;
+  asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+  return m;
+}
+// Softmax numerator exp(x - m) as 2^((x - m) log2(e)): the difference, the product and log2(e) are off by 2^-24, 2^-24 and 2^-26 of |x - m|, relative in the
+// result, ex2 by 2^-22. (x log2(e) - m log2(e) in one fma has one rounding less, and overflows where logits are near their type's largest value.)
+constexpr float kLog2e = 1.4426950408889634f;
+__device__ __forceinline__ float exp_term(float x, float m) {
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"((x - m) * kLog2e));
+  return e;
 }
 
-// Softmax numerators against the row's maximum and their sum. Rows of -inf alone: zeros, sum 0. An infinity or a NaN makes the row NaN.
-template <int V>
-__device__ __forceinline__ float softmax_terms(const float (&x)[V], float (&p)[V]) {
-  float m = -INFINITY;
+// Softmax numerators of kTok rows against their maxima, and the lane's share of their sums. Rows of -inf alone: zeros. An infinity or a NaN makes its row NaN.
+template <int V, int kTok>
+__device__ __forceinline__ void softmax_terms(float (&x)[kTok][V], float (&s)[kTok]) {
+  float m[kTok];
 #pragma unroll
-  for (int j = 0; j < V; ++j) m = max_nan(m, x[j]);
-  m = warp_max(m);
-  if (m == -INFINITY) m = 0.f;
-  float s = 0.f;
+  for (int i = 0; i < kTok; ++i) {
+    m[i] = x[i][0];
 #pragma unroll
-  for (int j = 0; j < V; ++j) p[j] = expf(x[j] - m), s += p[j];
-  return warp_sum(s);
+    for (int j = 1; j < V; ++j) m[i] = max_nan(m[i], x[i][j]);
+  }
+#pragma unroll
+  for (int i = 0; i < kTok; ++i) m[i] = warp_max(m[i]);
+#pragma unroll
+  for (int i = 0; i < kTok; ++i) {
+    const float c = m[i] == -INFINITY ? 0.f : m[i];
+    s[i] = 0.f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) x[i][j] = exp_term(x[i][j], c), s[i] += x[i][j];
+  }
 }
 
 // An unsigned number in the order of the logits: NaN above all, -0 = +0. 0 is left for experts that are not there.
@@ -96,48 +111,99 @@ __device__ __forceinline__ float key_value(uint32_t k) {
 }
 constexpr uint32_t kKeyMasked = 0x007fffffu;      // order_key(-inf)
 
+// A lane's candidates in falling order. Types of 16 bits leave nine low bits of the key free: it carries the index (turned over: the lower one wins a tie), and
+// one reduction over the warp gives both. In 32 bits the index is kept beside the key, and the lowest lane that holds the largest key has the lowest index.
+template <int V, bool kPacked> struct Candidates {
+  uint32_t key[V];
+  uint32_t idx[kPacked ? 1 : V];
+  __device__ __forceinline__ void order(int a, int b) {      // a's before b's
+    if constexpr (kPacked) {
+      const uint32_t hi = max(key[a], key[b]), lo = min(key[a], key[b]);
+      key[a] = hi, key[b] = lo;
+    } else {
+      const bool turn = key[a] < key[b] || (key[a] == key[b] && idx[a] > idx[b]);
+      const uint32_t k = key[a], i = idx[a];
+      key[a] = turn ? key[b] : k, key[b] = turn ? k : key[b];
+      idx[a] = turn ? idx[b] : i, idx[b] = turn ? i : idx[b];
+    }
+  }
+  // Batcher's odd-even merge sort of key[kFrom .. kFrom + kCount - 1]
+  template <int kFrom, int kCount, int kStep> __device__ __forceinline__ void merge() {
+    if constexpr (2 * kStep < kCount) {
+      merge<kFrom, kCount, 2 * kStep>();
+      merge<kFrom + kStep, kCount, 2 * kStep>();
+#pragma unroll
+      for (int i = kFrom + kStep; i + kStep < kFrom + kCount; i += 2 * kStep) order(i, i + kStep);
+    } else {
+      order(kFrom, kFrom + kStep);
+    }
+  }
+  template <int kFrom, int kCount> __device__ __forceinline__ void sort() {
+    if constexpr (kCount > 1) {
+      sort<kFrom, kCount / 2>();
+      sort<kFrom + kCount / 2, kCount / 2>();
+      merge<kFrom, kCount, 1>();
+    }
+  }
+  __device__ __forceinline__ void pop(bool mine) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      key[i] = mine ? (i + 1 < V ? key[i + 1 < V ? i + 1 : i] : 0u) : key[i];
+      if constexpr (!kPacked)
+        if (i + 1 < V) idx[i] = mine ? idx[i + 1 < V ? i + 1 : i] : idx[i];
+    }
+  }
+};
+
+// Bound by the issue of about 150 instructions a token (eight of 128 experts; a scan of all candidates in every round took twice as many).
 template <typename T, int V, bool kVec>
 __global__ void __launch_bounds__(256) k_gate(const T* __restrict__ logits, long long stride, int tokens, int E, int k, int renorm, float* __restrict__ weights,
                                               int* __restrict__ ids) {
+  constexpr bool kPacked = Elem<T>::kSize == 2;
   const int lane = threadIdx.x & 31;
   grid_dependency_wait();
   const int t = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   if (t >= tokens) return;
   float x[V];
   load_row<T, V, kVec>(logits + (long long)t * stride, E, lane, x, -INFINITY);
-  uint32_t key[V];
+  Candidates<V, kPacked> c;
 #pragma unroll
-  for (int j = 0; j < V; ++j) key[j] = lane * V + j < E ? order_key(x[j]) : 0u;
+  for (int j = 0; j < V; ++j) {
+    const int e = lane * V + j;
+    c.key[j] = e < E ? order_key(x[j]) : 0u;
+    if constexpr (kPacked) c.key[j] = e < E ? (c.key[j] & ~511u) | (511 - e) : 0u;
+    else c.idx[j] = e;
+  }
+  c.template sort<0, V>();
   uint32_t mine = 0u;      // lane j: key and index of the j-th largest
   int at = -1;
   for (int j = 0; j < k; ++j) {
-    uint32_t best = 0u;
-    int bi = 0;
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (key[i] > best) best = key[i], bi = i;
-    const uint32_t top = __reduce_max_sync(0xffffffffu, best);
-    const int src = __ffs(__ballot_sync(0xffffffffu, best == top)) - 1;
-    const int e = __shfl_sync(0xffffffffu, lane * V + bi, src);
-    if (lane == j) mine = top, at = e;
-    if (lane == src) {
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (i == bi) key[i] = 0u;
+    const uint32_t top = __reduce_max_sync(0xffffffffu, c.key[0]);
+    if constexpr (kPacked) {
+      if (lane == j) mine = top;
+      c.pop(c.key[0] == top);
+    } else {
+      const int src = __ffs(__ballot_sync(0xffffffffu, c.key[0] == top)) - 1;
+      const int e = __shfl_sync(0xffffffffu, c.idx[0], src);
+      if (lane == j) mine = top, at = e;
+      c.pop(lane == src);
     }
+  }
+  if constexpr (kPacked) {      // the bits that carried the index were zeros in numbers from 0 on, ones below
+    at = 511 - (int)(mine & 511u);
+    mine = mine >= 0xfffffe00u ? 0xffffffffu : mine & 0x80000000u ? mine & ~511u : mine | 511u;
   }
   const bool live = lane < k && mine > kKeyMasked;
   const uint32_t first = __shfl_sync(0xffffffffu, mine, 0);
   const float m = first <= kKeyMasked ? 0.f : key_value(first);
-  float w = live ? expf(key_value(mine) - m) : 0.f, s;
-  if (renorm) {
-    s = warp_sum(w);
-  } else {
+  const float w = live ? exp_term(key_value(mine), m) : 0.f;
+  float s = w;
+  if (!renorm) {
     s = 0.f;
 #pragma unroll
-    for (int j = 0; j < V; ++j) s += expf(x[j] - m);
-    s = warp_sum(s);
+    for (int j = 0; j < V; ++j) s += exp_term(x[j], m);
   }
+  s = warp_sum(s);
   if (lane < k) {
     weights[(long long)t * k + lane] = live ? w / s : 0.f;
     ids[(long long)t * k + lane] = live ? at : -1;
@@ -164,12 +230,13 @@ __global__ void __launch_bounds__(256) k_gate_backward(const float* __restrict__
 #pragma unroll
     for (int j = 0; j < V; ++j) d[j] = 0.f;
   } else {
-    float x[V];
-    load_row<T, V, kVec>(logits + (long long)t * stride, E, lane, x, -INFINITY);
-    const float s = softmax_terms<V>(x, d);
-    const float c = s == 0.f ? 0.f : -dot / s;
+    float x[1][V], s[1];
+    load_row<T, V, kVec>(logits + (long long)t * stride, E, lane, x[0], -INFINITY);
+    softmax_terms<V, 1>(x, s);
+    s[0] = warp_sum(s[0]);
+    const float c = s[0] == 0.f ? 0.f : -dot / s[0];
 #pragma unroll
-    for (int j = 0; j < V; ++j) d[j] *= c;
+    for (int j = 0; j < V; ++j) d[j] = x[0][j] * c;
   }
   T* row = out + (long long)t * E;
   store_row<T, V, kVec>(row, E, lane, d);
@@ -182,15 +249,21 @@ __global__ void __launch_bounds__(256) k_gate_backward(const float* __restrict__
 // launch adds the blocks in order. part: per block E floats, E ints, live tokens.
 __host__ __device__ inline int balance_words(int E) { return 2 * E + 4; }
 
-constexpr int kBalanceWarps = 16, kBalanceRanks = 8;
+// Up to 256 experts a warp has two tokens in hand, so that the chains load -> maximum -> sum overlap.
+constexpr int kBalanceRanks = 8;
+template <int V> struct BalanceShape {
+  static constexpr int kWarps = V <= 8 ? 32 : 16, kTok = V <= 8 ? 2 : 1;      // 32 KB of partial sums
+};
+constexpr int kBalanceBlocks = 148;
 
 template <typename T, int V, bool kVec>
-__global__ void __launch_bounds__(kBalanceWarps * 32) k_balance_part(const T* __restrict__ logits, long long stride, int tokens, int E, const int* __restrict__ ids, int k,
-                                                                     float* __restrict__ part) {
-  __shared__ float sp[kBalanceWarps][32 * V];
+__global__ void __launch_bounds__(BalanceShape<V>::kWarps * 32) k_balance_part(const T* __restrict__ logits, long long stride, int tokens, int E, const int* __restrict__ ids,
+                                                                               int k, float* __restrict__ part) {
+  constexpr int kWarps = BalanceShape<V>::kWarps, kTok = BalanceShape<V>::kTok;
+  __shared__ float sp[kWarps][32 * V];
   __shared__ int cnt[32 * V], live_n;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int i = threadIdx.x; i < 32 * V; i += kBalanceWarps * 32) cnt[i] = 0;
+  for (int i = threadIdx.x; i < 32 * V; i += kWarps * 32) cnt[i] = 0;
   if (threadIdx.x == 0) live_n = 0;
   __syncthreads();
   grid_dependency_wait();
@@ -198,84 +271,105 @@ __global__ void __launch_bounds__(kBalanceWarps * 32) k_balance_part(const T* __
 #pragma unroll
   for (int j = 0; j < V; ++j) acc[j] = 0.f;
   int n = 0;
-  for (int t = blockIdx.x * kBalanceWarps + warp; t < tokens; t += gridDim.x * kBalanceWarps) {
-    const int e = lane < k ? ids[(long long)t * k + lane] : -1;
-    float x[V], p[V];
-    load_row<T, V, kVec>(logits + (long long)t * stride, E, lane, x, -INFINITY);
-    const bool used = e >= 0 && e < E;
-    if (used) atomicAdd(&cnt[e], 1);
-    if (!__any_sync(0xffffffffu, used)) continue;      // an empty token
-    ++n;
-    const float s = softmax_terms<V>(x, p);
-    const float r = s == 0.f ? 0.f : 1.f / s;
+  const int step = gridDim.x * kWarps * kTok;
+  for (int t0 = (blockIdx.x * kWarps + warp) * kTok; t0 < tokens; t0 += step) {
+    float x[kTok][V], s[kTok];
+    int e[kTok];
 #pragma unroll
-    for (int j = 0; j < V; ++j) acc[j] = fmaf(p[j], r, acc[j]);
+    for (int i = 0; i < kTok; ++i) {
+      const bool in = t0 + i < tokens;
+      e[i] = in && lane < k ? ids[(long long)(t0 + i) * k + lane] : -1;
+      load_row<T, V, kVec>(logits + (long long)(in ? t0 + i : t0) * stride, E, lane, x[i], -INFINITY);
+    }
+    bool live[kTok];
+#pragma unroll
+    for (int i = 0; i < kTok; ++i) {
+      const bool used = e[i] >= 0 && e[i] < E;
+      if (used) atomicAdd(&cnt[e[i]], 1);
+      live[i] = __any_sync(0xffffffffu, used);      // else an empty token
+      n += live[i];
+    }
+    softmax_terms<V, kTok>(x, s);
+#pragma unroll
+    for (int o = 16; o; o >>= 1)
+#pragma unroll
+      for (int i = 0; i < kTok; ++i) s[i] += __shfl_xor_sync(0xffffffffu, s[i], o);
+#pragma unroll
+    for (int i = 0; i < kTok; ++i) {
+      if (!live[i]) continue;
+      const float r = s[i] == 0.f ? 0.f : __frcp_rn(s[i]);
+#pragma unroll
+      for (int j = 0; j < V; ++j) acc[j] = fmaf(x[i][j], r, acc[j]);
+    }
   }
   if (lane == 0 && n) atomicAdd(&live_n, n);
 #pragma unroll
   for (int j = 0; j < V; ++j) sp[warp][lane * V + j] = acc[j];
   __syncthreads();
   float* o = part + (long long)blockIdx.x * balance_words(E);
-  for (int e = threadIdx.x; e < E; e += kBalanceWarps * 32) {
+  for (int e = threadIdx.x; e < E; e += kWarps * 32) {
     float s = 0.f;
 #pragma unroll
-    for (int i = 0; i < kBalanceWarps; ++i) s += sp[i][e];
+    for (int i = 0; i < kWarps; ++i) s += sp[i][e];
     o[e] = s;
     reinterpret_cast<int*>(o)[E + e] = cnt[e];
   }
   if (threadIdx.x == 0) reinterpret_cast<int*>(o)[2 * E] = live_n;
 }
 
-// One cluster: a block takes an eighth of the experts, its threads eight shares of the partial sums (loads of eight in flight); the sums of the
-// experts meet in block 0. stats: f32 [2]: 1 / pairs, E / live tokens (the larger of it and 1 in both quotients).
-__global__ void __cluster_dims__(kBalanceRanks, 1, 1) __launch_bounds__(512)
-    k_balance_sum(const float* __restrict__ part, int blocks, int E, float* __restrict__ loss, int* __restrict__ counts, float* __restrict__ stats) {
-  __shared__ double sp[8][64];
-  __shared__ int sc[8][64];
+// One cluster: a block takes an eighth of the experts, a column of threads for each, every thread of which adds one of `slices` shares of the partial sums (148 at
+// most: loads of a thread are in flight together); the experts' sums meet in block 0. stats: f32 [2]: 1 / pairs, E / live tokens (at least 1 of both).
+__global__ void __cluster_dims__(kBalanceRanks, 1, 1) __launch_bounds__(1024)
+    k_balance_sum(const float* __restrict__ part, int blocks, int E, int log_cols, float* __restrict__ loss, int* __restrict__ counts, float* __restrict__ stats) {
+  __shared__ double sp[1024];
+  __shared__ int sc[1024];
   __shared__ double rank_v[kBalanceRanks];      // of block 0: every block's sum of products
   __shared__ long long rank_n[kBalanceRanks];
   __shared__ int live_s;
-  const int tid = threadIdx.x, col = tid & 63, slice = tid >> 6, rank = blockIdx.x;
-  const int per = (E + kBalanceRanks - 1) / kBalanceRanks, e = rank * per + col;
-  const long long W = balance_words(E);
+  const int tid = threadIdx.x, cols = 1 << log_cols, col = tid & (cols - 1), slice = tid >> log_cols, slices = 1024 >> log_cols, rank = blockIdx.x;
+  const int per = (E + kBalanceRanks - 1) / kBalanceRanks, e = rank * per + col, W = balance_words(E);
   grid_dependency_wait();
   double p = 0.0;
   int c = 0;
   const bool mine = col < per && e < E;
   if (mine) {
-    for (int b0 = slice; b0 < blocks; b0 += 64) {
-      float pv[8];
-      int cv[8];
+    for (int b0 = slice; b0 < blocks; b0 += slices * 10) {
+      float pv[10];
+      int cv[10];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int b = b0 + 8 * i;
+      for (int i = 0; i < 10; ++i) {
+        const int b = b0 + slices * i;
         pv[i] = b < blocks ? part[b * W + e] : 0.f;
         cv[i] = b < blocks ? reinterpret_cast<const int*>(part)[b * W + E + e] : 0;
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) p += (double)pv[i], c += cv[i];
+      for (int i = 0; i < 10; ++i) p += (double)pv[i], c += cv[i];
     }
   }
-  sp[slice][col] = p, sc[slice][col] = c;
-  if (rank == 0 && tid < 32) {
+  sp[tid] = p, sc[tid] = c;
+  if (rank == 0 && tid >= 992) {
     int l = 0;
-    for (int b = tid; b < blocks; b += 32) l += reinterpret_cast<const int*>(part)[b * W + 2 * E];
+    for (int b = tid - 992; b < blocks; b += 32) l += reinterpret_cast<const int*>(part)[b * W + 2 * E];
     l = __reduce_add_sync(0xffffffffu, l);
-    if (tid == 0) live_s = l;
+    if (tid == 992) live_s = l;
   }
   __syncthreads();
-  if (tid < 64) {
-#pragma unroll
-    for (int i = 1; i < 8; ++i) p += sp[i][tid], c += sc[i][tid];
-    if (mine) counts[e] = c;
-    double v = p * (double)c;
-    long long n = c;
+  if (tid < 64) {      // (cols <= 64)
+    double v = 0.0;
+    long long n = 0;
+    if (tid < cols) {
+      for (int i = 1; i < slices; ++i) p += sp[i * cols + tid], c += sc[i * cols + tid];
+      if (mine) counts[e] = c;
+      v = p * (double)c, n = c;
+    }
 #pragma unroll
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o), n += __shfl_xor_sync(0xffffffffu, n, o);
-    if (tid == 32) sp[0][0] = v, sc[1][0] = (int)n, sc[2][0] = (int)(n >> 32);
+    __syncwarp();
+    named_bar_sync(1, 64);      // everybody has read sp and sc
+    if (tid == 32) sp[0] = v, sc[0] = (int)(n & 0xffffffffll), sc[1] = (int)(n >> 32);
     named_bar_sync(1, 64);
     if (tid == 0) {
-      v += sp[0][0], n += (long long)(((unsigned long long)(unsigned)sc[2][0] << 32) | (unsigned)sc[1][0]);
+      v += sp[0], n += (long long)(((unsigned long long)(unsigned)sc[1] << 32) | (unsigned)sc[0]);
       asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(mapa_shared(smem_u32(&rank_v[rank]), 0)), "d"(v) : "memory");
       asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(mapa_shared(smem_u32(&rank_n[rank]), 0)), "l"(n) : "memory");
     }
@@ -302,25 +396,36 @@ __global__ void __launch_bounds__(256) k_balance_backward(const float* __restric
   float f[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) f[j] = lane * V + j < E ? (float)counts[lane * V + j] * inv : 0.f;
-  for (int t = blockIdx.x * 8 + (threadIdx.x >> 5); t < tokens; t += gridDim.x * 8) {
-    const int e = lane < k ? ids[(long long)t * k + lane] : -1;
-    float d[V];
-    if (__any_sync(0xffffffffu, e >= 0 && e < E)) {
-      float x[V];
-      load_row<T, V, kVec>(logits + (long long)t * stride, E, lane, x, -INFINITY);
-      const float s = softmax_terms<V>(x, d);
-      const float r = s == 0.f ? 0.f : 1.f / s;
-      float dot = 0.f;
+  constexpr int kTok = BalanceShape<V>::kTok;
+  const int step = gridDim.x * 8 * kTok;
+  for (int t0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * kTok; t0 < tokens; t0 += step) {
+    float x[kTok][V], s[kTok], dot[kTok];
+    int e[kTok];
 #pragma unroll
-      for (int j = 0; j < V; ++j) d[j] *= r, dot = fmaf(d[j], f[j], dot);
-      dot = warp_sum(dot);
-#pragma unroll
-      for (int j = 0; j < V; ++j) d[j] *= (f[j] - dot) * c;
-    } else {
-#pragma unroll
-      for (int j = 0; j < V; ++j) d[j] = 0.f;
+    for (int i = 0; i < kTok; ++i) {
+      const bool in = t0 + i < tokens;
+      e[i] = in && lane < k ? ids[(long long)(t0 + i) * k + lane] : -1;
+      load_row<T, V, kVec>(logits + (long long)(in ? t0 + i : t0) * stride, E, lane, x[i], -INFINITY);
     }
-    store_row<T, V, kVec>(out + (long long)t * E, E, lane, d);
+    softmax_terms<V, kTok>(x, s);
+#pragma unroll
+    for (int i = 0; i < kTok; ++i) {
+      dot[i] = 0.f;
+#pragma unroll
+      for (int j = 0; j < V; ++j) dot[i] = fmaf(x[i][j], f[j], dot[i]);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1)
+#pragma unroll
+      for (int i = 0; i < kTok; ++i) s[i] += __shfl_xor_sync(0xffffffffu, s[i], o), dot[i] += __shfl_xor_sync(0xffffffffu, dot[i], o);
+#pragma unroll
+    for (int i = 0; i < kTok; ++i) {
+      const bool live = __any_sync(0xffffffffu, e[i] >= 0 && e[i] < E);
+      const float r = s[i] == 0.f ? 0.f : __frcp_rn(s[i]), mean = dot[i] * r, rc = r * c;
+#pragma unroll
+      for (int j = 0; j < V; ++j) x[i][j] = live ? x[i][j] * rc * (f[j] - mean) : 0.f;
+      if (t0 + i < tokens) store_row<T, V, kVec>(out + (long long)(t0 + i) * E, E, lane, x[i]);
+    }
   }
 }
 
@@ -341,9 +446,9 @@ static bool vec_rows(const void* p, long long stride, int E, int size) {      //
   const int unit = E <= 128 && size == 2 ? 8 : 16;
   return ((uintptr_t)p % unit) == 0 && (stride * size) % unit == 0 && ((long long)E * size) % unit == 0;
 }
-static int balance_blocks(int tokens) {
-  const int want = (tokens + kBalanceWarps - 1) / kBalanceWarps;
-  return want < 296 ? want : 296;
+static int balance_blocks(int tokens) {      // 16 tokens or more each
+  const int want = (tokens + 15) / 16;
+  return want < kBalanceBlocks ? want : kBalanceBlocks;
 }
 
 }  // namespace b200
@@ -416,13 +521,15 @@ int b200moe_balance_loss(const void* logits, int dtype, long long stride, int to
       const T* lp = (const T*)logits;
       void* args[] = {&lp, &stride, &tokens, &E, &ids, &k, &part};
       const void* fn = vec_rows(logits, stride, E, sizeof(T)) ? (const void*)k_balance_part<T, V, true> : (const void*)k_balance_part<T, V, false>;
-      return launch_kernel(fn, blocks, kBalanceWarps * 32, 0, true, args, (cudaStream_t)stream);
+      return launch_kernel(fn, blocks, BalanceShape<V>::kWarps * 32, 0, true, args, (cudaStream_t)stream);
     });
   });
   if (rc) return rc;
   const float* cp = part;
-  void* args[] = {&cp, &blocks, &E, &loss, &counts, &stats};
-  return launch_kernel((const void*)k_balance_sum, kBalanceRanks, 512, 0, true, args, (cudaStream_t)stream);
+  int log_cols = 0;      // columns of a block: the power of two from its eighth of the experts on
+  while ((1 << log_cols) < (E + kBalanceRanks - 1) / kBalanceRanks) ++log_cols;
+  void* args[] = {&cp, &blocks, &E, &log_cols, &loss, &counts, &stats};
+  return launch_kernel((const void*)k_balance_sum, kBalanceRanks, 1024, 0, true, args, (cudaStream_t)stream);
 }
 
 int b200moe_balance_backward(const float* grad_loss, const void* logits, int dtype, long long stride, int tokens, int E, const int* ids, int k, const int* counts,

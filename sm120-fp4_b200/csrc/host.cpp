@@ -129,7 +129,8 @@ struct Ops {
   long long (*balance_workspace_bytes)(int, int);
   int (*balance_loss)(const void*, int, long long, int, int, const void*, int, void*, void*, void*, void*, long long, void*);
   int (*balance_backward)(const void*, const void*, int, long long, int, int, const void*, int, const void*, const void*, void*, void*);
-  int (*quantize_fp8)(const void*, int, long long, int, const void*, int, int, void*, long long, void*, void*);
+  long long (*quantize_fp8_workspace_bytes)(int, int, int);
+  int (*quantize_fp8)(const void*, int, long long, int, const void*, int, int, void*, long long, void*, void*, long long, void*);
   int (*matmul_fp8)(const void*, long long, const void*, const void*, long long, const void*, int, int, int, void*, int, long long, void*);
   int (*matmul_fp8_experts)(const void*, long long, const void*, int, const void*, long long, const void*, int, const void*, const void*, int, int, int, void*, int, long long,
                             int, void*);
@@ -304,8 +305,10 @@ PyObject* py_quantize_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
   {
     Released released;
     codes = at::empty_strided({rows, k}, {ld, 1}, at::TensorOptions().dtype(at::kFloat8_e4m3fn).device(x.device())), scales = fresh({rows, (k + 127) / 128}, at::kFloat, x);
+    const long long bytes = src.defined() ? ops.quantize_fp8_workspace_bytes((int)x.size(0), (int)rows, (int)k) : 0;
+    const at::Tensor ws = bytes > 0 ? fresh({bytes / 4}, at::kInt, x) : at::Tensor();
     rc = ops.quantize_fp8(x.data_ptr(), dtype_code(x.scalar_type()), x.size(0) > 1 ? x.stride(0) : ld, (int)x.size(0), src.defined() ? src.data_ptr() : nullptr, (int)rows, (int)k,
-                          codes.data_ptr(), ld, scales.data_ptr(), stream());
+                          codes.data_ptr(), ld, scales.data_ptr(), bytes > 0 ? ws.data_ptr() : nullptr, bytes, stream());
   }
   return pair(rc, codes, scales);
   END_HANDLE_TH_ERRORS

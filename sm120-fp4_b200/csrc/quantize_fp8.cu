@@ -7,6 +7,8 @@
 
 namespace b200 {
 
+constexpr long long kListValues = 1 << 22;
+
 // Rows, 16 bytes at a time: K and both row strides are multiples of 16 values, so that a lane's 16 values are whole. Eight lanes share a
 // group of 128; a lane whose values lie beyond K (the last group of a row) takes part in the maximum with zeros.
 template <typename T>
@@ -47,6 +49,65 @@ __global__ void __launch_bounds__(256) k_quantize_fp8_rows(const T* __restrict__
       *reinterpret_cast<uint4*>(codes + (long long)row * ldc + c) = q;
     }
     if ((threadIdx.x & 7) == 0) scales[(long long)row * KB + g] = gone ? 0.f : s.scale;
+  }
+}
+
+// Rows that are asked for several times (a token's copies for its experts): each source row is read and quantised once and its codes are stored to all of its
+// destinations, which hang on a list per source row: head i32 [x_rows], next i32 [rows], made by two small kernels. The order of a list is that of the atomics,
+// and does not matter: every destination gets the same bytes. Reading the source once per destination took 47 us for 4096 rows of 2816 eight times over (184 MB out
+// of L2); the destinations' 92 MB are what HBM has to take.
+__global__ void __launch_bounds__(256) k_no_heads(int* __restrict__ head, int x_rows) {
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i < x_rows) head[i] = -1;
+}
+__global__ void __launch_bounds__(256) k_link_rows(const int* __restrict__ src_row, int rows, int x_rows, int K, int* __restrict__ head, int* __restrict__ next,
+                                                   uint8_t* __restrict__ codes, long long ldc, float* __restrict__ scales) {
+  const int r = blockIdx.x * 256 + threadIdx.x, lane = threadIdx.x & 31, KB = (K + 127) >> 7;
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int s = r < rows ? src_row[r] : 0;
+  const bool gone = r < rows && (s < 0 || s >= x_rows);
+  if (r < rows && !gone) next[r] = atomicExch(head + s, r);
+  for (unsigned todo = __ballot_sync(0xffffffffu, gone); todo; todo &= todo - 1) {      // empty rows: zeros, by the whole warp
+    const long long e = r - lane + __ffs(todo) - 1;
+    for (int i = lane; i < K / 16; i += 32) *reinterpret_cast<uint4*>(codes + e * ldc + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+    for (int i = lane; i < KB; i += 32) scales[e * KB + i] = 0.f;
+  }
+}
+template <typename T>
+__global__ void __launch_bounds__(256) k_quantize_fp8_copies(const T* __restrict__ x, long long ldx, int x_rows, int K, const int* __restrict__ head, const int* __restrict__ next,
+                                                             uint8_t* __restrict__ codes, long long ldc, float* __restrict__ scales) {
+  constexpr int W = 16 * Elem<T>::kSize / 16;
+  const int KB = (K + 127) >> 7, quads = (KB + 3) >> 2;      // a warp takes four groups of a row
+  const long long u = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int row = (int)(u / quads), g = (int)(u - (long long)row * quads) * 4 + (threadIdx.x >> 3 & 3), c = g * 128 + (threadIdx.x & 7) * 16;
+  grid_dependency_wait();
+  grid_launch_dependents();
+  if (row >= x_rows) return;      // (whole warps)
+  uint4 w[W];
+#pragma unroll
+  for (int i = 0; i < W; ++i) w[i] = c < K ? *(reinterpret_cast<const uint4*>(x + (long long)row * ldx + c) + i) : make_uint4(0u, 0u, 0u, 0u);
+  int r = head[row];
+  float v[16], m = 0.f;
+#pragma unroll
+  for (int i = 0; i < W; ++i) unpack16<T>(w[i], v + i * (16 / W));
+#pragma unroll
+  for (int i = 0; i < 16; ++i) m = max_nan(m, fabsf(v[i]));
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const Fp8Scale s = fp8_scale(m);
+  uint4 q;
+  q.x = cvt_e4m3x4(v[0] * s.factor, v[1] * s.factor, v[2] * s.factor, v[3] * s.factor);
+  q.y = cvt_e4m3x4(v[4] * s.factor, v[5] * s.factor, v[6] * s.factor, v[7] * s.factor);
+  q.z = cvt_e4m3x4(v[8] * s.factor, v[9] * s.factor, v[10] * s.factor, v[11] * s.factor);
+  q.w = cvt_e4m3x4(v[12] * s.factor, v[13] * s.factor, v[14] * s.factor, v[15] * s.factor);
+  while (r >= 0) {
+    const int after = next[r];
+    if (c < K) *reinterpret_cast<uint4*>(codes + (long long)r * ldc + c) = q;
+    if ((threadIdx.x & 7) == 0 && g < KB) scales[(long long)r * KB + g] = s.scale;
+    r = after;
   }
 }
 
@@ -146,10 +207,26 @@ __global__ void __launch_bounds__(Elem<T>::kSize == 2 ? 256 : 512) k_quantize_fp
   }
 }
 
+// Copies by lists where rows are asked for twice or more on average and there are enough of them to pay for two more launches.
+static bool by_lists(int x_rows, int rows, int K) { return x_rows > 0 && rows / 2 >= x_rows && (long long)rows * K >= kListValues; }
+
 template <typename T>
-static int quantize_fp8_rows(const void* x, long long ldx, int x_rows, const int* src_row, int rows, int K, void* codes, long long ldc, float* scales, cudaStream_t st) {
+static int quantize_fp8_rows(const void* x, long long ldx, int x_rows, const int* src_row, int rows, int K, void* codes, long long ldc, float* scales, int* lists, cudaStream_t st) {
   const long long units = (long long)rows * ((K + 127) / 128);
   const bool vec = K % 16 == 0 && ldx % (16 / Elem<T>::kSize) == 0 && ldc % 16 == 0 && ((uintptr_t)x & 15) == 0 && ((uintptr_t)codes & 15) == 0;
+  if (vec && lists) {
+    const T* xt = (const T*)x;
+    uint8_t* ct = (uint8_t*)codes;
+    int *head = lists, *next = lists + x_rows;
+    void* a0[] = {&head, &x_rows};
+    if (int rc = launch_kernel((const void*)k_no_heads, (x_rows + 255) / 256, 256, 0, true, a0, st)) return rc;
+    void* a1[] = {&src_row, &rows, &x_rows, &K, &head, &next, &ct, &ldc, &scales};
+    if (int rc = launch_kernel((const void*)k_link_rows, (rows + 255) / 256, 256, 0, true, a1, st)) return rc;
+    const long long warps = (long long)x_rows * ((K + 511) / 512);
+    if (warps > 8ll * 0x7fffffff) return B200MOE_ERR_LIMIT;
+    void* a2[] = {&xt, &ldx, &x_rows, &K, &head, &next, &ct, &ldc, &scales};
+    return launch_kernel((const void*)k_quantize_fp8_copies<T>, (int)((warps + 7) / 8), 256, 0, true, a2, st);
+  }
   const long long blocks = (units + (vec ? 31 : 7)) / (vec ? 32 : 8);
   const void* fn = vec ? (const void*)k_quantize_fp8_rows<T> : (const void*)k_quantize_fp8_rows_any<T>;
   const T* xt = (const T*)x;
@@ -180,19 +257,27 @@ static int quantize_fp8_blocks(const void* w, int E, int N, int K, void* codes, 
 
 extern "C" {
 
+long long b200moe_quantize_fp8_workspace_bytes(int x_rows, int rows, int K) {
+  if (x_rows < 0 || rows < 0 || K < 1) return B200MOE_ERR_ARG;
+  return b200::by_lists(x_rows, rows, K) ? 4ll * ((long long)x_rows + rows) : 0;
+}
+
 int b200moe_quantize_fp8(const void* x, int dtype, long long x_stride, int x_rows, const int* src_row, int rows, int K, void* codes, long long codes_stride,
-                         float* scales, void* stream) {
+                         float* scales, void* workspace, long long workspace_bytes, void* stream) {
   using namespace b200;
   if (rows < 0 || x_rows < 0 || K < 1 || dtype < 0 || dtype > 2 || (x_stride < K && x_rows > 1) || codes_stride < K) return B200MOE_ERR_ARG;
   if (!src_row && rows != x_rows) return B200MOE_ERR_ARG;
   if (rows == 0) return B200MOE_OK;
   if ((!x && x_rows) || !codes || !scales) return B200MOE_ERR_ARG;
   const int size = dtype == DT_F32 ? 4 : 2;
-  if (((uintptr_t)x & (size - 1)) || ((uintptr_t)scales & 3)) return B200MOE_ERR_ARG;
+  if (((uintptr_t)x & (size - 1)) || (((uintptr_t)scales | (uintptr_t)workspace) & 3)) return B200MOE_ERR_ARG;
+  const long long need = src_row ? b200moe_quantize_fp8_workspace_bytes(x_rows, rows, K) : 0;
+  if (need && (!workspace || workspace_bytes < need)) return B200MOE_ERR_WORKSPACE;
   cudaStream_t st = (cudaStream_t)stream;
-  if (dtype == DT_BF16) return quantize_fp8_rows<__nv_bfloat16>(x, x_stride, x_rows, src_row, rows, K, codes, codes_stride, scales, st);
-  if (dtype == DT_F16) return quantize_fp8_rows<__half>(x, x_stride, x_rows, src_row, rows, K, codes, codes_stride, scales, st);
-  return quantize_fp8_rows<float>(x, x_stride, x_rows, src_row, rows, K, codes, codes_stride, scales, st);
+  int* lists = need ? (int*)workspace : nullptr;
+  if (dtype == DT_BF16) return quantize_fp8_rows<__nv_bfloat16>(x, x_stride, x_rows, src_row, rows, K, codes, codes_stride, scales, lists, st);
+  if (dtype == DT_F16) return quantize_fp8_rows<__half>(x, x_stride, x_rows, src_row, rows, K, codes, codes_stride, scales, lists, st);
+  return quantize_fp8_rows<float>(x, x_stride, x_rows, src_row, rows, K, codes, codes_stride, scales, lists, st);
 }
 
 int b200moe_quantize_fp8_blocks(const void* w, int dtype, int E, int N, int K, void* codes, long long codes_stride, float* scales, void* stream) {

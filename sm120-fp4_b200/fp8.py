@@ -54,8 +54,11 @@ def quantize_fp8(x: torch.Tensor, src_row: torch.Tensor | None = None):
     ld = _pad16(k)
     codes = torch.empty_strided((rows, k), (ld, 1), dtype=FP8, device=device)
     scales = torch.empty((rows, _groups(k)), dtype=torch.float32, device=device)
-    _lib.call(device, "quantize_fp8", _lib.lib().b200moe_quantize_fp8, x.data_ptr(), _lib.DTYPES[x.dtype], x.stride(0) if m > 1 else ld, m, _lib.ptr(src_row), rows, k,
-              codes.data_ptr(), ld, scales.data_ptr())
+    h = _lib.lib()
+    nbytes = 0 if src_row is None else h.b200moe_quantize_fp8_workspace_bytes(m, rows, k)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    _lib.call(device, "quantize_fp8", h.b200moe_quantize_fp8, x.data_ptr(), _lib.DTYPES[x.dtype], x.stride(0) if m > 1 else ld, m, _lib.ptr(src_row), rows, k,
+              codes.data_ptr(), ld, scales.data_ptr(), _lib.ptr(ws), nbytes)
     return codes, scales
 
 

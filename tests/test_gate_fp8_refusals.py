@@ -86,10 +86,12 @@ def test_c_abi_refusals():
     assert h.b200moe_balance_loss(p, 0, 8, 4, 8, p, 33, p, p, p, p, 1 << 20, None) == L.ERR_LIMIT
     assert h.b200moe_balance_loss(p, 0, 8, 4, 8, None, 2, p, p, p, p, 1 << 20, None) == L.ERR_ARG
     assert h.b200moe_balance_backward(p, p, 0, 8, 4, 8, p, 2, p, None, p, None) == L.ERR_ARG
-    assert h.b200moe_quantize_fp8(p, 0, 16, 4, None, 5, 16, p, 16, p, None) == L.ERR_ARG      # rows without a source
-    assert h.b200moe_quantize_fp8(p, 0, 16, 4, None, 4, 0, p, 16, p, None) == L.ERR_ARG
-    assert h.b200moe_quantize_fp8(p, 0, 16, 4, None, 4, 16, p, 15, p, None) == L.ERR_ARG
-    assert h.b200moe_quantize_fp8(None, 0, 16, 0, None, 0, 16, None, 16, None, None) == 0
+    assert h.b200moe_quantize_fp8(p, 0, 16, 4, None, 5, 16, p, 16, p, None, 0, None) == L.ERR_ARG      # rows without a source
+    assert h.b200moe_quantize_fp8(p, 0, 16, 4, None, 4, 0, p, 16, p, None, 0, None) == L.ERR_ARG
+    assert h.b200moe_quantize_fp8(p, 0, 16, 4, None, 4, 16, p, 15, p, None, 0, None) == L.ERR_ARG
+    assert h.b200moe_quantize_fp8(None, 0, 16, 0, None, 0, 16, None, 16, None, None, 0, None) == 0
+    assert h.b200moe_quantize_fp8_workspace_bytes(10, 20, 16) == 0 and h.b200moe_quantize_fp8_workspace_bytes(4096, 32768, 2048) == 4 * (4096 + 32768)
+    assert h.b200moe_quantize_fp8(p, 0, 2048, 4096, p, 32768, 2048, p, 2048, p, None, 0, None) == L.ERR_WORKSPACE
     assert h.b200moe_quantize_fp8_blocks(p, 0, 1, 4, 16, None, 16, p, None) == L.ERR_ARG
     assert h.b200moe_matmul_fp8(p, 16, p, p, 16, p, 4, 4, 17, p, 0, 4, None) == L.ERR_ARG      # rows shorter than K
     assert h.b200moe_matmul_fp8(p, 24, p, p, 32, p, 4, 4, 16, p, 0, 4, None) == L.ERR_ARG      # rows that do not start on 16 bytes

@@ -59,6 +59,27 @@ def test_quantize_rows(dtype, m, k):
     assert torch.equal(s2, torch.where(inside[:, None], s[at], torch.zeros(1, device="cuda")))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,copies,k", [(600, 8, 1024), (2000, 2, 2816), (300, 30, 704), (1500, 3, 1040), (4096, 8, 512)])
+def test_quantize_many_copies(dtype, m, copies, k):
+    """Rows that are asked for several times in calls large enough for the lists: some twice as often, some never, some indexes outside."""
+    import sm120fp4_b200 as pkg
+    x = randn(m, k, seed=m + k).to(dtype).cuda()
+    src = torch.randint(-3, m + 3, (m * copies + 5,), generator=torch.Generator().manual_seed(copies)).int()
+    src[:m // 2] = m // 3
+    src = src.cuda()
+    q, s = pkg.quantize_fp8(x)
+    got_q, got_s = pkg.quantize_fp8(x, src_row=src)
+    inside = (src >= 0) & (src < m)
+    at = src.clamp(0, m - 1).long()
+    assert same(got_q, torch.where(inside[:, None], q.float()[at], torch.zeros(1, device="cuda")))
+    assert torch.equal(got_s, torch.where(inside[:, None], s[at], torch.zeros(1, device="cuda")))
+    wide = torch.zeros(m, k + 8, dtype=dtype, device="cuda")[:, 4:4 + k]      # rows that start off 16 bytes: the other way to the same values
+    wide.copy_(x)
+    q2, s2 = pkg.quantize_fp8(wide, src_row=src)
+    assert same(q2, got_q) and torch.equal(s2, got_s)
+
+
 def test_quantize_every_value_of_a_group():
     """Every code and every border between two: values v / 448 of a group whose maximum is 448."""
     import sm120fp4_b200 as pkg

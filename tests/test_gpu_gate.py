@@ -1,7 +1,7 @@
 """GPU parity of the router from logits and of the balance loss: against their formulas in 64 bits, and gradients against differences.
 
-Tolerances count roundings. expf is within 2 ulp (2^-22 relative) and its argument x - m rounded once (|x - m| 2^-24 relative in the result); a sum over E
-is a tree of at most V + 5 additions, V = values of a lane; quotients and products one rounding each."""
+Tolerances count roundings. A softmax numerator is 2^((x - m) log2(e)): the difference's rounding, the product's and log2(e)'s are 2^-24, 2^-24 and 2^-26 of |x - m|
+relative in the result, ex2 is within 2^-22. A sum over E is a tree of at most V + 5 additions, V = values of a lane; quotients and products one rounding each."""
 import math
 
 import pytest
@@ -39,7 +39,7 @@ def spread(x):
 
 def rel_p(x):
     """Relative error of one probability (a quotient of an exponential and a sum of them)."""
-    one = min(spread(x), 104.0) * U + 4 * U      # (exponentials of differences above 104 are zero in fp32)
+    one = 2.25 * min(spread(x), 104.0) * U + 4 * U      # (exponentials of differences above 104 are zero in fp32)
     return 2 * one + (lane_values(x.shape[1]) + 7) * U
 
 
@@ -239,7 +239,7 @@ def test_balance(dtype, t, e, k):
         leaf = x.clone().requires_grad_(True)
         got, got_counts = pkg.balance_loss(leaf, ids)
         assert got.shape == () and torch.equal(got_counts, counts)
-        adds = -(-t // (8 * min(592, -(-t // 8)))) + 8
+        adds = -(-t // (16 * min(148, -(-t // 16)))) + 32      # tokens of a warp one after the other, warps of a block
         tol = (rel_p(x) + (adds + 4) * U)
         assert abs(float(got.double() - loss)) <= tol * float(loss) + 2.0 ** -126
         again = pkg.balance_loss(x, ids)
