@@ -72,28 +72,35 @@ __device__ __forceinline__ bool mbar_ready(uint32_t bar, uint32_t parity) {
   asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
   return __all_sync(0xffffffffu, ok != 0);
 }
+// How many of the next `steps` steps (kPer barriers each, one a lane in order, 32 / kPer steps at most) are ready, one at least; 0 where the wait ran out. A look at a
+// barrier takes 120 cycles; a look at all of them by different lanes takes no longer.
+template <int kPer> __device__ __forceinline__ int mbar_wait_steps(uint32_t bar, uint32_t parity, int steps, int lane, volatile int* abort_flag, uint32_t limit = (1u << 20)) {
+  uint32_t ok = 1;
+  if (lane < steps * kPer)
+    asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  const uint32_t open = ~__ballot_sync(0xffffffffu, ok != 0);
+  const int ready = open ? (__ffs(open) - 1) / kPer : steps;
+  __syncwarp();      // (what a lane has seen holds for all)
+  if (ready) return ready < steps ? ready : steps;
+  for (uint32_t it = 0; it < limit; ++it) {      // the first step: parked in the barrier
+    ok = 1;
+    if (lane < kPer)
+      asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    if (__all_sync(0xffffffffu, ok != 0)) {
+      __syncwarp();
+      return 1;
+    }
+    if ((it & 63u) == 63u && __any_sync(0xffffffffu, *abort_flag != 0)) return 0;
+  }
+  *abort_flag = 1;
+  return 0;
+}
 // mbar_wait_warp with a barrier of its own for each lane that is not done
 __device__ __forceinline__ bool mbar_wait_lanes(uint32_t bar, uint32_t parity, bool done, volatile int* abort_flag, uint32_t limit = (1u << 20)) {
   for (uint32_t it = 0; it < limit; ++it) {
     uint32_t ok = 1;
     if (!done)
       asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-    if (__all_sync(0xffffffffu, ok != 0)) return true;
-    if ((it & 63u) == 63u && __any_sync(0xffffffffu, *abort_flag != 0)) return false;
-  }
-  *abort_flag = 1;
-  return false;
-}
-// mbar_wait_warp for two barriers at once (one vote), what came before their arrivals in the whole cluster visible
-__device__ __forceinline__ bool mbar_wait_both(uint32_t bar0, uint32_t parity0, uint32_t bar1, uint32_t parity1, volatile int* abort_flag, uint32_t limit = (1u << 20)) {
-  for (uint32_t it = 0; it < limit; ++it) {
-    uint32_t ok;
-    asm volatile(
-        "{\n .reg .pred p, q;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 q, [%3], %4;\n"
-        " and.pred p, p, q;\n selp.u32 %0, 1, 0, p;\n}\n"
-        : "=r"(ok)
-        : "r"(bar0), "r"(parity0), "r"(bar1), "r"(parity1)
-        : "memory");
     if (__all_sync(0xffffffffu, ok != 0)) return true;
     if ((it & 63u) == 63u && __any_sync(0xffffffffu, *abort_flag != 0)) return false;
   }
@@ -150,10 +157,17 @@ template <int NT, bool kSwap, bool kPair> struct MmShape {
   static constexpr int kStages = kRing / kStageBytes < 9 ? kRing / kStageBytes : 9;
   static constexpr int kBufs = 512 / NT < 8 ? 512 / NT : 8;       // accumulators in TMEM
   static constexpr int kScaleRow = kSwap ? NT : 132;              // floats of a group's scales
+  static constexpr int kAhead = kBufs < 4 ? kBufs : 4;            // steps looked at together
   static constexpr int kRows = kSwap ? NT : kPair ? 256 : 128, kWeights = kSwap ? 128 : NT;      // of a tile
   static constexpr int kSmem = 1024 + kStages * kStageBytes + kRed + kOut + kBufs * kScaleRow * 4 + 2 * (MM_MAXU + 2) * 4;
   static_assert(kSmem <= 226 * 1024, "shared memory of a CTA");
 };
+
+// First accumulator column of a warp's c-th chunk: its own half of the tile, or (kSwap, where rows may be few) chunks in turn.
+template <int NT, bool kSwap, bool kPair> __device__ __forceinline__ int mm_column(int half, int c) {
+  using S = MmShape<NT, kSwap, kPair>;
+  return kSwap ? (c * (S::kEpi / 4) + half) * S::kChunk : half * S::kCols + c * S::kChunk;
+}
 
 struct MmTile { int row0, row_end, expert, n0; };
 
@@ -309,6 +323,20 @@ template <int DT, bool kAsync> __device__ __forceinline__ void put_rows(const Ma
     }
   }
 }
+// four weights' sums of a row
+__device__ __forceinline__ void put_four(const MatmulParams& p, int row, int n, const float (&o)[4]) {
+  const long long at = (long long)row * p.ldo + n;
+  if (p.out_dtype == DT_F32) {
+    if (p.vec && n + 4 <= p.N) *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + at) = make_float4(o[0], o[1], o[2], o[3]);
+    else put_some<DT_F32>(p.out, at, o, p.N - n);
+  } else if (p.out_dtype == DT_BF16) {
+    if (p.vec && n + 4 <= p.N) *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(p.out) + at) = make_uint2(Elem<__nv_bfloat16>::pack(o[0], o[1]), Elem<__nv_bfloat16>::pack(o[2], o[3]));
+    else put_some<DT_BF16>(p.out, at, o, p.N - n);
+  } else {
+    if (p.vec && n + 4 <= p.N) *reinterpret_cast<uint2*>(reinterpret_cast<__half*>(p.out) + at) = make_uint2(Elem<__half>::pack(o[0], o[1]), Elem<__half>::pack(o[2], o[3]));
+    else put_some<DT_F16>(p.out, at, o, p.N - n);
+  }
+}
 // This CTA's share of a tile whose inner size is split: 1 / kRanks of it, the sums of all ranks, added in rank order. A thread takes four weights of a row at a
 // time; all of its loads from the ranks' shared memory are in flight together.
 template <int NT, int kRanks>
@@ -333,17 +361,7 @@ __device__ __forceinline__ void mm_add_ranks(const MatmulParams& p, const MmTile
     float o[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int r = 0; r < kRanks; ++r) o[0] += v[j][r].x, o[1] += v[j][r].y, o[2] += v[j][r].z, o[3] += v[j][r].w;
-    const long long at = (long long)row * p.ldo + n;
-    if (p.out_dtype == DT_F32) {
-      if (p.vec && n + 4 <= p.N) *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + at) = make_float4(o[0], o[1], o[2], o[3]);
-      else put_some<DT_F32>(p.out, at, o, p.N - n);
-    } else if (p.out_dtype == DT_BF16) {
-      if (p.vec && n + 4 <= p.N) *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(p.out) + at) = make_uint2(Elem<__nv_bfloat16>::pack(o[0], o[1]), Elem<__nv_bfloat16>::pack(o[2], o[3]));
-      else put_some<DT_BF16>(p.out, at, o, p.N - n);
-    } else {
-      if (p.vec && n + 4 <= p.N) *reinterpret_cast<uint2*>(reinterpret_cast<__half*>(p.out) + at) = make_uint2(Elem<__half>::pack(o[0], o[1]), Elem<__half>::pack(o[2], o[3]));
-      else put_some<DT_F16>(p.out, at, o, p.N - n);
-    }
+    put_four(p, row, n, o);
   }
 }
 __device__ __forceinline__ void zero_rows(const MatmulParams& p, int r0, int r1, int first, int step) {
@@ -475,13 +493,27 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
     }
   } else if (warp == S::kEpi + 1) {                                  // ---- MMA issue
     const uint32_t el = elect_one();
-    constexpr uint32_t idesc = idesc_f8(kPair ? 256 : 128, NT);
+    uint32_t idesc = idesc_f8(kPair ? 256 : 128, NT);
     int st = 0, ph = 0, buf = 0, bph = 1;
     for (int i = 0; rounds.has(i); ++i) {
       int kb0, kb1;
-      rounds.tile(i, kb0, kb1);
-      for (int kb = kb0; kb < kb1 && !dead && (!kPair || rank == 0); ++kb) {
-        if (!mbar_wait_both(smem_u32(&acc_empty[buf]), bph, smem_u32(&full[st]), ph, abort_flag)) { dead = true; break; }
+      const int t = rounds.tile(i, kb0, kb1);
+      if constexpr (kSwap && NT > 16) {      // columns for the rows that the tile has
+        const MmTile tl = mm_tile<NT, kSwap, kPair>(p, first, off, t < 0 ? 0 : t);
+        idesc = idesc_f8(128, min(NT, (tl.row_end - tl.row0 + 15) & ~15));
+      }
+      for (int kb = kb0, ready = 0; kb < kb1 && !dead && (!kPair || rank == 0); ++kb, --ready) {
+        if constexpr (S::kAhead < 4) {      // the operands first: they are there long before the accumulator is free
+          if (!mbar_wait_warp(smem_u32(&full[st]), ph, abort_flag) || !mbar_wait_warp(smem_u32(&acc_empty[buf]), bph, abort_flag)) { dead = true; break; }
+        } else if (!ready) {      // lane 2j: the operands of the step after the next j, lane 2j + 1: its accumulator
+          const int j = lane >> 1 < S::kAhead ? lane >> 1 : 0;
+          int q = (lane & 1 ? buf : st) + j;
+          const int wrap = lane & 1 ? S::kBufs : S::kStages;
+          uint32_t par = lane & 1 ? bph : ph;
+          if (q >= wrap) q -= wrap, par ^= 1;
+          ready = mbar_wait_steps<2>(smem_u32(lane & 1 ? &acc_empty[q] : &full[q]), par, min(S::kAhead, kb1 - kb), lane, abort_flag);
+          if (!ready) { dead = true; break; }
+        }
         tc_fence_after();
         const uint32_t a = ((smem_u32(smem + st * S::kStageBytes) >> 4) & 0x3fff) | kDescLoSw128, b = a + (16384 >> 4);
 #pragma unroll
@@ -538,10 +570,18 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
           for (int i = 0; i < R; ++i) ca[j][i] = va[j][i];
         }
         if (kb + 4 < kb1) fetch(kb + 4);
+        int ready = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           if (kb + j >= kb1) break;
-          if (!mbar_wait_warp(smem_u32(&scale_empty[buf]), bph, abort_flag)) { dead = true; break; }
+          if (!ready) {
+            int q = buf + (lane < S::kAhead ? lane : 0);
+            uint32_t par = bph;
+            if (q >= S::kBufs) q -= S::kBufs, par ^= 1;
+            ready = mbar_wait_steps<1>(smem_u32(&scale_empty[q]), par, min(min(S::kAhead, 4 - j), kb1 - kb - j), lane, abort_flag);
+            if (!ready) { dead = true; break; }
+          }
+          --ready;
           float* s = scales + buf * S::kScaleRow;
 #pragma unroll
           for (int i = 0; i < R; ++i)
@@ -559,6 +599,7 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
     if constexpr (S::kSplitRegs) regs_inc<S::kEpiRegs>();
     const int quad = warp & 3, half = warp >> 2, col0 = half * S::kCols;
     const int l = quad * 32 + lane;                                  // accumulator lane
+    bool red_in_use = false;
     const uint32_t lead_empty = mapa_shared(smem_u32(&acc_empty[0]), 0);
     int buf = 0, ph = 0;
     for (int i = 0; rounds.has(i); ++i) {
@@ -568,19 +609,29 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
       float acc[S::kCols];
 #pragma unroll
       for (int j = 0; j < S::kCols; ++j) acc[j] = 0.f;
-      for (int kb = kb0; kb < kb1 && !dead; ++kb) {
-        if (!mbar_ready(smem_u32(&acc_full[buf]), ph) && !mbar_wait_warp(smem_u32(&acc_full[buf]), ph, abort_flag)) { dead = true; break; }
+      const int rows = kSwap ? min(NT, tl.row_end - tl.row0) : NT;      // columns in use
+      for (int kb = kb0, ready = 0; kb < kb1 && !dead; ++kb, --ready) {
+        if constexpr (S::kAhead < 4) {
+          if (!mbar_ready(smem_u32(&acc_full[buf]), ph) && !mbar_wait_warp(smem_u32(&acc_full[buf]), ph, abort_flag)) { dead = true; break; }
+        } else if (!ready) {
+          int q = buf + (lane < S::kAhead ? lane : 0);
+          uint32_t par = ph;
+          if (q >= S::kBufs) q -= S::kBufs, par ^= 1;
+          ready = mbar_wait_steps<1>(smem_u32(&acc_full[q]), par, min(S::kAhead, kb1 - kb), lane, abort_flag);
+          if (!ready) { dead = true; break; }
+        }
         tc_fence_after();
         const float* s = scales + buf * S::kScaleRow;
-        const uint32_t taddr = tb + buf * NT + col0 + ((uint32_t)(quad * 32) << 16);
+        const uint32_t taddr = tb + buf * NT + ((uint32_t)(quad * 32) << 16);
         uint32_t v[2][S::kChunk];
-        tmem_ld_cols<S::kChunk>(taddr, v[0]);
+        tmem_ld_cols<S::kChunk>(taddr + mm_column<NT, kSwap, kPair>(half, 0), v[0]);
         const float sr = kSwap ? 0.f : s[l] * s[128 + half];
 #pragma unroll
         for (int c = 0; c < S::kCols / S::kChunk; ++c) {
+          const int col = mm_column<NT, kSwap, kPair>(half, c);
           tmem_ld_wait();
           if (c + 1 < S::kCols / S::kChunk) {
-            tmem_ld_cols<S::kChunk>(taddr + S::kChunk * (c + 1), v[(c + 1) & 1]);
+            if (!kSwap || mm_column<NT, kSwap, kPair>(half, c + 1) < rows) tmem_ld_cols<S::kChunk>(taddr + mm_column<NT, kSwap, kPair>(half, c + 1), v[(c + 1) & 1]);
           } else {      // all of it is in registers: the tensor core may have the accumulator back
             tc_fence_before();
             __syncwarp();
@@ -588,12 +639,13 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
             else mbar_arrive_p(smem_u32(&acc_empty[buf]), lane == 0);
             if (!kSwap) mbar_arrive_p(smem_u32(&scale_empty[buf]), lane == 0);
           }
+          if (kSwap && col >= rows) continue;
 #pragma unroll
           for (int i = 0; i < S::kChunk; i += 4) {
             float* o = acc + c * S::kChunk + i;
             const uint32_t* x = v[c & 1] + i;
             float4 sc = make_float4(sr, sr, sr, sr);
-            if constexpr (kSwap) sc = *reinterpret_cast<const float4*>(s + col0 + c * S::kChunk + i);
+            if constexpr (kSwap) sc = *reinterpret_cast<const float4*>(s + col + i);
             fma2(o[0], o[1], x[0], x[1], sc.x, sc.y);
             fma2(o[2], o[3], x[2], x[3], sc.z, sc.w);
           }
@@ -613,23 +665,25 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
           else put_rows<DT_F32, kPair>(p, buf, acc, row0, tl.row_end, n, lane);
         }
       } else {
+        // to shared memory [row][128 weights] and out of it again row by row (as they stand, a store instruction writes 64 bytes of one row: 8000 cycles a tile of 64)
+        if (red_in_use) named_bar_sync(1, S::kEpi * 32);      // the last tile's sums are read
+#pragma unroll
+        for (int c = 0; c < S::kCols / S::kChunk; ++c) {
+          const int col = mm_column<NT, kSwap, kPair>(half, c);
+          if (col >= rows) continue;
+#pragma unroll
+          for (int j = 0; j < S::kChunk; ++j) red[(col + j) * 128 + l] = acc[c * S::kChunk + j];
+        }
         if (!rounds.shared(i)) {
-          const int n = tl.n0 + l;
-          if (!dead && t >= 0 && n < p.N) {
-#pragma unroll
-            for (int j = 0; j < S::kCols; ++j) {
-              const int row = tl.row0 + col0 + j;
-              if (row < tl.row_end) {
-                const long long at = (long long)row * p.ldo + n;
-                if (p.out_dtype == DT_BF16) put<DT_BF16>(p.out, at, acc[j]);
-                else if (p.out_dtype == DT_F16) put<DT_F16>(p.out, at, acc[j]);
-                else put<DT_F32>(p.out, at, acc[j]);
-              }
+          named_bar_sync(1, S::kEpi * 32);
+          red_in_use = true;
+          if (!dead && t >= 0)
+            for (int j = tid; j < rows * 32; j += S::kEpi * 32) {
+              const int n = tl.n0 + (j & 31) * 4;
+              const float4 v = *reinterpret_cast<const float4*>(red + j * 4);
+              if (n < p.N) put_four(p, tl.row0 + (j >> 5), n, {v.x, v.y, v.z, v.w});
             }
-          }
         } else {
-#pragma unroll
-          for (int j = 0; j < S::kCols; ++j) red[(col0 + j) * 128 + l] = acc[j];
           __syncwarp();
           cluster_sync_all();
           if (!dead && t >= 0) {
