@@ -770,20 +770,53 @@ static int launch_matmul(const MatmulParams& p, const void* a, long long lda, co
   return B200MOE_OK;
 }
 
-// Which form: rows on the lanes (128 x 256 tiles) where a run of rows fills them and the tiles fill the SMs, otherwise weights on the lanes with
-// the rows' tile that a run needs, and clusters large enough to give every SM a part of the tiles that there are (two for the tiles of the last round).
+// The forms with weights on the lanes: rows of a tile, and microseconds of a call and of a group, as fitted to measured calls (20 sizes from 1 x 2048 x 2048 to
+// 4096 x 2816 x 704 in every form and cluster, weights in L2).
+struct MmForm { int rows; float call, group; };
+constexpr MmForm kMmForms[] = {{16, 4.9f, 0.17f}, {32, 5.4f, 0.22f}, {64, 6.4f, 0.30f}, {128, 10.0f, 0.35f}};
+constexpr float kMmPairCall = 5.6f, kMmPairGroup = 0.48f, kMmPairRound = 0.7f;
+
+// The largest cluster that gives its CTAs a part each: of eight CTAs only as many clusters as three quarters of the SMs hold (16 of them took two rounds: 8.2 us instead
+// of 5.1 at 1 x 2048 x 2048), two where tiles are more than the SMs, for those of the last round.
+static int matmul_cluster(long long tiles, int KB, int sms) {
+  int cluster = 2;
+  while (cluster < 8 && tiles * cluster * 2 <= (cluster == 4 ? sms * 3 / 4 : sms) && KB >= cluster * 4) cluster *= 2;
+  return cluster;
+}
+
+// One matrix: the form of the least time by that model; many rows take CTA pairs (512 x 4096 x 4096: pairs 19.7 us, single CTAs of 128 x 256 21.1, weights on the
+// lanes 23.0; 200 rows: 18.8, 20.0, 16.0).
+// A matrix per expert: by the mean rows of a run, whose lengths the host does not know. Up to 12 tiles of 16 rows; then 128 x 256, which lose less than 10 % to tiles
+// of 32 and 64 while runs are alike (25 rows, 128 experts of 1536 x 2048: 79.6 us, 73.6 and 75.6) and gain where a few are long (19 rows on average, skewed, 2816 x
+// 704: 37.7 us, 61.4 and 58.0); pairs where the rows that tiles of 256 leave empty no longer matter (375 rows: pairs 229 us, single CTAs 217; 1000: 121, 125).
 static int matmul(const MatmulParams& p, const void* a, long long lda, const void* w, long long ldw, cudaStream_t st) {
   const int sms = sm_count();
   if (sms <= 0) return B200MOE_ERR_DEVICE;
-  const long long runs = p.offsets ? (p.U < p.M ? p.U : p.M) : 1, mean = p.M / runs;
-  const auto tiles = [&](int r, int c) { return (p.M / r + (p.offsets ? runs : (p.M % r != 0))) * ((p.N + c - 1) / c); };      // (at most)
-  if (mean >= 256 && tiles(256, 256) >= sms / 2) return launch_matmul<256, false, true>(p, a, lda, w, ldw, tiles(256, 256), 1, sms, st);
-  if (mean >= 96 && tiles(128, 256) >= sms / 2) return launch_matmul<256, false, false>(p, a, lda, w, ldw, tiles(128, 256), 1, sms, st);
-  const int nt = mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 64 ? 64 : 128;
-  const long long n = tiles(nt, 128);
-  int cluster = 2;
-  while (cluster < 8 && n * cluster * 2 <= sms && p.KB >= cluster * 4) cluster *= 2;
-  switch (nt) {
+  int rows, cluster;
+  long long n;
+  if (p.offsets) {
+    const long long runs = p.U < p.M ? p.U : p.M, mean = p.M / runs;
+    const auto tiles = [&](int r, int c) { return (p.M / r + runs) * ((p.N + c - 1) / c); };      // (at most)
+    if (mean > 512) return launch_matmul<256, false, true>(p, a, lda, w, ldw, tiles(256, 256), 1, sms, st);
+    if (mean > 12) return launch_matmul<256, false, false>(p, a, lda, w, ldw, tiles(128, 256), 1, sms, st);
+    rows = 16, n = tiles(rows, 128), cluster = matmul_cluster(n, p.KB, sms);
+  } else {
+    const auto tiles = [&](int r, int c) { return (long long)((p.M + r - 1) / r) * ((p.N + c - 1) / c); };
+    const long long pairs = tiles(256, 256), rounds = (pairs + sms / 2 - 1) / (sms / 2);
+    float best = kMmPairCall + (float)rounds * (float)p.KB * kMmPairGroup + (float)(rounds - 1) * kMmPairRound;
+    rows = 0;
+    for (const MmForm& f : kMmForms) {
+      const long long t = tiles(f.rows, 128);
+      const int c = matmul_cluster(t, p.KB, sms), workers = sms / c * c;
+      const long long full = t / workers, rest = t - full * workers;
+      int parts = c;
+      while (parts > 1 && (rest * parts > workers || p.KB < 2 * parts)) parts /= 2;
+      const float time = f.call + ((float)full * (float)p.KB + (float)(rest ? (p.KB + parts - 1) / parts : 0)) * f.group + (float)(full + (rest > 0) - 1) * (f.call - 4.5f);
+      if (time < best) best = time, rows = f.rows, n = t, cluster = c;
+    }
+    if (!rows) return launch_matmul<256, false, true>(p, a, lda, w, ldw, pairs, 1, sms, st);
+  }
+  switch (rows) {
     case 16: return launch_matmul<16, true, false>(p, a, lda, w, ldw, n, cluster, sms, st);
     case 32: return launch_matmul<32, true, false>(p, a, lda, w, ldw, n, cluster, sms, st);
     case 64: return launch_matmul<64, true, false>(p, a, lda, w, ldw, n, cluster, sms, st);

@@ -178,7 +178,7 @@ def operands(m, n, k, seed=0):
     return *pkg.quantize_fp8(x), *pkg.quantize_fp8_weight(w)
 
 
-SIZES = [(1, 1, 1), (1, 4096, 4096), (1, 128, 128), (2, 16, 16), (3, 130, 200), (16, 1536, 2048), (17, 300, 384), (32, 2816, 704), (33, 257, 100), (64, 64, 8192), (65, 129, 640),
+SIZES = [(1, 2048, 2048), (8, 1536, 2048), (48, 4096, 1024), (200, 4096, 512), (520, 4096, 256), (1, 1, 1), (1, 4096, 4096), (1, 128, 128), (2, 16, 16), (3, 130, 200), (16, 1536, 2048), (17, 300, 384), (32, 2816, 704), (33, 257, 100), (64, 64, 8192), (65, 129, 640),
          (100, 4096, 130), (128, 1408, 2816), (129, 100, 512), (200, 2048, 256), (333, 2816, 704), (500, 5001, 300), (1000, 4100, 272), (1024, 4096, 1024), (1300, 7000, 129), (2100, 2570, 640), (2048, 2560, 256)]
 
 
