@@ -7,12 +7,14 @@
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/variable.h>
 
 namespace {
 
@@ -156,6 +158,17 @@ at::Tensor once(at::Tensor out, const char* what) {
   return (*error)({out.detach().requires_grad_(true)})[0];
 }
 
+// A leaf's gradient is handed over on the stream on which its accumulator was made. Where an eager graph keeps that alive, a backward pass that is being captured
+// on another stream would have the engine wait across the two, which ends the process: refused while it still can be.
+void check_capture(const at::Tensor& x, const char* what) {
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None || !x.is_leaf()) return;
+  const auto node = torch::autograd::impl::try_get_grad_accumulator(x);
+  if (!node) return;
+  const auto made_on = node->stream();
+  TORCH_CHECK(!made_on || *made_on == c10::cuda::getCurrentCUDAStream().unwrap(), what,
+              ": a graph of the same leaf that was made on another stream is still alive; drop its outputs before a capture that takes gradients");
+}
+
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
@@ -259,6 +272,7 @@ PyObject* py_top_k_gate(PyObject*, PyObject* const* args, Py_ssize_t n) {
   {
     Released released;
     if (x.requires_grad() && at::GradMode::is_enabled()) {
+      check_capture(x, "top_k_gate");
       const variable_list out = Gate::apply(x, (int64_t)k, renormalize);
       weights = out[0], ids = out[1];
     } else {
@@ -281,6 +295,7 @@ PyObject* py_balance_loss(PyObject*, PyObject* const* args, Py_ssize_t n) {
   {
     Released released;
     if (x.requires_grad() && at::GradMode::is_enabled()) {
+      check_capture(x, "balance_loss");
       const variable_list out = Balance::apply(x, ids);
       loss = out[0], counts = out[1];
     } else {

@@ -753,7 +753,13 @@ static int launch_matmul(const MatmulParams& p, const void* a, long long lda, co
   if (int rc = codes_map(&rows, a, p.M, p.K, lda, kSwap ? NT : 128)) return rc;
   if (int rc = codes_map(&weights, w, (long long)p.E * p.N, p.K, ldw, kSwap ? 128 : S::kBRows)) return rc;
   const void* fn = (const void*)k_matmul_fp8<NT, kSwap, kPair>;
-  B200_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+  static std::atomic<unsigned long long> opted_in{0};      // devices on which this form may have its shared memory
+  int dev = 0;
+  B200_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev > 63 || !(opted_in.load(std::memory_order_relaxed) >> dev & 1)) {
+    B200_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+    if (dev <= 63) opted_in.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
   const int ranks = kPair ? 2 : cluster;
   const long long most = sms / ranks;
   const int clusters = (int)(tiles < most ? (tiles > 0 ? tiles : 1) : most);

@@ -266,8 +266,8 @@ int b200moe_quantize_fp8(const void* x, int dtype, long long x_stride, int x_row
                          float* scales, void* workspace, long long workspace_bytes, void* stream) {
   using namespace b200;
   if (rows < 0 || x_rows < 0 || K < 1 || dtype < 0 || dtype > 2 || (x_stride < K && x_rows > 1) || codes_stride < K) return B200MOE_ERR_ARG;
+  if (rows == 0) return B200MOE_OK;      // (an empty src_row has no address)
   if (!src_row && rows != x_rows) return B200MOE_ERR_ARG;
-  if (rows == 0) return B200MOE_OK;
   if ((!x && x_rows) || !codes || !scales) return B200MOE_ERR_ARG;
   const int size = dtype == DT_F32 ? 4 : 2;
   if (((uintptr_t)x & (size - 1)) || (((uintptr_t)scales | (uintptr_t)workspace) & 3)) return B200MOE_ERR_ARG;

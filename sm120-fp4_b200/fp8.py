@@ -9,7 +9,7 @@ of a row (activations) or per 128x128 block (weights), the quantisers that make 
     q, s = quantize_fp8(x, src_row=pairs // top_k)
     y = matmul_fp8_experts(q, s, w, w_scale, experts, offsets)      # row i is what pair pairs[i] gets
 
-Nothing here synchronises or keeps state between calls; every call can be captured into a CUDA graph and runs on the tensors' device, on its current stream."""
+Nothing here synchronises or keeps state between calls; every call but matmul_fp8_status can be captured into a CUDA graph and runs on the tensors' device, on its current stream."""
 from __future__ import annotations
 
 import torch
@@ -165,7 +165,8 @@ def matmul_fp8_experts(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, 
     return out
 
 
-def matmul_fp8_status(device: torch.device | None = None) -> None:
-    """Raises if a bounded wait inside a matmul_fp8 / matmul_fp8_experts call ran out on this device since the last look (results are then incomplete). Synchronises
-    the current stream."""
-    _lib.call(torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device), "matmul_fp8_status", _lib.lib().b200moe_matmul_fp8_status)
+def matmul_fp8_status(device: torch.device | str | int | None = None) -> None:
+    """Raises if a bounded wait inside a matmul_fp8 / matmul_fp8_experts call ran out on this device (default: the current one) since the last look: results are then
+    incomplete. Synchronises the device's current stream."""
+    device = torch.device("cuda" if device is None else device)
+    _lib.call(torch.device("cuda", torch.cuda.current_device()) if device.index is None else device, "matmul_fp8_status", _lib.lib().b200moe_matmul_fp8_status)

@@ -3,11 +3,11 @@ keeps experts evenly used, with the number of pairs of each. Both have gradients
 torch (softmax, top-k, renormalise: sm120fp4/kernels/moe_layer.py:195-200).
 
 Nothing here synchronises or keeps state between calls: forward and backward can be captured into a CUDA graph. A capture of a backward pass wants, as with
-every autograd function, that no eager graph of the same leaves is alive."""
+every autograd function, that no graph of the same leaves that was made on another stream is alive: logits that are such a leaf are refused (RuntimeError), where the host
+extension takes the call; for leaves further back it is the caller's to see to."""
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -36,6 +36,13 @@ def _gate(logits: torch.Tensor, top_k: int, renormalize: bool):
     return weights, ids
 
 
+def _once(out: torch.Tensor, what: str) -> torch.Tensor:
+    """The gradient of a gradient is not there: whoever asks for it is told so."""
+    if not torch.is_grad_enabled():
+        return out
+    return torch._C._functions.DelayedError(f"{what} is differentiable once".encode(), 1)(out.detach().requires_grad_(True))
+
+
 class _Gate(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, top_k, renormalize):
@@ -46,16 +53,15 @@ class _Gate(torch.autograd.Function):
         return weights, ids
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad, _):
         weights, ids, logits = ctx.saved_tensors
         dtype, e = ctx.like
         tokens, k = weights.shape
         out = torch.empty((tokens, e), dtype=dtype, device=weights.device)
-        grad = grad.contiguous()
+        grad = grad.detach().contiguous()
         _lib.call(out.device, "top_k_gate backward", _lib.lib().b200moe_gate_backward, grad.data_ptr(), weights.data_ptr(), ids.data_ptr(), _lib.ptr(logits),
                   _lib.DTYPES[dtype], e if logits is None else max(logits.stride(0), e), tokens, e, k, int(ctx.renormalize), out.data_ptr())
-        return out, None, None
+        return _once(out, "top_k_gate"), None, None
 
 
 def top_k_gate(logits: torch.Tensor, top_k: int, renormalize: bool = True):
@@ -96,15 +102,14 @@ class _Balance(torch.autograd.Function):
         return loss, counts
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad, _):
         logits, ids, counts, stats = ctx.saved_tensors
         tokens, e = logits.shape
         out = torch.empty((tokens, e), dtype=logits.dtype, device=logits.device)
-        grad = grad.contiguous()
+        grad = grad.detach().contiguous()
         _lib.call(out.device, "balance_loss backward", _lib.lib().b200moe_balance_backward, grad.data_ptr(), logits.data_ptr(), _lib.DTYPES[logits.dtype],
                   max(logits.stride(0), e), tokens, e, ids.data_ptr(), ids.shape[1], counts.data_ptr(), stats.data_ptr(), out.data_ptr())
-        return out, None
+        return _once(out, "balance_loss"), None
 
 
 def balance_loss(logits: torch.Tensor, ids: torch.Tensor):

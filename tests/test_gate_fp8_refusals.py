@@ -103,3 +103,28 @@ def test_c_abi_refusals():
     assert h.b200moe_matmul_fp8_experts(p, 16, p, 4, p, 16, p, 2, p, p, 1025, 4, 16, p, 0, 4, 0, None) == L.ERR_LIMIT
     assert h.b200moe_matmul_fp8_experts(p, 16, p, 4, p, 16, p, 2, None, p, 1, 4, 16, p, 0, 4, 0, None) == L.ERR_ARG
     assert h.b200moe_matmul_fp8_experts(p, 16, p, 4, p, 16, p, 2, p, p, 0, 4, 16, p, 0, 4, 0, None) == 0      # no runs, nothing to zero
+
+
+def test_calls_go_to_the_tensors_device(monkeypatch):
+    """A call on a device that is not the current one makes it current for the launch, and takes that device's current stream."""
+    import contextlib
+    import sm120fp4_b200._lib as L
+    here, seen = [0], []
+
+    @contextlib.contextmanager
+    def guard(device):
+        before, here[0] = here[0], device.index
+        yield
+        here[0] = before
+    monkeypatch.setattr(torch.cuda, "device", guard)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: here[0], raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: 100 + i, raising=False)
+    fn = lambda *args: seen.append((here[0], *args)) or 0
+    L.call(torch.device("cuda", 0), "x", fn, 1)
+    L.call(torch.device("cuda", 3), "x", fn, 2)
+    assert seen == [(0, 1, 100), (3, 2, 103)] and here == [0]
+    with pytest.raises(L.B200MoEError):
+        L.call(torch.device("cuda", 3), "x", lambda *args: L.ERR_ARG)
+    a, b = torch.zeros(1), torch.zeros(1)
+    with pytest.raises(RuntimeError, match="GPU"):
+        L.one_device("x", a, b)
