@@ -136,8 +136,6 @@ __device__ __forceinline__ void fma2(float& a0, float& a1, uint32_t x0, uint32_t
 template <int R> __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R)); }
 template <int R> __device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R)); }
 
-constexpr int kOutRow = 256 + 16;                 // bytes from a row to the next on its way out of a pair's tile: eight lanes' 16-byte stores meet all banks
-
 template <int NT, bool kSwap, bool kPair> struct MmShape {
   static constexpr int kEpi = NT >= 128 ? 8 : 4;                  // epilogue warps: two per lane quadrant where a thread's columns would be more than 64 (128: kSwap false)
   static constexpr int kCols = NT / (kEpi / 4);                   // columns of a thread
@@ -151,9 +149,9 @@ template <int NT, bool kSwap, bool kPair> struct MmShape {
   static constexpr int kBRows = kPair ? NT / 2 : NT;              // rows of the B operand in this CTA's shared memory
   static constexpr int kStageBytes = 16384 + kBRows * 128;
   static constexpr int kRed = kSwap ? NT * 128 * 4 : 0;           // sums of a split inner size
-  static constexpr int kOutWarp = kSwap ? 0 : kPair ? 32 * kOutRow : 2048;      // a warp's sums on their way out: 32 rows x 256 (64) bytes
+  static constexpr int kOutWarp = kSwap ? 0 : 8192;               // a warp's sums on their way out: two boxes of 32 rows x 128 bytes
   static constexpr int kOut = kEpi * kOutWarp;
-  static constexpr int kRing = 196 * 1024 - kRed - (kPair ? kOut : 0);
+  static constexpr int kRing = 218 * 1024 - kRed - kOut;
   static constexpr int kStages = kRing / kStageBytes < 9 ? kRing / kStageBytes : 9;
   static constexpr int kBufs = 512 / NT < 8 ? 512 / NT : 8;       // accumulators in TMEM
   static constexpr int kScaleRow = kSwap ? NT : 132;              // floats of a group's scales
@@ -233,91 +231,70 @@ template <int DT, int C> __device__ __forceinline__ void put_some(void* out, lon
   for (int i = 0; i < C; ++i)
     if (i < n) put<DT>(out, at + i, v[i]);
 }
-// A warp's 32 rows x 128 columns (a row a thread) to the output, by way of 32 x 64 bytes of shared memory, so that a store instruction writes 64 bytes of
-// eight rows instead of 16 bytes of 32: a tile's stores took 5900 cycles without. 16-byte chunks are placed by (row >> 1) & 3, free of bank conflicts.
-// kAsync: 32 x 256 bytes of shared memory, a bulk copy for each row (128 columns of 16 bits, 64 of 32 at a time), which the next tile's math does not wait for: all
-// SMs end their tiles at about the same time, and 4100 cycles passed until L2 had taken the stores.
-template <int DT, bool kAsync> __device__ __forceinline__ void put_rows(const MatmulParams& p, uint8_t* buf, const float (&acc)[128], int row0, int row_end, int n, int lane) {
-  constexpr int kSize = DT == DT_F32 ? 4 : 2, kStep = 64 / kSize;      // columns of a round
-  if (!p.vec) {
-    const int row = row0 + lane;
+// A warp's 32 rows x 128 columns (a row a thread) to the output, by way of boxes of 32 rows x 128 bytes in shared memory, chunks of 16 bytes turned by the row as the
+// copy engine's 128-byte swizzle has them. A box goes out in one copy, which the next tile's math does not wait for: all SMs end their tiles at about the same
+// time, and 5900 cycles passed until the threads' own stores (16 bytes of 32 rows an instruction) had left; a copy for each row took the engine 256 of them a
+// tile. Rows beyond the run's end, and rows that do not start (or end) on 16 bytes, are stored by the warp, row by row.
+template <int DT> __device__ __forceinline__ void put_rows(const MatmulParams& p, const CUtensorMap* map_out, uint8_t* buf, const float (&acc)[128], int row0, int row_end, int n,
+                                                           int lane) {
+  constexpr int kSize = DT == DT_F32 ? 4 : 2, kCols = 128 / kSize;      // columns of a box
+  // The copy stores nothing beyond the matrix: no rows, but along a row whole 16 bytes only.
+  const bool rows_whole = p.vec && (row0 + 32 <= row_end || row_end == p.M), ends_on_16 = (p.N * kSize) % 16 == 0;
 #pragma unroll
-    for (int i = 0; i < 128; ++i)
-      if (row < row_end && n + i < p.N) put<DT>(p.out, (long long)row * p.ldo + n + i, acc[i]);
-    return;
-  }
-  if constexpr (kAsync) {
-    constexpr int kCols = 256 / kSize;
-    const int row = row0 + lane;
-    uint8_t *mine = buf + lane * kOutRow, *o = reinterpret_cast<uint8_t*>(p.out) + ((long long)row * p.ldo + n) * kSize;
-#pragma unroll
-    for (int c0 = 0; c0 < 128; c0 += kCols) {
-      const int bytes = min(256, (p.N - n - c0) * kSize);
-      if (bytes <= 0) break;
-      asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");      // the row's last copy has left
-#pragma unroll
-      for (int q = 0; q < 16; ++q) {
-        uint4 w;
-        const float* v = acc + c0 + q * 16 / kSize;
-        if constexpr (DT == DT_F32) {
-          w = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-        } else {
-          using T = std::conditional_t<DT == DT_BF16, __nv_bfloat16, __half>;
-          w = make_uint4(Elem<T>::pack(v[0], v[1]), Elem<T>::pack(v[2], v[3]), Elem<T>::pack(v[4], v[5]), Elem<T>::pack(v[6], v[7]));
-        }
-        *reinterpret_cast<uint4*>(mine + q * 16) = w;
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      const int whole = bytes & ~15;
-      if (row < row_end) {
-        if (whole)
-          asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;\n cp.async.bulk.commit_group;" ::"l"(o + c0 * kSize), "r"(smem_u32(mine)), "r"(whole) : "memory");
-        for (int i = whole; i < bytes; i += 2) *reinterpret_cast<uint16_t*>(o + c0 * kSize + i) = *reinterpret_cast<const uint16_t*>(mine + i);
-      }
-    }
-    return;
-  }
-  uint8_t* o[4];      // rows i * 8 + lane / 4
-  bool row_ok[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = row0 + i * 8 + lane / 4;
-    row_ok[i] = row < row_end;
-    o[i] = reinterpret_cast<uint8_t*>(p.out) + ((long long)row * p.ldo + n) * kSize + (lane & 3) * 16;
-  }
-  const int left = (p.N - n) * kSize - (lane & 3) * 16;      // bytes of a row from this lane's first chunk on
-  uint8_t *put_at = buf + lane * 64, *get_at = buf + (lane / 4) * 64 + (((lane & 3) ^ (lane >> 3 & 3)) << 4);
-  const int turn = (lane >> 1 & 3) << 4;
-#pragma unroll
-  for (int c0 = 0; c0 < 128; c0 += kStep) {
+  for (int c0 = 0; c0 < 128; c0 += kCols) {
     if (n + c0 >= p.N) break;
+    uint8_t* box = buf + (c0 / kCols & 1) * 4096;
+    if (lane == 0) {      // the last copy from this box has left: the tile before's, or of this tile the one before the last
+      if (c0 == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+      else if (c0 >= 2 * kCols) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+    }
     __syncwarp();
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
+    for (int q = 0; q < 8; ++q) {
       uint4 w;
-      const float* v = acc + c0 + q * kStep / 4;
+      const float* v = acc + c0 + q * 16 / kSize;
       if constexpr (DT == DT_F32) {
         w = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
       } else {
         using T = std::conditional_t<DT == DT_BF16, __nv_bfloat16, __half>;
         w = make_uint4(Elem<T>::pack(v[0], v[1]), Elem<T>::pack(v[2], v[3]), Elem<T>::pack(v[4], v[5]), Elem<T>::pack(v[6], v[7]));
       }
-      *reinterpret_cast<uint4*>(put_at + ((q << 4) ^ turn)) = w;
+      *reinterpret_cast<uint4*>(box + lane * 128 + ((q ^ (lane & 7)) << 4)) = w;
     }
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {      // row r = i * 8 + lane / 4: its chunks are turned by (r >> 1) & 3 = (lane >> 3) & 3
-      const uint4 w = *reinterpret_cast<const uint4*>(get_at + i * 512);
-      if (!row_ok[i]) continue;
-      if (left >= c0 * kSize + 16) {
-        *reinterpret_cast<uint4*>(o[i] + c0 * kSize) = w;
+    if (rows_whole && (ends_on_16 || n + c0 + kCols <= p.N)) {
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0)
+        asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];\n cp.async.bulk.commit_group;" ::"l"(map_out), "r"((n + c0) * kSize), "r"(row0),
+                     "r"(smem_u32(box)) : "memory");
+    } else {
+      __syncwarp();
+      const int rows = min(32, row_end - row0);
+      uint8_t* o = reinterpret_cast<uint8_t*>(p.out) + ((long long)row0 * p.ldo + n + c0) * kSize;
+      if (p.vec) {      // four rows an instruction
+        const int left = (p.N - n - c0) * kSize - (lane & 7) * 16;      // bytes of a row from this lane's chunk on
+        for (int r = lane >> 3; r < rows; r += 4) {
+          const uint8_t* from = box + r * 128 + (((lane & 7) ^ (r & 7)) << 4);
+          uint8_t* to = o + r * p.ldo * kSize + (lane & 7) * 16;
+          if (left >= 16) *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(from);
+          else
+            for (int i = 0; i < left; i += kSize) {
+              if constexpr (kSize == 4) *reinterpret_cast<uint32_t*>(to + i) = *reinterpret_cast<const uint32_t*>(from + i);
+              else *reinterpret_cast<uint16_t*>(to + i) = *reinterpret_cast<const uint16_t*>(from + i);
+            }
+        }
       } else {
-        const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+        const int cols = min(kCols, p.N - n - c0);
+        for (int r = 0; r < rows; ++r)
 #pragma unroll
-        for (int j = 0; j < 16 / kSize; ++j)
-          if (left >= c0 * kSize + (j + 1) * kSize) {
-            if constexpr (kSize == 4) reinterpret_cast<uint32_t*>(o[i] + c0 * kSize)[j] = x[j];
-            else reinterpret_cast<uint16_t*>(o[i] + c0 * kSize)[j] = (uint16_t)(x[j / 2] >> (16 * (j & 1)));
+          for (int i = 0; i < kCols / 32; ++i) {
+            const int c = i * 32 + lane, at = c * kSize;
+            const uint8_t* from = box + r * 128 + (((at >> 4) ^ (r & 7)) << 4) + (at & 15);
+            uint8_t* to = o + (r * p.ldo + c) * kSize;
+            if (c < cols) {
+              if constexpr (kSize == 4) *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(from);
+              else *reinterpret_cast<uint16_t*>(to) = *reinterpret_cast<const uint16_t*>(from);
+            }
           }
       }
     }
@@ -379,14 +356,15 @@ __device__ __forceinline__ void zero_rows(const MatmulParams& p, int r0, int r1,
 
 template <int NT, bool kSwap, bool kPair>
 __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
-    k_matmul_fp8(const __grid_constant__ CUtensorMap map_rows, const __grid_constant__ CUtensorMap map_weights, const __grid_constant__ MatmulParams p, int cluster) {
+    k_matmul_fp8(const __grid_constant__ CUtensorMap map_rows, const __grid_constant__ CUtensorMap map_weights, const __grid_constant__ CUtensorMap map_out,
+                 const __grid_constant__ MatmulParams p, int cluster) {
   using S = MmShape<NT, kSwap, kPair>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   float* red = reinterpret_cast<float*>(smem + S::kStages * S::kStageBytes);      // [NT][128]
-  float* scales = reinterpret_cast<float*>(smem + S::kStages * S::kStageBytes + S::kRed);
-  uint8_t* outs = reinterpret_cast<uint8_t*>(scales + S::kBufs * S::kScaleRow);
-  int* first = reinterpret_cast<int*>(outs + S::kOut);
+  uint8_t* outs = smem + S::kStages * S::kStageBytes + S::kRed;      // on 1024 bytes
+  float* scales = reinterpret_cast<float*>(outs + S::kOut);
+  int* first = reinterpret_cast<int*>(scales + S::kBufs * S::kScaleRow);
   int* off = first + MM_MAXU + 1;
   __shared__ uint64_t full[S::kStages], empty[S::kStages], acc_full[S::kBufs], acc_empty[S::kBufs], scale_empty[S::kBufs], drained;
   __shared__ uint32_t tmem_base;
@@ -660,9 +638,11 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
         if (!dead) {
           const int row0 = tl.row0 + crow + quad * 32, n = tl.n0 + col0;
           uint8_t* buf = outs + warp * S::kOutWarp;
-          if (p.out_dtype == DT_BF16) put_rows<DT_BF16, kPair>(p, buf, acc, row0, tl.row_end, n, lane);
-          else if (p.out_dtype == DT_F16) put_rows<DT_F16, kPair>(p, buf, acc, row0, tl.row_end, n, lane);
-          else put_rows<DT_F32, kPair>(p, buf, acc, row0, tl.row_end, n, lane);
+          if (row0 < tl.row_end) {
+            if (p.out_dtype == DT_BF16) put_rows<DT_BF16>(p, &map_out, buf, acc, row0, tl.row_end, n, lane);
+            else if (p.out_dtype == DT_F16) put_rows<DT_F16>(p, &map_out, buf, acc, row0, tl.row_end, n, lane);
+            else put_rows<DT_F32>(p, &map_out, buf, acc, row0, tl.row_end, n, lane);
+          }
         }
       } else {
         // to shared memory [row][128 weights] and out of it again row by row (as they stand, a store instruction writes 64 bytes of one row: 8000 cycles a tile of 64)
@@ -696,7 +676,7 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
         }
       }
     }
-    if constexpr (kPair) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");      // shared memory stays until the copies have read it
+    if constexpr (!kSwap) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");      // shared memory stays until the copies have read it
     if (p.offsets && p.zero_rest) {      // rows outside every run, and of experts that are not there
       const int step = gridDim.x * S::kEpi * 32, me = blockIdx.x * S::kEpi * 32 + tid;
       if (unknown_s)
@@ -729,8 +709,8 @@ static PFN_cuTensorMapEncodeTiled_v12000 map_encoder() {
   }
   return (PFN_cuTensorMapEncodeTiled_v12000)p;
 }
-// E4M3 matrix of `rows` rows of K codes, `stride` bytes apart: boxes of 128 codes x box_rows, 128-byte swizzle, zeros beyond the matrix
-static int codes_map(CUtensorMap* map, const void* base, long long rows, int K, long long stride, int box_rows) {
+// Matrix of `rows` rows of K bytes, `stride` bytes apart: boxes of 128 bytes x box_rows, 128-byte swizzle, zeros (or nothing stored) beyond the matrix
+static int bytes_map(CUtensorMap* map, const void* base, long long rows, long long K, long long stride, int box_rows) {
   auto enc = map_encoder();
   if (!enc) return B200MOE_ERR_DEVICE;
   cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)stride};
@@ -749,9 +729,12 @@ static int sm_count() {
 template <int NT, bool kSwap, bool kPair>
 static int launch_matmul(const MatmulParams& p, const void* a, long long lda, const void* w, long long ldw, long long tiles, int cluster, int sms, cudaStream_t st) {
   using S = MmShape<NT, kSwap, kPair>;
-  CUtensorMap rows, weights;
-  if (int rc = codes_map(&rows, a, p.M, p.K, lda, kSwap ? NT : 128)) return rc;
-  if (int rc = codes_map(&weights, w, (long long)p.E * p.N, p.K, ldw, kSwap ? 128 : S::kBRows)) return rc;
+  CUtensorMap rows, weights, out = {};
+  if (int rc = bytes_map(&rows, a, p.M, p.K, lda, kSwap ? NT : 128)) return rc;
+  if (int rc = bytes_map(&weights, w, (long long)p.E * p.N, p.K, ldw, kSwap ? 128 : S::kBRows)) return rc;
+  const int size = p.out_dtype == DT_F32 ? 4 : 2;
+  if (!kSwap && p.vec)
+    if (int rc = bytes_map(&out, p.out, p.M, (long long)p.N * size, p.ldo * size, 32)) return rc;
   const void* fn = (const void*)k_matmul_fp8<NT, kSwap, kPair>;
   static std::atomic<unsigned long long> opted_in{0};      // devices on which this form may have its shared memory
   int dev = 0;
@@ -771,7 +754,7 @@ static int launch_matmul(const MatmulParams& p, const void* a, long long lda, co
   attr[1].val.clusterDim.x = ranks, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr, cfg.numAttrs = ranks > 1 ? 2 : 1;
   MatmulParams q = p;
-  void* args[] = {&rows, &weights, &q, &cluster};
+  void* args[] = {&rows, &weights, &out, &q, &cluster};
   B200_CUDA_TRY(cudaLaunchKernelExC(&cfg, fn, args));
   return B200MOE_OK;
 }
@@ -839,7 +822,10 @@ static int matmul_args(const void* a, long long lda, const float* sa, const void
   if (M > (1 << 30) || N > (1 << 30) || K > (1 << 30)) return B200MOE_ERR_LIMIT;
   return B200MOE_OK;
 }
-static int stores_16(const void* out, int out_dtype, long long ldo) { return ((uintptr_t)out & 15) == 0 && (ldo * (out_dtype == DT_F32 ? 4 : 2)) % 16 == 0; }
+static int stores_16(const void* out, int out_dtype, int N, long long ldo) {
+  const int size = out_dtype == DT_F32 ? 4 : 2;
+  return ((uintptr_t)out & 15) == 0 && (ldo * size) % 16 == 0 && ((long long)N + 256) * size < (1ll << 31);
+}
 
 }  // namespace b200
 
@@ -850,7 +836,7 @@ int b200moe_matmul_fp8(const void* a, long long a_stride, const float* a_scales,
   using namespace b200;
   if (int rc = matmul_args(a, a_stride, a_scales, w, w_stride, w_scales, M, N, K, out, out_dtype, out_stride)) return rc;
   if (M == 0 || N == 0) return B200MOE_OK;
-  const MatmulParams p = {a_scales, w_scales, out, nullptr, nullptr, 0, 1, M, N, K, (K + 127) / 128, (N + 127) / 128, out_dtype, 0, stores_16(out, out_dtype, out_stride), out_stride};
+  const MatmulParams p = {a_scales, w_scales, out, nullptr, nullptr, 0, 1, M, N, K, (K + 127) / 128, (N + 127) / 128, out_dtype, 0, stores_16(out, out_dtype, N, out_stride), out_stride};
   return matmul(p, a, a_stride, w, w_stride, (cudaStream_t)stream);
 }
 
@@ -868,7 +854,7 @@ int b200moe_matmul_fp8_experts(const void* a, long long a_stride, const float* a
   }
   if (!experts || !offsets) return B200MOE_ERR_ARG;
   const MatmulParams p = {a_scales, w_scales, out, experts, offsets, runs, E, rows, N, K, (K + 127) / 128, (N + 127) / 128, out_dtype, zero_rest,
-                          stores_16(out, out_dtype, out_stride), out_stride};
+                          stores_16(out, out_dtype, N, out_stride), out_stride};
   return matmul(p, a, a_stride, w, w_stride, (cudaStream_t)stream);
 }
 

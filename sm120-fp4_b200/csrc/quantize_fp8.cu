@@ -111,32 +111,34 @@ __global__ void __launch_bounds__(256) k_quantize_fp8_copies(const T* __restrict
   }
 }
 
-// Rows of any length, stride and alignment: a warp per group, four values a lane, one at a time.
+// Rows of any length, stride and alignment: a warp per group, four neighbouring values a lane, loaded one at a time (the four loads of a warp share their sectors) and
+// stored as one word where the rows of the codes allow it.
 template <typename T>
 __global__ void __launch_bounds__(256) k_quantize_fp8_rows_any(const T* __restrict__ x, long long ldx, int x_rows, const int* __restrict__ src_row, int rows, int K,
-                                                               uint8_t* __restrict__ codes, long long ldc, float* __restrict__ scales) {
+                                                               uint8_t* __restrict__ codes, long long ldc, float* __restrict__ scales, int words) {
   const int lane = threadIdx.x & 31, KB = (K + 127) >> 7;
   const long long units = (long long)rows * KB;
   grid_dependency_wait();
   grid_launch_dependents();
   for (long long u = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); u < units; u += (long long)gridDim.x * 8) {
-    const int row = (int)(u / KB), g = (int)(u - (long long)row * KB);
+    const int row = (int)(u / KB), g = (int)(u - (long long)row * KB), c = g * 128 + lane * 4;
     const int src = src_row ? src_row[row] : row;
     const bool gone = src < 0 || src >= x_rows;
     float v[4], m = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int c = g * 128 + i * 32 + lane;
-      v[i] = !gone && c < K ? Elem<T>::load(x + (long long)src * ldx + c) : 0.f;
-      m = max_nan(m, fabsf(v[i]));
-    }
+    for (int i = 0; i < 4; ++i) v[i] = !gone && c + i < K ? Elem<T>::load(x + (long long)src * ldx + c + i) : 0.f;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    for (int i = 0; i < 4; ++i) m = max_nan(m, fabsf(v[i]));
+    asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(m));
     const Fp8Scale s = fp8_scale(m);
+    const uint32_t q = cvt_e4m3x4(v[0] * s.factor, v[1] * s.factor, v[2] * s.factor, v[3] * s.factor);
+    uint8_t* o = codes + (long long)row * ldc + c;
+    if (words && c + 4 <= K) {
+      *reinterpret_cast<uint32_t*>(o) = q;
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int c = g * 128 + i * 32 + lane;
-      if (c < K) codes[(long long)row * ldc + c] = (uint8_t)cvt_e4m3x4(v[i] * s.factor, 0.f, 0.f, 0.f);
+      for (int i = 0; i < 4; ++i)
+        if (c + i < K) o[i] = (uint8_t)(q >> (8 * i));
     }
     if (lane == 0) scales[(long long)row * KB + g] = gone ? 0.f : s.scale;
   }
@@ -231,7 +233,8 @@ static int quantize_fp8_rows(const void* x, long long ldx, int x_rows, const int
   const void* fn = vec ? (const void*)k_quantize_fp8_rows<T> : (const void*)k_quantize_fp8_rows_any<T>;
   const T* xt = (const T*)x;
   uint8_t* ct = (uint8_t*)codes;
-  void* args[] = {&xt, &ldx, &x_rows, &src_row, &rows, &K, &ct, &ldc, &scales};
+  int words = ldc % 4 == 0 && ((uintptr_t)codes & 3) == 0;      // (read by the second form only)
+  void* args[] = {&xt, &ldx, &x_rows, &src_row, &rows, &K, &ct, &ldc, &scales, &words};
   return launch_kernel(fn, (int)(blocks < 1 << 30 ? blocks : 1 << 30), 256, 0, true, args, st);
 }
 

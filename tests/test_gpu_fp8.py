@@ -227,6 +227,29 @@ def test_matmul_views_and_out():
                 assert bool((buf[:, :left] == 7).all()) and bool((buf[:, left + n:] == 7).all())
 
 
+def test_matmul_row_ends_inside_16_bytes():
+    """Rows of the output on 16 bytes whose last values end inside 16: what stands behind them stays."""
+    import sm120fp4_b200 as pkg
+    for m, n, k in [(40, 150, 128), (1300, 5003, 256)]:
+        a, sa, w, sw = operands(m, n, k, m)
+        for dtype in TYPES:
+            want = pkg.matmul_fp8(a, sa, w, sw, out_dtype=dtype)
+            close(want, a, sa, w, sw)
+            buf = torch.full((m, (n + 63) // 16 * 16), 7.0, dtype=dtype, device="cuda")
+            assert torch.equal(pkg.matmul_fp8(a, sa, w, sw, out=buf[:, :n]), want) and bool((buf[:, n:] == 7).all())
+    off = [0, 3, 500, 533, 900]      # runs that end inside a warp's 32 rows, results of both widths
+    a, sa = pkg.quantize_fp8(randn(900, 256, seed=1).cuda())
+    w, sw = pkg.quantize_fp8_weight(randn(4, 310, 256, seed=2).cuda())
+    experts, offsets = torch.tensor([3, 1, 0, 2], dtype=torch.int32, device="cuda"), torch.tensor(off, dtype=torch.int32, device="cuda")
+    for dtype in TYPES:
+        buf = torch.full((900, 320), 7.0, dtype=dtype, device="cuda")
+        pkg.matmul_fp8_experts(a, sa, w, sw, experts, offsets, out=buf[:, :310])
+        assert bool((buf[:, 310:] == 7).all())
+        for u, e in enumerate((3, 1, 0, 2)):
+            r = slice(off[u], off[u + 1])
+            close(buf[r, :310], a[r], sa[r], w[e], sw[e])
+
+
 def test_matmul_nan_and_infinity_stay_in_their_rows():
     import sm120fp4_b200 as pkg
     for m in (20, 300, 1100):
