@@ -143,7 +143,7 @@ template <int NT, bool kSwap, bool kPair> struct MmShape {
   // 128 sums and 64 values in flight a thread: registers go from the other warps (a warpgroup of four, one idle) to the epilogue's eight. A launch of 12 warps has
   // 168 a thread: 8 * kEpiRegs + 4 * (504 - 2 * kEpiRegs) = 12 * 168. Both shares are those with which ptxas spills nothing (192 / 120 spilled and took 148
   // instead of 126 us at 8192 x 4096 x 4096).
-  static constexpr int kEpiRegs = kPair ? 176 : 184;
+  static constexpr int kEpiRegs = kPair ? 184 : 176;
   static constexpr bool kSplitRegs = kCols == 128;
   static constexpr int kThreads = kSplitRegs ? 384 : (kEpi + 3) * 32;
   static constexpr int kBRows = kPair ? NT / 2 : NT;              // rows of the B operand in this CTA's shared memory

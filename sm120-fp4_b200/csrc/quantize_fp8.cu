@@ -111,36 +111,57 @@ __global__ void __launch_bounds__(256) k_quantize_fp8_copies(const T* __restrict
   }
 }
 
-// Rows of any length, stride and alignment: a warp per group, four neighbouring values a lane, loaded one at a time (the four loads of a warp share their sectors) and
-// stored as one word where the rows of the codes allow it.
-template <typename T>
+// Rows of any length, stride and alignment: a warp takes four groups of a row, four neighbouring values a lane and group, loaded kLoad at a time (what rows and strides
+// allow; the loads of a warp share their sectors) and stored as one word where the rows of the codes allow it.
+constexpr int kAnyGroups = 4;
+template <typename T, int kLoad>
 __global__ void __launch_bounds__(256) k_quantize_fp8_rows_any(const T* __restrict__ x, long long ldx, int x_rows, const int* __restrict__ src_row, int rows, int K,
                                                                uint8_t* __restrict__ codes, long long ldc, float* __restrict__ scales, int words) {
-  const int lane = threadIdx.x & 31, KB = (K + 127) >> 7;
-  const long long units = (long long)rows * KB;
+  struct alignas(sizeof(T) * kLoad) Part { T t[kLoad]; };
+  const int lane = threadIdx.x & 31, KB = (K + 127) >> 7, row = blockIdx.x * 8 + (threadIdx.x >> 5);
   grid_dependency_wait();
   grid_launch_dependents();
-  for (long long u = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); u < units; u += (long long)gridDim.x * 8) {
-    const int row = (int)(u / KB), g = (int)(u - (long long)row * KB), c = g * 128 + lane * 4;
-    const int src = src_row ? src_row[row] : row;
-    const bool gone = src < 0 || src >= x_rows;
-    float v[4], m = 0.f;
+  if (row >= rows) return;
+  const int src = src_row ? src_row[row] : row;
+  const bool gone = src < 0 || src >= x_rows;
+  const T* from = x + (long long)(gone ? 0 : src) * ldx;
+  for (int g0 = blockIdx.y * kAnyGroups; g0 < KB; g0 += gridDim.y * kAnyGroups) {
+    float v[kAnyGroups][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = !gone && c + i < K ? Elem<T>::load(x + (long long)src * ldx + c + i) : 0.f;
+    for (int j = 0; j < kAnyGroups; ++j) {      // all loads in flight
+      const int c = (g0 + j) * 128 + lane * 4;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) m = max_nan(m, fabsf(v[i]));
-    asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(m));
-    const Fp8Scale s = fp8_scale(m);
-    const uint32_t q = cvt_e4m3x4(v[0] * s.factor, v[1] * s.factor, v[2] * s.factor, v[3] * s.factor);
-    uint8_t* o = codes + (long long)row * ldc + c;
-    if (words && c + 4 <= K) {
-      *reinterpret_cast<uint32_t*>(o) = q;
-    } else {
+      for (int i = 0; i < 4; i += kLoad) {
+        if (!gone && c + i + kLoad <= K) {
+          const Part w = *reinterpret_cast<const Part*>(from + c + i);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (c + i < K) o[i] = (uint8_t)(q >> (8 * i));
+          for (int h = 0; h < kLoad; ++h) v[j][i + h] = Elem<T>::load(&w.t[h]);
+        } else {
+#pragma unroll
+          for (int h = 0; h < kLoad; ++h) v[j][i + h] = !gone && c + i + h < K ? Elem<T>::load(from + c + i + h) : 0.f;
+        }
+      }
     }
-    if (lane == 0) scales[(long long)row * KB + g] = gone ? 0.f : s.scale;
+#pragma unroll
+    for (int j = 0; j < kAnyGroups; ++j) {
+      if (g0 + j >= KB) break;
+      const int c = (g0 + j) * 128 + lane * 4;
+      float m = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m = max_nan(m, fabsf(v[j][i]));
+      asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(m));
+      const Fp8Scale s = fp8_scale(m);
+      const uint32_t q = cvt_e4m3x4(v[j][0] * s.factor, v[j][1] * s.factor, v[j][2] * s.factor, v[j][3] * s.factor);
+      uint8_t* o = codes + (long long)row * ldc + c;
+      if (words && c + 4 <= K) {
+        *reinterpret_cast<uint32_t*>(o) = q;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (c + i < K) o[i] = (uint8_t)(q >> (8 * i));
+      }
+      if (lane == 0) scales[(long long)row * KB + g0 + j] = gone ? 0.f : s.scale;
+    }
   }
 }
 
@@ -229,13 +250,25 @@ static int quantize_fp8_rows(const void* x, long long ldx, int x_rows, const int
     void* a2[] = {&xt, &ldx, &x_rows, &K, &head, &next, &ct, &ldc, &scales};
     return launch_kernel((const void*)k_quantize_fp8_copies<T>, (int)((warps + 7) / 8), 256, 0, true, a2, st);
   }
-  const long long blocks = (units + (vec ? 31 : 7)) / (vec ? 32 : 8);
-  const void* fn = vec ? (const void*)k_quantize_fp8_rows<T> : (const void*)k_quantize_fp8_rows_any<T>;
   const T* xt = (const T*)x;
   uint8_t* ct = (uint8_t*)codes;
-  int words = ldc % 4 == 0 && ((uintptr_t)codes & 3) == 0;      // (read by the second form only)
+  if (vec) {
+    void* args[] = {&xt, &ldx, &x_rows, &src_row, &rows, &K, &ct, &ldc, &scales};
+    const long long blocks = (units + 31) / 32;
+    return launch_kernel((const void*)k_quantize_fp8_rows<T>, (int)(blocks < 1 << 30 ? blocks : 1 << 30), 256, 0, true, args, st);
+  }
+  int words = ldc % 4 == 0 && ((uintptr_t)codes & 3) == 0;
   void* args[] = {&xt, &ldx, &x_rows, &src_row, &rows, &K, &ct, &ldc, &scales, &words};
-  return launch_kernel(fn, (int)(blocks < 1 << 30 ? blocks : 1 << 30), 256, 0, true, args, st);
+  const auto loads = [&](int n) { return ldx % n == 0 && (uintptr_t)x % (n * sizeof(T)) == 0; };
+  const void* fn = loads(4) ? (const void*)k_quantize_fp8_rows_any<T, 4> : loads(2) ? (const void*)k_quantize_fp8_rows_any<T, 2> : (const void*)k_quantize_fp8_rows_any<T, 1>;
+  const int quads = ((K + 127) / 128 + kAnyGroups - 1) / kAnyGroups;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((rows + 7) / 8, quads < 65535 ? quads : 65535), cfg.blockDim = dim3(256), cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization, attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr, cfg.numAttrs = 1;
+  B200_CUDA_TRY(cudaLaunchKernelExC(&cfg, fn, args));
+  return B200MOE_OK;
 }
 
 template <typename T>
