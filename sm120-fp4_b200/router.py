@@ -11,6 +11,10 @@ _WS: dict = {}   # (device index, stream) -> scratch tensor, grown on demand: st
 
 
 def _workspace(device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
+    """Kept for the eager calls of one stream, which the stream runs one after the other. A captured call is replayed on any stream, beside graphs that
+    were captured on the same one: it gets scratch of its own, from the graph's memory."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
     key = (device.index, stream)
     ws = _WS.get(key)
     if ws is None or ws.numel() < nbytes:
@@ -21,8 +25,8 @@ def _workspace(device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
 
 def route(ids: torch.Tensor, num_experts: int, experts: torch.Tensor, offsets: torch.Tensor, pairs: torch.Tensor) -> None:
     """Fills the caller's tables on the current stream. The scratch memory of the counting sort is kept per (device, stream)
-    and only grows, so a call of a size seen before allocates nothing (it can be captured into a CUDA graph) and calls on
-    different streams do not share scratch."""
+    and only grows, so a call of a size seen before allocates nothing, and calls on different streams do not share scratch. A call that is
+    captured into a CUDA graph has scratch of its own, in the graph's memory."""
     if ids.dtype != torch.int32 or experts.dtype != torch.int32 or offsets.dtype != torch.int32 or pairs.dtype != torch.int32:
         raise TypeError("route takes int32 tensors")
     p, umax = ids.numel(), experts.numel()
