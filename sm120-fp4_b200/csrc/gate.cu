@@ -530,7 +530,7 @@ int b200moe_balance_loss(const void* logits, int dtype, long long stride, int to
   });
   if (rc) return rc;
   const float* cp = part;
-  int log_cols = 0;      // columns of a block: the power of two from its eighth of the experts on
+  int log_cols = 5;      // columns of a block: the power of two from its eighth of the experts on, 32 at least (1024 / 32 shares are added one after the other)
   while ((1 << log_cols) < (E + kBalanceRanks - 1) / kBalanceRanks) ++log_cols;
   void* args[] = {&cp, &blocks, &E, &log_cols, &loss, &counts, &stats};
   return launch_kernel((const void*)k_balance_sum, kBalanceRanks, 1024, 0, true, args, (cudaStream_t)stream);
