@@ -159,6 +159,7 @@ def check(code: int, what: str = "") -> None:
     raise B200MoEError(code, f"{what or 'b200moe'}: {msg} ({code})")
 
 
+MAX_SIZE = 1 << 30   # rows, columns and tokens of the router's and FP8 operators
 DTYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}   # dtype codes of the C ABI
 
 

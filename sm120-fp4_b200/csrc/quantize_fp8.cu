@@ -303,6 +303,7 @@ int b200moe_quantize_fp8(const void* x, int dtype, long long x_stride, int x_row
                          float* scales, void* workspace, long long workspace_bytes, void* stream) {
   using namespace b200;
   if (rows < 0 || x_rows < 0 || K < 1 || dtype < 0 || dtype > 2 || (x_stride < K && x_rows > 1) || codes_stride < K) return B200MOE_ERR_ARG;
+  if (rows > (1 << 30) || x_rows > (1 << 30) || K > (1 << 30)) return B200MOE_ERR_LIMIT;
   if (rows == 0) return B200MOE_OK;      // (an empty src_row has no address)
   if (!src_row && rows != x_rows) return B200MOE_ERR_ARG;
   if ((!x && x_rows) || !codes || !scales) return B200MOE_ERR_ARG;
@@ -322,7 +323,7 @@ int b200moe_quantize_fp8_blocks(const void* w, int dtype, int E, int N, int K, v
   if (E < 0 || N < 0 || K < 1 || dtype < 0 || dtype > 2 || codes_stride < K) return B200MOE_ERR_ARG;
   if (E == 0 || N == 0) return B200MOE_OK;
   if (!w || !codes || !scales) return B200MOE_ERR_ARG;
-  if ((N + 127) / 128 > 65535) return B200MOE_ERR_LIMIT;
+  if (N > 65535 * 128 || K > (1 << 30)) return B200MOE_ERR_LIMIT;
   const int size = dtype == DT_F32 ? 4 : 2;
   if (((uintptr_t)w & (size - 1)) || ((uintptr_t)scales & 3)) return B200MOE_ERR_ARG;
   cudaStream_t st = (cudaStream_t)stream;

@@ -20,6 +20,12 @@ FP8 = torch.float8_e4m3fn
 GROUP = 128
 
 
+def _sizes(what: str, *tensors) -> None:
+    for t in tensors:
+        if t is not None and any(n > _lib.MAX_SIZE for n in t.shape):
+            raise ValueError(f"{what} takes sizes up to {_lib.MAX_SIZE}, not {tuple(t.shape)}")
+
+
 def _groups(n: int) -> int:
     return -(-n // GROUP)
 
@@ -40,6 +46,7 @@ def quantize_fp8(x: torch.Tensor, src_row: torch.Tensor | None = None):
         raise ValueError(f"expected [M, K] with K >= 1, got {tuple(x.shape)}")
     if x.dtype not in _lib.DTYPES:
         raise TypeError(f"quantize_fp8 takes bf16, fp16 or fp32, not {x.dtype}")
+    _sizes("quantize_fp8", x, src_row)
     device = _lib.one_device("quantize_fp8", x)
     m, k = x.shape
     if x.stride(1) != 1 and k > 1 or x.stride(0) < k and m > 1:
@@ -69,6 +76,7 @@ def quantize_fp8_weight(w: torch.Tensor):
         raise ValueError(f"expected [N, K] or [E, N, K] with K >= 1, got {tuple(w.shape)}")
     if w.dtype not in _lib.DTYPES:
         raise TypeError(f"quantize_fp8_weight takes bf16, fp16 or fp32, not {w.dtype}")
+    _sizes("quantize_fp8_weight", w)
     device = _lib.one_device("quantize_fp8_weight", w)
     w = w.contiguous()
     n, k = w.shape[-2:]
@@ -123,6 +131,7 @@ def matmul_fp8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale:
             return new if type(new) is not int else _lib.check(new, "matmul_fp8")
     if a.dim() != 2 or w.dim() != 2 or a.shape[1] != w.shape[1] or a.shape[1] < 1:
         raise ValueError(f"matmul_fp8: expected [M, K] and [N, K] with K >= 1, got {tuple(a.shape)} and {tuple(w.shape)}")
+    _sizes("matmul_fp8", a, w)
     lda, ldw = _row_stride(a, "matmul_fp8", "a"), _row_stride(w, "matmul_fp8", "w")
     (m, k), n = a.shape, w.shape[0]
     a_scale = _scales(a_scale, (m, _groups(k)), "matmul_fp8", "a_scale")
@@ -146,6 +155,7 @@ def matmul_fp8_experts(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, 
             return new if type(new) is not int else _lib.check(new, what)
     if a.dim() != 2 or w.dim() != 3 or a.shape[1] != w.shape[2] or a.shape[1] < 1 or w.shape[0] < 1:
         raise ValueError(f"{what}: expected [P, K] and [E, N, K] with K >= 1, got {tuple(a.shape)} and {tuple(w.shape)}")
+    _sizes(what, a, w)
     lda, ldw = _row_stride(a, what, "a"), _row_stride(w, what, "w")
     (m, k), (e, n, _) = a.shape, w.shape
     if e > 1 and w.stride(0) != n * ldw:

@@ -19,8 +19,8 @@ def _logits(logits: torch.Tensor, what: str) -> torch.Tensor:
         raise ValueError(f"{what}: expected logits [tokens, experts], got {tuple(logits.shape)}")
     if logits.dtype not in _lib.DTYPES:
         raise TypeError(f"{what} takes bf16, fp16 or fp32 logits, not {logits.dtype}")
-    if not 1 <= logits.shape[1] <= MAX_EXPERTS:
-        raise ValueError(f"{what} takes 1 to {MAX_EXPERTS} experts, not {logits.shape[1]}")
+    if not 1 <= logits.shape[1] <= MAX_EXPERTS or logits.shape[0] > _lib.MAX_SIZE:
+        raise ValueError(f"{what} takes 1 to {MAX_EXPERTS} experts and at most {_lib.MAX_SIZE} tokens, not {tuple(logits.shape)}")
     _lib.one_device(what, logits)
     if logits.stride(1) != 1 and logits.shape[1] > 1 or logits.stride(0) < logits.shape[1] and logits.shape[0] > 1:
         return logits.contiguous()

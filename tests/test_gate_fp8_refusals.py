@@ -6,6 +6,10 @@ import torch
 def test_python_refusals():
     import sm120fp4_b200 as pkg
     x = torch.zeros(4, 8)
+    long = torch.zeros(1, 2).expand((1 << 30) + 1, 2)      # (one row of memory)
+    for fn in (lambda t: pkg.top_k_gate(t, 1), lambda t: pkg.balance_loss(t, torch.zeros(4, 2, dtype=torch.int32)), pkg.quantize_fp8, pkg.quantize_fp8_weight):
+        with pytest.raises(ValueError):
+            fn(long)
     with pytest.raises(ValueError):
         pkg.top_k_gate(torch.zeros(8), 2)
     with pytest.raises(TypeError):
@@ -79,6 +83,11 @@ def test_c_abi_refusals():
     assert h.b200moe_gate(p, 0, 64, 4, 64, 17, 1, p, p, None) == L.ERR_LIMIT
     assert h.b200moe_gate(p + 1, 0, 8, 4, 8, 2, 1, p, p, None) == L.ERR_ARG
     assert h.b200moe_gate(None, 0, 8, 0, 8, 2, 1, None, None, None) == 0
+    assert h.b200moe_gate(p, 0, 8, (1 << 30) + 1, 8, 2, 1, p, p, None) == L.ERR_LIMIT
+    assert h.b200moe_quantize_fp8(p, 0, 16, (1 << 30) + 1, None, (1 << 30) + 1, 16, p, 16, p, None, 0, None) == L.ERR_LIMIT
+    assert h.b200moe_quantize_fp8_blocks(p, 0, 1, 65535 * 128 + 1, 16, p, 16, p, None) == L.ERR_LIMIT
+    assert h.b200moe_matmul_fp8(p, 16, p, p, 16, p, (1 << 30) + 1, 4, 16, p, 0, 4, None) == L.ERR_LIMIT
+    assert h.b200moe_matmul_fp8_experts(p, 16, p, 4, p, 16, p, 1 << 20, p, p, 1, 1 << 11, 16, p, 0, 1 << 11, 0, None) == L.ERR_LIMIT      # rows of all experts beyond 2^31
     assert h.b200moe_gate_backward(p, p, p, None, 0, 8, 4, 8, 2, 0, p, None) == L.ERR_ARG
     assert h.b200moe_balance_workspace_bytes(-1, 8) == L.ERR_ARG and h.b200moe_balance_workspace_bytes(1, 513) == L.ERR_LIMIT
     assert h.b200moe_balance_workspace_bytes(1000, 64) > 0

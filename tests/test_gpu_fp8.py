@@ -335,6 +335,18 @@ def test_experts_tables_with_gaps_and_unknown_experts():
     assert pkg.matmul_fp8_experts(a[:0], sa[:0], w, sw, experts, torch.zeros_like(offsets)).shape == (0, 130)
 
 
+def test_experts_may_come_twice_and_in_any_order():
+    import sm120fp4_b200 as pkg
+    a, sa = pkg.quantize_fp8(randn(90, 256, seed=1).cuda())
+    w, sw = pkg.quantize_fp8_weight(randn(3, 70, 256, seed=2).cuda())
+    experts, off = [2, 0, 2, 1, 0], [0, 30, 31, 60, 60, 90]
+    got = pkg.matmul_fp8_experts(a, sa, w, sw, torch.tensor(experts, dtype=torch.int32, device="cuda"), torch.tensor(off, dtype=torch.int32, device="cuda"))
+    for u, e in enumerate(experts):
+        r = slice(off[u], off[u + 1])
+        if off[u + 1] > off[u]:
+            close(got[r], a[r], sa[r], w[e], sw[e])
+
+
 def test_experts_row_is_the_same_whatever_its_run():
     """A row's result does not depend on the rows beside it, within one form of the kernel."""
     import sm120fp4_b200 as pkg

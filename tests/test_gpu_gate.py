@@ -241,7 +241,7 @@ def test_balance(dtype, t, e, k):
         assert got.shape == () and torch.equal(got_counts, counts)
         adds = -(-t // (16 * min(148, -(-t // 16)))) + 32      # tokens of a warp one after the other, warps of a block
         tol = (rel_p(x) + (adds + 4) * U)
-        assert abs(float(got.double() - loss)) <= tol * float(loss) + 2.0 ** -126
+        assert abs(float(got.detach().double() - loss)) <= tol * float(loss) + 2.0 ** -126
         again = pkg.balance_loss(x, ids)
         assert torch.equal(again[0], got.detach()) and torch.equal(again[1], counts)
         up = torch.tensor(0.37, device="cuda")
@@ -293,6 +293,15 @@ def test_balance_nan_in_padding_stays_there():
     b[0].backward()
     assert torch.equal(a[1], b[1]) and abs(float(a[0]) - float(b[0])) <= 64 * U * float(a[0])
     assert torch.equal(x.grad[:30], clean.grad) and float(x.grad[30:].float().abs().max()) == 0.0
+
+
+def test_balance_counts_an_expert_as_often_as_it_stands():
+    import sm120fp4_b200 as pkg
+    x = logits(3, 8, torch.float32, 1)
+    ids = torch.tensor([[3, 3, 3], [3, 1, -1], [7, 7, 0]], dtype=torch.int32, device="cuda")
+    loss, counts = pkg.balance_loss(x, ids)
+    want = balance64(x, ids, 8)
+    assert counts.tolist() == [1, 1, 0, 4, 0, 0, 0, 2] and torch.equal(counts, want[1]) and abs(float(loss) - float(want[0])) <= (rel_p(x) + 40 * U) * float(want[0])
 
 
 def test_balance_refusals():
