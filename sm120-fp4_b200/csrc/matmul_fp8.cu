@@ -113,11 +113,7 @@ __device__ __forceinline__ bool mbar_wait_lanes(uint32_t bar, uint32_t parity, b
   *abort_flag = 1;
   return false;
 }
-__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
-  return v;
-}
+__device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory"); }
 __device__ __forceinline__ void tmem_ld_32x32b_x32(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
@@ -320,30 +316,22 @@ __device__ __forceinline__ void put_four(const MatmulParams& p, int row, int n, 
     else put_some<DT_F16>(p.out, at, o, p.N - n);
   }
 }
-// This CTA's share of a tile whose inner size is split: 1 / kRanks of it, the sums of all ranks, added in rank order. A thread takes four weights of a row at a
-// time; all of its loads from the ranks' shared memory are in flight together.
+// A tile whose inner size is split over kRanks CTAs: rank r sums the columns (rows of the output) r * NT / kRanks .., to which every CTA has stored its part: red is
+// [rank it came from][column][128 weights] there. Sums in rank order; a thread takes four weights of a row at a time.
 template <int NT, int kRanks>
 __device__ __forceinline__ void mm_add_ranks(const MatmulParams& p, const MmTile& tl, const float* red, int cluster_rank, int tid) {
   using S = MmShape<NT, true, false>;
-  constexpr int kThreads = S::kEpi * 32, kItems = NT * 32 / kRanks, kEach = (kItems + kThreads - 1) / kThreads;
-  const int base = cluster_rank & ~(kRanks - 1), rank = cluster_rank - base;
-  float4 v[kEach][kRanks];
+  constexpr int kThreads = S::kEpi * 32, kItems = NT * 32 / kRanks;
+  const int rank = cluster_rank & (kRanks - 1);
+  for (int i = tid; i < kItems; i += kThreads) {
+    const int row = tl.row0 + rank * (NT / kRanks) + i / 32, n = tl.n0 + (i & 31) * 4;
+    if (row >= tl.row_end || n >= p.N) continue;
+    float4 v[kRanks];
 #pragma unroll
-  for (int j = 0; j < kEach; ++j) {
-    const int i = tid + j * kThreads;
-    if (kItems % kThreads == 0 || i < kItems) {
-      const uint32_t mine = smem_u32(red) + (rank * kItems + i) * 16;
-#pragma unroll
-      for (int r = 0; r < kRanks; ++r) v[j][r] = ld_cluster_f32x4(mapa_shared(mine, base + r));
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < kEach; ++j) {
-    const int i = tid + j * kThreads, at4 = rank * kItems + i, row = tl.row0 + at4 / 32, n = tl.n0 + (at4 & 31) * 4;
-    if ((kItems % kThreads && i >= kItems) || row >= tl.row_end || n >= p.N) continue;
+    for (int r = 0; r < kRanks; ++r) v[r] = *reinterpret_cast<const float4*>(red + (r * kItems + i) * 4);
     float o[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int r = 0; r < kRanks; ++r) o[0] += v[j][r].x, o[1] += v[j][r].y, o[2] += v[j][r].z, o[3] += v[j][r].w;
+    for (int r = 0; r < kRanks; ++r) o[0] += v[r].x, o[1] += v[r].y, o[2] += v[r].z, o[3] += v[r].w;
     put_four(p, row, n, o);
   }
 }
@@ -447,6 +435,7 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
       int kb0, kb1;
       const int t = rounds.tile(i, kb0, kb1);
       const MmTile tl = mm_tile<NT, kSwap, kPair>(p, first, off, kSwap && t < 0 ? 0 : t);
+      if (rounds.shared(i)) cluster_arrive();
       for (int kb = kb0; kb < kb1 && !dead; ++kb) {
         if (!mbar_wait_warp(smem_u32(&empty[st]), ph, abort_flag)) { dead = true; break; }
         const uint32_t bar = smem_u32(&full[st]), sa = smem_u32(smem + st * S::kStageBytes);
@@ -464,7 +453,7 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
         ++issued;
         if (++st == S::kStages) st = 0, ph ^= 1;
       }
-      if (rounds.shared(i)) __syncwarp(), cluster_sync_all(), cluster_sync_all();
+      if (rounds.shared(i)) __syncwarp(), cluster_wait(), cluster_sync_all();
     }
     // The tensor core's word that it has read a slot goes to this CTA's barriers (from the leader, in a pair): all of it arrives before the CTA may end, or it
     // would reach the barriers of the CTA that comes after it.
@@ -482,6 +471,7 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
     for (int i = 0; rounds.has(i); ++i) {
       int kb0, kb1;
       const int t = rounds.tile(i, kb0, kb1);
+      if (rounds.shared(i)) cluster_arrive();
       if constexpr (kSwap && NT > 16) {      // columns for the rows that the tile has
         const MmTile tl = mm_tile<NT, kSwap, kPair>(p, first, off, t < 0 ? 0 : t);
         idesc = idesc_f8(128, min(NT, (tl.row_end - tl.row0 + 15) & ~15));
@@ -515,7 +505,7 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
         if (++st == S::kStages) st = 0, ph ^= 1;
         if (++buf == S::kBufs) buf = 0, bph ^= 1;
       }
-      if (rounds.shared(i)) __syncwarp(), cluster_sync_all(), cluster_sync_all();
+      if (rounds.shared(i)) __syncwarp(), cluster_wait(), cluster_sync_all();
     }
     if (dead) {
       if constexpr (kPair) umma2_commit_p(&drained, 1, el & (rank == 0));
@@ -544,6 +534,7 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
           vb[j] = __ldg(rb + g);
         }
       };
+      if (rounds.shared(i)) cluster_arrive();
       if (!dead && kb0 < kb1) fetch(kb0);
       for (int kb = kb0; kb < kb1 && !dead; kb += 4) {
         float ca[4][R], cb[4];
@@ -576,13 +567,14 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
           if (++buf == S::kBufs) buf = 0, bph ^= 1;
         }
       }
-      if (rounds.shared(i)) __syncwarp(), cluster_sync_all(), cluster_sync_all();
+      if (rounds.shared(i)) __syncwarp(), cluster_wait(), cluster_sync_all();
     }
   }
   } else {                                                           // ---- epilogue
     if constexpr (S::kSplitRegs) regs_inc<S::kEpiRegs>();
     const int quad = warp & 3, half = warp >> 2, col0 = half * S::kCols;
     const int l = quad * 32 + lane;                                  // accumulator lane
+    constexpr int kLogNT = NT == 16 ? 4 : NT == 32 ? 5 : NT == 64 ? 6 : NT == 128 ? 7 : 8;
     bool red_in_use = false;
     const uint32_t lead_empty = mapa_shared(smem_u32(&acc_empty[0]), 0);
     int buf = 0, ph = 0;
@@ -590,6 +582,7 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
       int kb0, kb1;
       const int t = rounds.tile(i, kb0, kb1);
       const MmTile tl = mm_tile<NT, kSwap, kPair>(p, first, off, kSwap && t < 0 ? 0 : t);
+      if (rounds.shared(i)) __syncwarp(), cluster_arrive();      // this CTA is there, and its last tile's sums are read
       float acc[S::kCols];
 #pragma unroll
       for (int j = 0; j < S::kCols; ++j) acc[j] = 0.f;
@@ -651,16 +644,16 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
           }
         }
       } else {
-        // to shared memory [row][128 weights] and out of it again row by row (as they stand, a store instruction writes 64 bytes of one row: 8000 cycles a tile of 64)
-        if (red_in_use) named_bar_sync(1, S::kEpi * 32);      // the last tile's sums are read
-#pragma unroll
-        for (int c = 0; c < S::kCols / S::kChunk; ++c) {
-          const int col = mm_column<NT, kSwap, kPair>(half, c);
-          if (col >= rows) continue;
-#pragma unroll
-          for (int j = 0; j < S::kChunk; ++j) red[(col + j) * 128 + l] = acc[c * S::kChunk + j];
-        }
         if (!rounds.shared(i)) {
+          // to shared memory [row][128 weights] and out of it again row by row (as they stand, a store instruction writes 64 bytes of one row: 8000 cycles a tile of 64)
+          if (red_in_use) named_bar_sync(1, S::kEpi * 32);      // the last tile's sums are read
+#pragma unroll
+          for (int c = 0; c < S::kCols / S::kChunk; ++c) {
+            const int col = mm_column<NT, kSwap, kPair>(half, c);
+            if (col >= rows) continue;
+#pragma unroll
+            for (int j = 0; j < S::kChunk; ++j) red[(col + j) * 128 + l] = acc[c * S::kChunk + j];
+          }
           named_bar_sync(1, S::kEpi * 32);
           red_in_use = true;
           if (!dead && t >= 0)
@@ -670,6 +663,25 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
               if (n < p.N) put_four(p, tl.row0 + (j >> 5), n, {v.x, v.y, v.z, v.w});
             }
         } else {
+          // each column's sums to the CTA that adds them: stores one way instead of loads there and back, and one barrier that is waited for
+          __syncwarp();
+          cluster_wait();
+          if (t >= 0) {
+            const int log_parts = rounds.log_parts, log_own = kLogNT - log_parts, here = rank & ((1 << log_parts) - 1), base = rank - here;
+            const uint32_t mine = smem_u32(red) + (here << log_own) * 512 + l * 4;
+            constexpr int kOwn = NT / 8;      // columns in a row that always have one owner
+#pragma unroll
+            for (int c = 0; c < S::kCols / S::kChunk; ++c) {
+              const int col = mm_column<NT, kSwap, kPair>(half, c);
+              if (col >= rows) continue;
+#pragma unroll
+              for (int g = 0; g < S::kChunk; g += kOwn) {
+                const uint32_t to = mapa_shared(mine + ((col + g) & ((1 << log_own) - 1)) * 512, base + ((col + g) >> log_own));
+#pragma unroll
+                for (int j = 0; j < kOwn; ++j) st_cluster_f32(to + j * 512, acc[c * S::kChunk + g + j]);
+              }
+            }
+          }
           __syncwarp();
           cluster_sync_all();
           if (!dead && t >= 0) {
@@ -677,8 +689,6 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
             else if (rounds.log_parts == 2) mm_add_ranks<NT, 4>(p, tl, red, rank, tid);
             else mm_add_ranks<NT, 8>(p, tl, red, rank, tid);
           }
-          __syncwarp();
-          cluster_sync_all();      // the peers' sums stay until everybody has read them
         }
       }
     }
@@ -780,7 +790,7 @@ static int matmul_cluster(long long tiles, int KB, int sms) {
 }
 
 // One matrix: the form of the least time by that model; many rows take CTA pairs (512 x 4096 x 4096: pairs 19.7 us, single CTAs of 128 x 256 21.1, weights on the
-// lanes 23.0; 200 rows: 18.8, 20.0, 16.0).
+// lanes 23.0; 200 rows: 18.8, 20.0, 14.6).
 // A matrix per expert: by the mean rows of a run, whose lengths the host does not know. Up to 12 tiles of 16 rows; then 128 x 256, which lose less than 10 % to tiles
 // of 32 and 64 while runs are alike (25 rows, 128 experts of 1536 x 2048: 79.6 us, 73.6 and 75.6) and gain where a few are long (19 rows on average, skewed, 2816 x
 // 704: 37.7 us, 61.4 and 58.0); pairs where the rows that tiles of 256 leave empty no longer matter (375 rows: pairs 229 us, single CTAs 217; 1000: 121, 125).
