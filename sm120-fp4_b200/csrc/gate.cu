@@ -4,7 +4,7 @@
 //   balance  L = E sum_e f_e P_e, f_e = n_e / sum n, P_e = mean over live tokens of softmax(l)_e
 //            dl = g E / T' p_e (f_e - sum_j p_j f_j)
 // Measured on the GPU: gate of 16384 x 128 fp32 9.6 us and its gradient 5.7 (issue of 350 instructions a token, 69 % of the slots), of one token 1.8; balance loss of
-// 65536 x 256 bf16 18 us + 2, its gradient 20 (146 and 192 instructions a token at 59 and 70 % of the slots; the bytes are 5 and 10 us).
+// 65536 x 256 bf16 14.7 us + 2, its gradient 20 (about 150 and 190 instructions a token; the bytes are 5 and 10 us). Cold caches, but for the one token.
 // A warp per token with its logits in registers; sums in fp32, statistics by shuffles, no atomic decides a value. A logit of -inf is an
 // expert that may not be taken: a slot for which none is left gets id -1 (an empty slot of the layer) and weight 0.
 #include "common.cuh"
@@ -80,25 +80,17 @@ __device__ __forceinline__ float exp_term(float x, float m) {
   return e;
 }
 
-// Softmax numerators of kTok rows against their maxima, and the lane's share of their sums. Rows of -inf alone: zeros. An infinity or a NaN makes its row NaN.
-template <int V, int kTok>
-__device__ __forceinline__ void softmax_terms(float (&x)[kTok][V], float (&s)[kTok]) {
-  float m[kTok];
+// Softmax numerators against the row's maximum, and the lane's share of their sum. Rows of -inf alone: zeros. An infinity or a NaN makes the row NaN.
+template <int V> __device__ __forceinline__ float softmax_terms(float (&x)[V]) {
+  float m = x[0];
 #pragma unroll
-  for (int i = 0; i < kTok; ++i) {
-    m[i] = x[i][0];
+  for (int j = 1; j < V; ++j) m = max_nan(m, x[j]);
+  m = warp_max(m);
+  if (m == -INFINITY) m = 0.f;
+  float s = 0.f;
 #pragma unroll
-    for (int j = 1; j < V; ++j) m[i] = max_nan(m[i], x[i][j]);
-  }
-#pragma unroll
-  for (int i = 0; i < kTok; ++i) m[i] = warp_max(m[i]);
-#pragma unroll
-  for (int i = 0; i < kTok; ++i) {
-    const float c = m[i] == -INFINITY ? 0.f : m[i];
-    s[i] = 0.f;
-#pragma unroll
-    for (int j = 0; j < V; ++j) x[i][j] = exp_term(x[i][j], c), s[i] += x[i][j];
-  }
+  for (int j = 0; j < V; ++j) x[j] = exp_term(x[j], m), s += x[j];
+  return s;
 }
 
 // An unsigned number in the order of the logits: NaN above all, -0 = +0. 0 is left for experts that are not there.
@@ -232,13 +224,11 @@ __global__ void __launch_bounds__(256) k_gate_backward(const float* __restrict__
 #pragma unroll
     for (int j = 0; j < V; ++j) d[j] = 0.f;
   } else {
-    float x[1][V], s[1];
-    load_row<T, V, kVec>(logits + (long long)t * stride, E, lane, x[0], -INFINITY);
-    softmax_terms<V, 1>(x, s);
-    s[0] = warp_sum(s[0]);
-    const float c = s[0] == 0.f ? 0.f : -dot / s[0];
+    load_row<T, V, kVec>(logits + (long long)t * stride, E, lane, d, -INFINITY);
+    const float s = warp_sum(softmax_terms<V>(d));
+    const float c = s == 0.f ? 0.f : -dot / s;
 #pragma unroll
-    for (int j = 0; j < V; ++j) d[j] = x[0][j] * c;
+    for (int j = 0; j < V; ++j) d[j] *= c;
   }
   T* row = out + (long long)t * E;
   store_row<T, V, kVec>(row, E, lane, d);
@@ -251,17 +241,14 @@ __global__ void __launch_bounds__(256) k_gate_backward(const float* __restrict__
 // launch adds the blocks in order. part: per block E floats, E ints, live tokens.
 __host__ __device__ inline int balance_words(int E) { return 2 * E + 4; }
 
-// Up to 256 experts a warp has two tokens in hand, so that the chains load -> maximum -> sum overlap.
-constexpr int kBalanceRanks = 8;
-template <int V> struct BalanceShape {
-  static constexpr int kWarps = V <= 8 ? 32 : 16, kTok = V <= 8 ? 2 : 1;      // 32 KB of partial sums
-};
-constexpr int kBalanceBlocks = 148;
+// 64 warps an SM hide the chain load -> maximum -> sum (two tokens in hand a warp at half of that took 17.4 instead of 14.5 us at 65536 x 256).
+constexpr int kBalanceRanks = 8, kBalanceBlocks = 296;
+template <int V> constexpr int kBalanceWarps = V <= 8 ? 32 : 16;      // 32 KB of partial sums
 
 template <typename T, int V, bool kVec>
-__global__ void __launch_bounds__(BalanceShape<V>::kWarps * 32) k_balance_part(const T* __restrict__ logits, long long stride, int tokens, int E, const int* __restrict__ ids,
-                                                                               int k, float* __restrict__ part) {
-  constexpr int kWarps = BalanceShape<V>::kWarps, kTok = BalanceShape<V>::kTok;
+__global__ void __launch_bounds__(kBalanceWarps<V> * 32, 2) k_balance_part(const T* __restrict__ logits, long long stride, int tokens, int E, const int* __restrict__ ids, int k,
+                                                                           float* __restrict__ part) {
+  constexpr int kWarps = kBalanceWarps<V>;
   __shared__ float sp[kWarps][32 * V];
   __shared__ int cnt[32 * V], live_n;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -273,36 +260,17 @@ __global__ void __launch_bounds__(BalanceShape<V>::kWarps * 32) k_balance_part(c
 #pragma unroll
   for (int j = 0; j < V; ++j) acc[j] = 0.f;
   int n = 0;
-  const int step = gridDim.x * kWarps * kTok;
-  for (int t0 = (blockIdx.x * kWarps + warp) * kTok; t0 < tokens; t0 += step) {
-    float x[kTok][V], s[kTok];
-    int e[kTok];
+  for (int t = blockIdx.x * kWarps + warp; t < tokens; t += gridDim.x * kWarps) {
+    const int e = lane < k ? ids[(long long)t * k + lane] : -1;
+    float x[V];
+    load_row<T, V, kVec>(logits + (long long)t * stride, E, lane, x, -INFINITY);
+    const bool used = e >= 0 && e < E;
+    if (used) atomicAdd(&cnt[e], 1);
+    if (!__any_sync(0xffffffffu, used)) continue;      // an empty token
+    ++n;
+    const float s = warp_sum(softmax_terms<V>(x)), r = s == 0.f ? 0.f : __frcp_rn(s);
 #pragma unroll
-    for (int i = 0; i < kTok; ++i) {
-      const bool in = t0 + i < tokens;
-      e[i] = in && lane < k ? ids[(long long)(t0 + i) * k + lane] : -1;
-      load_row<T, V, kVec>(logits + (long long)(in ? t0 + i : t0) * stride, E, lane, x[i], -INFINITY);
-    }
-    bool live[kTok];
-#pragma unroll
-    for (int i = 0; i < kTok; ++i) {
-      const bool used = e[i] >= 0 && e[i] < E;
-      if (used) atomicAdd(&cnt[e[i]], 1);
-      live[i] = __any_sync(0xffffffffu, used);      // else an empty token
-      n += live[i];
-    }
-    softmax_terms<V, kTok>(x, s);
-#pragma unroll
-    for (int o = 16; o; o >>= 1)
-#pragma unroll
-      for (int i = 0; i < kTok; ++i) s[i] += __shfl_xor_sync(0xffffffffu, s[i], o);
-#pragma unroll
-    for (int i = 0; i < kTok; ++i) {
-      if (!live[i]) continue;
-      const float r = s[i] == 0.f ? 0.f : __frcp_rn(s[i]);
-#pragma unroll
-      for (int j = 0; j < V; ++j) acc[j] = fmaf(x[i][j], r, acc[j]);
-    }
+    for (int j = 0; j < V; ++j) acc[j] = fmaf(x[j], r, acc[j]);
   }
   if (lane == 0 && n) atomicAdd(&live_n, n);
 #pragma unroll
@@ -319,7 +287,7 @@ __global__ void __launch_bounds__(BalanceShape<V>::kWarps * 32) k_balance_part(c
   if (threadIdx.x == 0) reinterpret_cast<int*>(o)[2 * E] = live_n;
 }
 
-// One cluster: a block takes an eighth of the experts, a column of threads for each, every thread of which adds one of `slices` shares of the partial sums (148 at
+// One cluster: a block takes an eighth of the experts, a column of threads for each, every thread of which adds one of `slices` shares of the partial sums (296 at
 // most: loads of a thread are in flight together); the experts' sums meet in block 0. stats: f32 [2]: 1 / pairs, E / live tokens (at least 1 of both).
 __global__ void __cluster_dims__(kBalanceRanks, 1, 1) __launch_bounds__(1024)
     k_balance_sum(const float* __restrict__ part, int blocks, int E, int log_cols, float* __restrict__ loss, int* __restrict__ counts, float* __restrict__ stats) {
@@ -391,7 +359,7 @@ __global__ void __cluster_dims__(kBalanceRanks, 1, 1) __launch_bounds__(1024)
 }
 
 template <typename T, int V, bool kVec>
-__global__ void __launch_bounds__(256) k_balance_backward(const float* __restrict__ grad, const T* __restrict__ logits, long long stride, int tokens, int E,
+__global__ void __launch_bounds__(256, V <= 8 ? 8 : 4) k_balance_backward(const float* __restrict__ grad, const T* __restrict__ logits, long long stride, int tokens, int E,
                                                           const int* __restrict__ ids, int k, const int* __restrict__ counts, const float* __restrict__ stats,
                                                           T* __restrict__ out) {
   const int lane = threadIdx.x & 31;
@@ -400,36 +368,24 @@ __global__ void __launch_bounds__(256) k_balance_backward(const float* __restric
   float f[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) f[j] = lane * V + j < E ? (float)counts[lane * V + j] * inv : 0.f;
-  constexpr int kTok = BalanceShape<V>::kTok;
-  const int step = gridDim.x * 8 * kTok;
-  for (int t0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * kTok; t0 < tokens; t0 += step) {
-    float x[kTok][V], s[kTok], dot[kTok];
-    int e[kTok];
+  for (int t = blockIdx.x * 8 + (threadIdx.x >> 5); t < tokens; t += gridDim.x * 8) {
+    const int e = lane < k ? ids[(long long)t * k + lane] : -1;
+    float x[V];
+    load_row<T, V, kVec>(logits + (long long)t * stride, E, lane, x, -INFINITY);
+    if (__any_sync(0xffffffffu, e >= 0 && e < E)) {
+      float s = softmax_terms<V>(x), dot = 0.f;
 #pragma unroll
-    for (int i = 0; i < kTok; ++i) {
-      const bool in = t0 + i < tokens;
-      e[i] = in && lane < k ? ids[(long long)(t0 + i) * k + lane] : -1;
-      load_row<T, V, kVec>(logits + (long long)(in ? t0 + i : t0) * stride, E, lane, x[i], -INFINITY);
+      for (int j = 0; j < V; ++j) dot = fmaf(x[j], f[j], dot);
+#pragma unroll
+      for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o), dot += __shfl_xor_sync(0xffffffffu, dot, o);
+      const float r = s == 0.f ? 0.f : __frcp_rn(s), mean = dot * r, rc = r * c;
+#pragma unroll
+      for (int j = 0; j < V; ++j) x[j] *= rc * (f[j] - mean);
+    } else {      // an empty token
+#pragma unroll
+      for (int j = 0; j < V; ++j) x[j] = 0.f;
     }
-    softmax_terms<V, kTok>(x, s);
-#pragma unroll
-    for (int i = 0; i < kTok; ++i) {
-      dot[i] = 0.f;
-#pragma unroll
-      for (int j = 0; j < V; ++j) dot[i] = fmaf(x[i][j], f[j], dot[i]);
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1)
-#pragma unroll
-      for (int i = 0; i < kTok; ++i) s[i] += __shfl_xor_sync(0xffffffffu, s[i], o), dot[i] += __shfl_xor_sync(0xffffffffu, dot[i], o);
-#pragma unroll
-    for (int i = 0; i < kTok; ++i) {
-      const bool live = __any_sync(0xffffffffu, e[i] >= 0 && e[i] < E);
-      const float r = s[i] == 0.f ? 0.f : __frcp_rn(s[i]), mean = dot[i] * r, rc = r * c;
-#pragma unroll
-      for (int j = 0; j < V; ++j) x[i][j] = live ? x[i][j] * rc * (f[j] - mean) : 0.f;
-      if (t0 + i < tokens) store_row<T, V, kVec>(out + (long long)(t0 + i) * E, E, lane, x[i]);
-    }
+    store_row<T, V, kVec>(out + (long long)t * E, E, lane, x);
   }
 }
 
@@ -525,7 +481,7 @@ int b200moe_balance_loss(const void* logits, int dtype, long long stride, int to
       const T* lp = (const T*)logits;
       void* args[] = {&lp, &stride, &tokens, &E, &ids, &k, &part};
       const void* fn = vec_rows(logits, stride, E, sizeof(T)) ? (const void*)k_balance_part<T, V, true> : (const void*)k_balance_part<T, V, false>;
-      return launch_kernel(fn, blocks, BalanceShape<V>::kWarps * 32, 0, true, args, (cudaStream_t)stream);
+      return launch_kernel(fn, blocks, kBalanceWarps<V> * 32, 0, true, args, (cudaStream_t)stream);
     });
   });
   if (rc) return rc;
