@@ -60,7 +60,7 @@ def test_quantize_rows(dtype, m, k):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("m,copies,k", [(600, 8, 1024), (2000, 2, 2816), (300, 30, 704), (1500, 3, 1040), (4096, 8, 512)])
+@pytest.mark.parametrize("m,copies,k", [(1400, 8, 1024), (2000, 2, 2816), (600, 30, 704), (4000, 3, 1040), (4096, 8, 512), (9000, 8, 160)])
 def test_quantize_many_copies(dtype, m, copies, k):
     """Rows that are asked for several times in calls large enough for the lists: some twice as often, some never, some indexes outside."""
     import sm120fp4_b200 as pkg
