@@ -791,9 +791,10 @@ static int matmul_cluster(long long tiles, int KB, int sms) {
 
 // One matrix: the form of the least time by that model; many rows take CTA pairs (512 x 4096 x 4096: pairs 19.7 us, single CTAs of 128 x 256 21.1, weights on the
 // lanes 23.0; 200 rows: 18.8, 20.0, 14.6).
-// A matrix per expert: by the mean rows of a run, whose lengths the host does not know. Up to 12 tiles of 16 rows; then 128 x 256, which lose less than 10 % to tiles
-// of 32 and 64 while runs are alike (25 rows, 128 experts of 1536 x 2048: 79.6 us, 73.6 and 75.6) and gain where a few are long (19 rows on average, skewed, 2816 x
-// 704: 37.7 us, 61.4 and 58.0); pairs where the rows that tiles of 256 leave empty no longer matter (375 rows: pairs 229 us, single CTAs 217; 1000: 121, 125).
+// A matrix per expert: by the mean rows of a run, whose lengths the host does not know. A few rows take tiles of 16; from 8 on (3 where the inner size has four
+// groups or less, and a tile's ends count for more) 128 x 256, which lose some to them while runs are alike and gain more where a few are long (us, tiles of 16 / 128 x 256, 8 rows:
+// 1536 x 2048 alike 72.8 / 81.1, skewed 44.8 / 43.7; 2816 x 704 52.3 / 55.5, 41.7 / 32.9; 1536 x 512 48.0 / 45.3, 36.7 / 25.4; 3 rows of it 45.3 / 40.8, 24.0 / 22.1);
+// pairs where the rows that tiles of 256 leave empty no longer matter (375 rows: pairs 229 us, single CTAs 217; 1000: 121, 125).
 static int matmul(const MatmulParams& p, const void* a, long long lda, const void* w, long long ldw, cudaStream_t st) {
   const int sms = sm_count();
   if (sms <= 0) return B200MOE_ERR_DEVICE;
@@ -803,7 +804,7 @@ static int matmul(const MatmulParams& p, const void* a, long long lda, const voi
     const long long runs = p.U < p.M ? p.U : p.M, mean = p.M / runs;
     const auto tiles = [&](int r, int c) { return (p.M / r + runs) * ((p.N + c - 1) / c); };      // (at most)
     if (mean > 512) return launch_matmul<256, false, true>(p, a, lda, w, ldw, tiles(256, 256), 1, sms, st);
-    if (mean > 12) return launch_matmul<256, false, false>(p, a, lda, w, ldw, tiles(128, 256), 1, sms, st);
+    if (mean > (p.KB <= 4 ? 2 : 7)) return launch_matmul<256, false, false>(p, a, lda, w, ldw, tiles(128, 256), 1, sms, st);
     rows = 16, n = tiles(rows, 128), cluster = matmul_cluster(n, p.KB, sms);
   } else {
     const auto tiles = [&](int r, int c) { return (long long)((p.M + r - 1) / r) * ((p.N + c - 1) / c); };

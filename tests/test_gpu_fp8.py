@@ -288,7 +288,8 @@ def runs_of(counts):
 
 
 @pytest.mark.parametrize("counts,n,k", [([1], 64, 128), ([1, 0, 2, 1], 1536, 256), ([5, 17, 0, 1, 40], 300, 704), ([200, 3, 129, 0, 1], 257, 300), ([0, 0, 0], 64, 64),
-                                        ([16] * 40, 704, 512), ([130, 1, 500, 127, 128, 0, 300, 90], 1408, 640), ([1500], 200, 384), ([2] * 300, 48, 160), ([600, 255, 1, 900, 0, 513], 1400, 300)])
+                                        ([16] * 40, 704, 512), ([130, 1, 500, 127, 128, 0, 300, 90], 1408, 640), ([1500], 200, 384), ([2] * 300, 48, 160), ([600, 255, 1, 900, 0, 513], 1400, 300), ([900, 130, 0, 1300], 1400, 300),
+                                        ([3, 0, 5, 1, 9] * 8, 520, 640), ([40] + [1] * 50, 300, 512)])
 def test_experts(counts, n, k):
     import sm120fp4_b200 as pkg
     e = len(counts) + 2
