@@ -16,7 +16,7 @@ LIB_PATH = Path(os.environ["B200MOE_LIB"]) if os.environ.get("B200MOE_LIB") else
 _lib = None
 _host = None
 ONE_CLUSTER = 8192 * 16   # values of one matrix up to which the quantiser keeps them in registers and takes no workspace
-NO_HOST = SimpleNamespace(**{name: lambda *args: None for name in ("quantize_own_scale", "quantize_128x4", "top_k_gate", "balance_loss", "quantize_fp8", "matmul_fp8", "matmul_fp8_experts")})
+NO_HOST = SimpleNamespace(**{name: lambda *args: None for name in ("quantize_own_scale", "quantize_128x4", "top_k_gate", "balance_loss", "quantize_fp8", "quantize_fp8_weight", "matmul_fp8", "matmul_fp8_experts")})
 
 ERR_ARG, ERR_SHAPE, ERR_CUDA, ERR_DEVICE, ERR_TIMEOUT, ERR_WORKSPACE, ERR_LIMIT, ERR_RANGE, ERR_ORDER = -1, -2, -3, -4, -5, -6, -7, -8, -9
 
@@ -143,8 +143,9 @@ def host():
         if module is not NO_HOST:
             module.bind(*(C.cast(f, C.c_void_p).value for f in (h.b200moe_quantize_nvfp4_own_scale, h.b200moe_quantize_nvfp4)), ONE_CLUSTER)
             module.bind_ops(*(C.cast(f, C.c_void_p).value for f in (
-                h.b200moe_gate, h.b200moe_gate_backward, h.b200moe_balance_workspace_bytes, h.b200moe_balance_loss, h.b200moe_balance_backward, h.b200moe_quantize_fp8_workspace_bytes, h.b200moe_quantize_fp8,
-                h.b200moe_matmul_fp8, h.b200moe_matmul_fp8_experts, h.b200moe_error_string)))
+                h.b200moe_gate, h.b200moe_gate_backward, h.b200moe_balance_workspace_bytes, h.b200moe_balance_loss, h.b200moe_balance_backward,
+                h.b200moe_quantize_fp8_workspace_bytes, h.b200moe_quantize_fp8, h.b200moe_quantize_fp8_blocks, h.b200moe_matmul_fp8, h.b200moe_matmul_fp8_experts,
+                h.b200moe_error_string)))
         _host = module
     return _host
 

@@ -136,6 +136,7 @@ struct Ops {
   int (*balance_backward)(const void*, const void*, int, long long, int, int, const void*, int, const void*, const void*, void*, void*);
   long long (*quantize_fp8_workspace_bytes)(int, int, int);
   int (*quantize_fp8)(const void*, int, long long, int, const void*, int, int, void*, long long, void*, void*, long long, void*);
+  int (*quantize_fp8_blocks)(const void*, int, int, int, int, void*, long long, void*, void*);
   int (*matmul_fp8)(const void*, long long, const void*, const void*, long long, const void*, int, int, int, void*, int, long long, void*);
   int (*matmul_fp8_experts)(const void*, long long, const void*, int, const void*, long long, const void*, int, const void*, const void*, int, int, int, void*, int, long long,
                             int, void*);
@@ -351,6 +352,28 @@ PyObject* py_quantize_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// quantize_fp8_weight(w): a matrix or stacked ones
+PyObject* py_quantize_fp8_weight(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 1 || !tensors(args, 1)) Py_RETURN_NONE;
+  const at::Tensor w = THPVariable_Unpack(args[0]);
+  if (!here(w) || (w.dim() != 2 && w.dim() != 3) || dtype_code(w.scalar_type()) < 0 || w.numel() < 1 || !w.is_contiguous() || w.size(-1) > kMaxSize || w.size(-2) > 65535 * 128 ||
+      w.size(0) > kMaxSize)
+    Py_RETURN_NONE;
+  const int64_t e = w.dim() == 3 ? w.size(0) : 1, rows = w.size(-2), k = w.size(-1), ld = (k + 15) & ~15ll, nb = (rows + 127) / 128, kb = (k + 127) / 128;
+  at::Tensor codes, scales;
+  int rc;
+  {
+    Released released;
+    const auto options = at::TensorOptions().dtype(at::kFloat8_e4m3fn).device(w.device());
+    codes = w.dim() == 3 ? at::empty_strided({e, rows, k}, {rows * ld, ld, 1}, options) : at::empty_strided({rows, k}, {ld, 1}, options);
+    scales = w.dim() == 3 ? fresh({e, nb, kb}, at::kFloat, w) : fresh({nb, kb}, at::kFloat, w);
+    rc = ops.quantize_fp8_blocks(w.data_ptr(), dtype_code(w.scalar_type()), (int)e, (int)rows, (int)k, codes.data_ptr(), ld, scales.data_ptr(), raw_stream());
+  }
+  return pair(rc, codes, scales);
+  END_HANDLE_TH_ERRORS
+}
+
 // bytes between rows of codes that the products take as they are, 0 for others
 int64_t codes_stride(const at::Tensor& t) {
   if (!here(t) || t.scalar_type() != at::kFloat8_e4m3fn) return 0;
@@ -409,6 +432,7 @@ PyMethodDef methods[] = {{"bind", (PyCFunction)(void (*)(void))py_bind, METH_FAS
                          {"top_k_gate", (PyCFunction)(void (*)(void))py_top_k_gate, METH_FASTCALL, nullptr},
                          {"balance_loss", (PyCFunction)(void (*)(void))py_balance_loss, METH_FASTCALL, nullptr},
                          {"quantize_fp8", (PyCFunction)(void (*)(void))py_quantize_fp8, METH_FASTCALL, nullptr},
+                         {"quantize_fp8_weight", (PyCFunction)(void (*)(void))py_quantize_fp8_weight, METH_FASTCALL, nullptr},
                          {"matmul_fp8", (PyCFunction)(void (*)(void))py_matmul_fp8, METH_FASTCALL, nullptr},
                          {"matmul_fp8_experts", (PyCFunction)(void (*)(void))py_matmul_fp8_experts, METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};

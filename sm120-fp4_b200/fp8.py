@@ -72,6 +72,9 @@ def quantize_fp8(x: torch.Tensor, src_row: torch.Tensor | None = None):
 def quantize_fp8_weight(w: torch.Tensor):
     """w [N, K] or stacked experts [E, N, K], bf16, fp16 or fp32 -> (codes float8_e4m3fn of the same shape, scales f32 [..., ceil(N / 128), ceil(K / 128)]), a scale
     for every 128x128 block, as in quantize_fp8."""
+    out = (_lib._host or _lib.host()).quantize_fp8_weight(w)      # (as in quantize_fp8)
+    if out is not None:
+        return out if type(out) is tuple else _lib.check(out, "quantize_fp8_weight")
     if w.dim() not in (2, 3) or w.shape[-1] < 1:
         raise ValueError(f"expected [N, K] or [E, N, K] with K >= 1, got {tuple(w.shape)}")
     if w.dtype not in _lib.DTYPES:

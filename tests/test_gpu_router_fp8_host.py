@@ -58,6 +58,9 @@ def test_fp8_outputs(monkeypatch):
             assert _lib.host().quantize_fp8(x, s) is not None
             same(pkg.quantize_fp8(x, src_row=s), general(monkeypatch, lambda: pkg.quantize_fp8(x, src_row=s)))
         a, sa = pkg.quantize_fp8(x)
+        for v in (randn(3, 200, k, seed=1), randn(131, k, seed=2).half(), randn(1, 1, k, seed=3).bfloat16()):
+            assert _lib.host().quantize_fp8_weight(v) is not None
+            same(pkg.quantize_fp8_weight(v), general(monkeypatch, lambda: pkg.quantize_fp8_weight(v)))
         w, sw = pkg.quantize_fp8_weight(randn(3, 200, k, seed=1))
         for dtype in (torch.bfloat16, torch.float32):
             assert _lib.host().matmul_fp8(a, sa, w[0], sw[0], dtype) is not None
@@ -77,7 +80,8 @@ def test_what_is_left_to_the_general_path():
     for i in (ids.long(), ids[:4], ids.cpu(), ids[0], ids.t(), torch.zeros(8, 33, dtype=torch.int32, device="cuda"), None):
         assert h.balance_loss(x, i) is None
     for v in (x.t(), x[:0], x[0], x.double(), x.cpu(), None):
-        assert h.quantize_fp8(v, None) is None
+        assert h.quantize_fp8(v, None) is None and h.quantize_fp8_weight(v) is None
+    assert h.quantize_fp8_weight(x[:, :32]) is None and h.quantize_fp8_weight(x[None, None]) is None
     for s in (ids, ids[:, 0], ids[0].long(), ids[0].cpu(), 3):
         assert h.quantize_fp8(x, s) is None
     a, sa = pkg.quantize_fp8(randn(4, 256))
