@@ -3,7 +3,7 @@
 //            dl = w_j (g_j - sum g w) at id_j (normalised), or p_e (g_e - sum g w) for all experts
 //   balance  L = E sum_e f_e P_e, f_e = n_e / sum n, P_e = mean over live tokens of softmax(l)_e
 //            dl = g E / T' p_e (f_e - sum_j p_j f_j)
-// Measured on the GPU: gate of 16384 x 128 fp32 9.6 us and its gradient 5.7 (issue of 350 instructions a token, 69 % of the slots), of one token 1.8; balance loss of
+// Measured on the GPU: gate of 16384 x 128 fp32 9.6 us and its gradient 5.7 (issue of about 300 instructions a token, 69 % of the slots), of one token 1.8; balance loss of
 // 65536 x 256 bf16 14.7 us + 2, its gradient 20 (about 150 and 190 instructions a token; the bytes are 5 and 10 us). Cold caches, but for the one token.
 // A warp per token with its logits in registers; sums in fp32, statistics by shuffles, no atomic decides a value. A logit of -inf is an
 // expert that may not be taken: a slot for which none is left gets id -1 (an empty slot of the layer) and weight 0.
@@ -93,11 +93,10 @@ template <int V> __device__ __forceinline__ float softmax_terms(float (&x)[V]) {
   return s;
 }
 
-// An unsigned number in the order of the logits: NaN above all, -0 = +0. 0 is left for experts that are not there.
+// An unsigned number in the order of the logits: NaN above all, -0 = +0 (the addition gives the one NaN, 0x7fffffff, and no -0).
 __device__ __forceinline__ uint32_t order_key(float v) {
-  if (v != v) return 0xffffffffu;
   const uint32_t u = __float_as_uint(v + 0.f);
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+  return u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float key_value(uint32_t k) {
   if (k == 0xffffffffu) return NAN;
@@ -115,11 +114,18 @@ template <int V, bool kPacked> struct Candidates {
       const uint32_t hi = max(key[a], key[b]), lo = min(key[a], key[b]);
       key[a] = hi, key[b] = lo;
     } else {
-      const bool turn = key[a] < key[b] || (key[a] == key[b] && idx[a] > idx[b]);
+      const bool turn = V <= 8 ? key[a] < key[b] : key[a] < key[b] || (key[a] == key[b] && idx[a] > idx[b]);
       const uint32_t k = key[a], i = idx[a];
       key[a] = turn ? key[b] : k, key[b] = turn ? k : key[b];
       idx[a] = turn ? idx[b] : i, idx[b] = turn ? i : idx[b];
     }
+  }
+  // Neighbours alone change places, so that equal keys stay in the order of their indexes without a look at these.
+  __device__ __forceinline__ void sort_neighbours() {
+#pragma unroll
+    for (int n = V - 1; n > 0; --n)
+#pragma unroll
+      for (int i = 0; i < n; ++i) order(i, i + 1);
   }
   // Batcher's odd-even merge sort of key[kFrom .. kFrom + kCount - 1]
   template <int kFrom, int kCount, int kStep> __device__ __forceinline__ void merge() {
@@ -149,7 +155,7 @@ template <int V, bool kPacked> struct Candidates {
   }
 };
 
-// Bound by issue (eight of 128 experts in 32 bits: 350 instructions a token; with a scan of all candidates in every round 11.2 us instead of 9.6 at 16384 tokens).
+// Bound by issue (eight of 128 experts in 32 bits: about 300 instructions a token; with a scan of all candidates in every round 11.2 us instead of 9.4 at 16384 tokens).
 template <typename T, int V, bool kVec>
 __global__ void __launch_bounds__(256) k_gate(const T* __restrict__ logits, long long stride, int tokens, int E, int k, int renorm, float* __restrict__ weights,
                                               int* __restrict__ ids) {
@@ -162,15 +168,17 @@ __global__ void __launch_bounds__(256) k_gate(const T* __restrict__ logits, long
   load_row<T, V, kVec>(logits + (long long)t * stride, E, lane, x, -INFINITY);
   Candidates<V, kPacked> c;
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
+  for (int j = 0; j < V; ++j) {      // (beyond E: -inf; if such a one is taken, none but masked ones are left)
     const int e = lane * V + j;
-    c.key[j] = e < E ? order_key(x[j]) : 0u;
-    if constexpr (kPacked) c.key[j] = e < E ? (c.key[j] & ~511u) | (511 - e) : 0u;
+    c.key[j] = order_key(x[j]);
+    if constexpr (kPacked) c.key[j] = (c.key[j] & ~511u) | (511 - e);
     else c.idx[j] = e;
   }
-  c.template sort<0, V>();
+  if constexpr (kPacked || V > 8) c.template sort<0, V>();
+  else c.sort_neighbours();
   uint32_t mine = 0u;      // lane j: key and index of the j-th largest
   int at = -1;
+#pragma unroll 2
   for (int j = 0; j < k; ++j) {
     const uint32_t top = __reduce_max_sync(0xffffffffu, c.key[0]);
     if constexpr (kPacked) {
@@ -192,14 +200,17 @@ __global__ void __launch_bounds__(256) k_gate(const T* __restrict__ logits, long
   const float m = first <= kKeyMasked ? 0.f : key_value(first);
   const float w = live ? exp_term(key_value(mine), m) : 0.f;
   float s = w;
-  if (!renorm) {
+  if (renorm) {
+#pragma unroll
+    for (int o = 8; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);      // (16 lanes have all of it)
+  } else {
     s = 0.f;
 #pragma unroll
     for (int j = 0; j < V; ++j) s += exp_term(x[j], m);
+    s = warp_sum(s);
   }
-  s = warp_sum(s);
   if (lane < k) {
-    weights[(long long)t * k + lane] = live ? w / s : 0.f;
+    weights[(long long)t * k + lane] = live ? w * __frcp_rn(s) : 0.f;
     ids[(long long)t * k + lane] = live ? at : -1;
   }
 }

@@ -135,6 +135,12 @@ def test_gate_extreme_values():
     assert ids[3].tolist() == [5, 6] and w[3].isnan().all()        # NaN above all, and seen in the weights
     assert ids[4, 0] == 2 and w[4].isnan().any()
     assert ids[5].tolist() == [-1, -1] and w[5].tolist() == [0.0, 0.0]
+    for bits, dtype in ((0xFFC1, torch.bfloat16), (0xFE01, torch.float16)):      # a NaN with its sign bit set is a NaN like any other
+        y = torch.zeros(1, 40, dtype=dtype)
+        y.view(torch.int16)[0, 17] = bits - 65536
+        w2, ids2 = pkg.top_k_gate(y.cuda(), 2)
+        w3, ids3 = pkg.top_k_gate(y.cuda().float(), 2)
+        assert ids2.tolist() == ids3.tolist() == [[17, 0]] and bool(w2.isnan().all()) and bool(w3.isnan().all())
     assert int(ids.max()) < 16
 
 
