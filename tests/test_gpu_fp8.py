@@ -411,6 +411,31 @@ def test_layer_from_router_to_combine():
     pkg.matmul_fp8_status()
 
 
+def test_layer_of_a_padded_batch():
+    """Tokens that may use no expert (logits of -inf) have ids of -1 from the gate on: no expert counts them, no run holds them, the rows behind the last run are zeros."""
+    import sm120fp4_b200 as pkg
+    for t, live, e, k in [(40, 25, 16, 4), (3000, 1801, 32, 2)]:
+        x, logit = randn(t, 256, seed=1).bfloat16().cuda(), randn(t, e, seed=2).cuda()
+        logit[live:] = -math.inf
+        logit[:live, 3] = -math.inf      # an expert that is switched off
+        w, sw = pkg.quantize_fp8_weight(randn(e, 130, 256, seed=3).cuda())
+        weights, ids = pkg.top_k_gate(logit, k)
+        loss, counts = pkg.balance_loss(logit, ids)
+        experts, offsets, pairs = pkg.route_tables(ids, e)
+        assert int(ids[live:].max()) == -1 and int(ids[:live].min()) >= 0 and float(weights[live:].abs().max()) == 0.0
+        assert int(counts.sum()) == live * k == int(offsets[-1]) and int(counts[3]) == 0
+        q, s = pkg.quantize_fp8(x, src_row=pairs // k)
+        y = pkg.matmul_fp8_experts(q, s, w, sw, experts, offsets, out_dtype=torch.float32)
+        begin = offsets.tolist()
+        for u, i in enumerate(experts.tolist()):
+            if begin[u + 1] > begin[u]:
+                r = slice(begin[u], begin[u + 1])
+                assert i != 3 and int(counts[i]) == begin[u + 1] - begin[u]
+                close(y[r], q[r], s[r], w[i], sw[i])
+                assert same(q[r], codes64(x[(pairs[r] // k).long()], 1)[0])
+        assert float(y[live * k:].abs().max()) == 0.0
+
+
 def test_products_on_two_streams_at_once():
     import sm120fp4_b200 as pkg
     sets = [operands(m, n, k, 31 * m) for m, n, k in [(8, 1024, 2048), (700, 4096, 512)]]
