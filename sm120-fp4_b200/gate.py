@@ -1,5 +1,5 @@
 """The router from its logits on: `top_k_gate` gives the (weights, ids) that `Weights.forward` and `route` take, `balance_loss` the auxiliary loss that
-keeps experts evenly used, with the number of pairs of each. Both have gradients with respect to the logits. The reference leaves this part to
+keeps experts evenly used, with the number of pairs of each. Both have gradients with respect to the logits (reverse mode; forward mode is refused). The reference leaves this part to
 torch (softmax, top-k, renormalise: sm120fp4/kernels/moe_layer.py:195-200).
 
 Nothing here synchronises or keeps state between calls: forward and backward can be captured into a CUDA graph. A capture of a backward pass wants, as with
@@ -15,6 +15,8 @@ MAX_EXPERTS, MAX_TOP_K = 512, 16
 
 
 def _logits(logits: torch.Tensor, what: str) -> torch.Tensor:
+    if torch.autograd.forward_ad.unpack_dual(logits).tangent is not None:      # outputs without a tangent would read as a derivative of zero
+        raise NotImplementedError(f"{what} has no forward-mode derivative")
     if logits.dim() != 2:
         raise ValueError(f"{what}: expected logits [tokens, experts], got {tuple(logits.shape)}")
     if logits.dtype not in _lib.DTYPES:
