@@ -122,6 +122,13 @@ def lib() -> C.CDLL:
     return _lib
 
 
+def host_functions(h: C.CDLL) -> tuple:
+    """The library's functions that the host extension calls for the router and the FP8 operators, in the order in which it keeps them."""
+    return (h.b200moe_gate, h.b200moe_gate_backward, h.b200moe_balance_workspace_bytes, h.b200moe_balance_loss, h.b200moe_balance_backward,
+            h.b200moe_quantize_fp8_workspace_bytes, h.b200moe_quantize_fp8, h.b200moe_quantize_fp8_blocks, h.b200moe_matmul_fp8, h.b200moe_matmul_fp8_experts,
+            h.b200moe_error_string)
+
+
 def host():
     """The native host side of small calls (csrc/host.cpp), bound to the loaded library; NO_HOST, which takes no call, beside a library that
     came without it, or with one that was built for another torch: every call then takes its general path, to the same kernels."""
@@ -142,10 +149,7 @@ def host():
             warnings.warn(f"the host extension is left out, small calls take longer: {why}; build it again with `python {_PKG / 'build.py'}`", RuntimeWarning, stacklevel=3)
         if module is not NO_HOST:
             module.bind(*(C.cast(f, C.c_void_p).value for f in (h.b200moe_quantize_nvfp4_own_scale, h.b200moe_quantize_nvfp4)), ONE_CLUSTER)
-            module.bind_ops(*(C.cast(f, C.c_void_p).value for f in (
-                h.b200moe_gate, h.b200moe_gate_backward, h.b200moe_balance_workspace_bytes, h.b200moe_balance_loss, h.b200moe_balance_backward,
-                h.b200moe_quantize_fp8_workspace_bytes, h.b200moe_quantize_fp8, h.b200moe_quantize_fp8_blocks, h.b200moe_matmul_fp8, h.b200moe_matmul_fp8_experts,
-                h.b200moe_error_string)))
+            module.bind_ops(*(C.cast(f, C.c_void_p).value for f in host_functions(h)))
         _host = module
     return _host
 

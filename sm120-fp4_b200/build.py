@@ -48,11 +48,19 @@ HOST_SRC, HOST = CSRC / "host.cpp", PKG / f"_host{sysconfig.get_config_var('EXT_
 HOST_BUILT_BY = PKG / "build" / "host.command"
 
 
+def one_cxx_library(cxx: str) -> list[str]:
+    """The extension takes the C++ library that torch has loaded. A compiler that knows it as an archive only would put a second one into the extension, and the two share
+    some of their objects and not others: writing a number to a stream ends the process."""
+    r = subprocess.run([cxx, "-print-file-name=libstdc++.so"], stdout=subprocess.PIPE, text=True)
+    return ["-nostdlib++"] if r.stdout.strip() == "libstdc++.so" else []      # (the bare name: there is no such file)
+
+
 def host_command(out: Path) -> list[str]:
     import torch
     root = Path(torch.__file__).resolve().parent
     cuda = Path(nvcc()).resolve().parent.parent
-    return [os.environ.get("CXX") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+    cxx = os.environ.get("CXX") or "g++"
+    return [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", *one_cxx_library(cxx), f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
             f'-DB200_TORCH_VERSION="{torch.__version__}"',
             f"-I{root / 'include'}", f"-I{cuda / 'include'}", f"-I{sysconfig.get_paths()['include']}", str(HOST_SRC), "-o", str(out),
             f"-L{root / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]

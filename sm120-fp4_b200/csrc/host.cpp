@@ -154,7 +154,9 @@ bool plain_logits(const at::Tensor& x) {
 }
 long long row_stride(const at::Tensor& x) { return std::max(x.stride(0), x.size(1)); }
 bool vector_of(const at::Tensor& t, at::ScalarType type) { return here(t) && t.dim() == 1 && t.scalar_type() == type && t.is_contiguous(); }
-void checked(int rc, const char* what) { TORCH_CHECK(rc == 0, what, ": ", ops.error_string(rc), " (", rc, ")"); }
+void checked(int rc, const char* what) {      // (the message as one string: no streams)
+  if (rc) TORCH_CHECK(false, std::string(what) + ": " + ops.error_string(rc) + " (" + std::to_string(rc) + ")");
+}
 // The gradient of a gradient is not there: whoever asks for it is told so.
 at::Tensor once(at::Tensor out, const char* what) {
   if (!at::GradMode::is_enabled()) return out;

@@ -1,5 +1,6 @@
 """Corners of the router and FP8 operators: tensors that are not stored as they read, derivatives that are not there, padded batches, rows that are asked for very
 often, outputs with the longest rows."""
+import ctypes as C
 import math
 
 import pytest
@@ -44,6 +45,23 @@ def test_forward_mode_is_refused(path):
     for call in (lambda t: pkg.top_k_gate(t, 2)[0], lambda t: pkg.balance_loss(t, ids)[0]):
         with pytest.raises(RuntimeError):
             torch.func.jvp(call, (x,), (torch.ones_like(x),))
+
+
+def test_an_error_in_a_gradient_reaches_the_caller():
+    """The library says no inside a backward pass, on a thread of the autograd engine: an exception like any other."""
+    h, host, no = L.lib(), L.host(), C.CFUNCTYPE(C.c_int, *L.SIGNATURES["b200moe_gate_backward"][1])(lambda *args: L.ERR_ARG)
+    functions = L.host_functions(h)
+    x = randn(5, 16, seed=1).requires_grad_(True)
+    w = pkg.top_k_gate(x, 3)[0]
+    assert host.top_k_gate(x, 3, True) is not None
+    try:
+        host.bind_ops(*(C.cast(no, C.c_void_p).value if f is h.b200moe_gate_backward else C.cast(f, C.c_void_p).value for f in functions))
+        with pytest.raises(RuntimeError, match=r"top_k_gate backward: bad argument.*\(-1\)"):
+            w.sum().backward()
+    finally:
+        host.bind_ops(*(C.cast(f, C.c_void_p).value for f in functions))
+    pkg.top_k_gate(x, 3)[0].sum().backward()
+    assert x.grad is not None
 
 
 # ---------------------------------------------------------------------------------------------------- tensors that are not stored as they read

@@ -16,3 +16,12 @@ def test_forward_mode_is_refused():
                 call()
         with pytest.raises(RuntimeError, match="GPU"):      # plain tensors get as far as ever
             pkg.top_k_gate(x, 2)
+
+
+def test_the_host_extension_has_no_cxx_library_of_its_own():
+    """Two C++ libraries in a process share some of their objects and not others: numbers written to a stream end it."""
+    import sm120fp4_b200._lib as L
+    host = L.host()
+    assert host is not L.NO_HOST
+    with open(host.__file__, "rb") as f:
+        assert b"St7codecvtIDsc" not in f.read()      # (a part of the library that nothing here names)
