@@ -168,6 +168,14 @@ MAX_SIZE = 1 << 30   # rows, columns and tokens of the router's and FP8 operator
 DTYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}   # dtype codes of the C ABI
 
 
+def stored(t: torch.Tensor) -> torch.Tensor:
+    """t with its values in memory as they read: the sign of a negated view (the imaginary part of a conjugate is one) is a mark beside them, and the zeros that some
+    gradients are made of have no memory at all."""
+    if t._is_zerotensor():
+        t = t.clone()
+    return t.resolve_neg()
+
+
 def one_device(what: str, *tensors) -> torch.device:
     """The device that all of them are on: a GPU."""
     device = tensors[0].device

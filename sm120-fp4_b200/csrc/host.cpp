@@ -40,7 +40,7 @@ bool plain_tensor(const at::Tensor& t) {
   using c10::DispatchKey;
   const c10::DispatchKeySet k = t.key_set();
   return t.is_cuda() && t.layout() == at::kStrided && !k.has(DispatchKey::Python) && !k.has(DispatchKey::FuncTorchBatched) && !k.has(DispatchKey::FuncTorchGradWrapper) &&
-         !k.has(DispatchKey::Functionalize) && !k.has(DispatchKey::Negative);
+         !k.has(DispatchKey::Functionalize) && !k.has(DispatchKey::Negative) && !k.has(DispatchKey::ZeroTensor);
 }
 
 // a matrix the kernels take as it is: bf16 or fp32, whole blocks of 16, contiguous, on the current device
@@ -164,6 +164,13 @@ at::Tensor once(at::Tensor out, const char* what) {
   return (*error)({out.detach().requires_grad_(true)})[0];
 }
 
+// A gradient with its values in memory as they read: the sign of a negated view is a mark beside them, and some gradients are zeros without memory.
+at::Tensor stored(const at::Tensor& grad) {
+  at::Tensor t = grad.detach();
+  if (t._is_zerotensor()) t = t.clone();
+  return t.resolve_neg().contiguous();
+}
+
 // A leaf's gradient is handed over on the stream on which its accumulator was made. Where an eager graph keeps that alive, a backward pass that is being captured
 // on another stream would have the engine wait across the two, which ends the process: refused while it still can be.
 void check_capture(const at::Tensor& x, const char* what) {
@@ -202,7 +209,7 @@ struct GateBackward : torch::autograd::Node {
   variable_list apply(variable_list&& grads) override {
     std::lock_guard<std::mutex> lock(mutex_);
     if (!grads[0].defined() || !task_should_compute_output(0)) return {at::Tensor()};
-    const at::Tensor w = weights.unpack(shared_from_this()), i = ids.unpack(), l = renormalize ? at::Tensor() : x.unpack(), grad = grads[0].detach().contiguous();
+    const at::Tensor w = weights.unpack(shared_from_this()), i = ids.unpack(), l = renormalize ? at::Tensor() : x.unpack(), grad = stored(grads[0]);
     const at::Tensor out = fresh({w.size(0), e}, dtype, w);
     checked(ops.gate_backward(grad.data_ptr(), w.data_ptr(), i.data_ptr(), l.defined() ? l.data_ptr() : nullptr, dtype_code(dtype), l.defined() ? row_stride(l) : e, (int)w.size(0),
                               (int)e, (int)w.size(1), renormalize, out.data_ptr(), raw_stream()),
@@ -239,7 +246,7 @@ struct BalanceBackward : torch::autograd::Node {
   variable_list apply(variable_list&& grads) override {
     std::lock_guard<std::mutex> lock(mutex_);
     if (!grads[0].defined() || !task_should_compute_output(0)) return {at::Tensor()};
-    const at::Tensor l = x.unpack(), i = ids.unpack(), c = counts.unpack(), s = stats.unpack(), grad = grads[0].detach().contiguous();
+    const at::Tensor l = x.unpack(), i = ids.unpack(), c = counts.unpack(), s = stats.unpack(), grad = stored(grads[0]);
     const at::Tensor out = fresh({l.size(0), l.size(1)}, l.scalar_type(), l);
     checked(ops.balance_backward(grad.data_ptr(), l.data_ptr(), dtype_code(l.scalar_type()), row_stride(l), (int)l.size(0), (int)l.size(1), i.data_ptr(), (int)i.size(1), c.data_ptr(),
                                  s.data_ptr(), out.data_ptr(), raw_stream()),

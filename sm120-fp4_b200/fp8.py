@@ -49,6 +49,7 @@ def quantize_fp8(x: torch.Tensor, src_row: torch.Tensor | None = None):
     _sizes("quantize_fp8", x, src_row)
     device = _lib.one_device("quantize_fp8", x)
     m, k = x.shape
+    x = _lib.stored(x)
     if x.stride(1) != 1 and k > 1 or x.stride(0) < k and m > 1:
         x = x.contiguous()
     rows = m
@@ -56,7 +57,7 @@ def quantize_fp8(x: torch.Tensor, src_row: torch.Tensor | None = None):
         if src_row.dtype != torch.int32 or src_row.dim() != 1:
             raise TypeError("quantize_fp8: src_row is int32 [R]")
         _lib.one_device("quantize_fp8", x, src_row)
-        src_row = src_row.contiguous()
+        src_row = _lib.stored(src_row).contiguous()
         rows = src_row.shape[0]
     ld = _pad16(k)
     codes = torch.empty_strided((rows, k), (ld, 1), dtype=FP8, device=device)
@@ -81,7 +82,7 @@ def quantize_fp8_weight(w: torch.Tensor):
         raise TypeError(f"quantize_fp8_weight takes bf16, fp16 or fp32, not {w.dtype}")
     _sizes("quantize_fp8_weight", w)
     device = _lib.one_device("quantize_fp8_weight", w)
-    w = w.contiguous()
+    w = _lib.stored(w).contiguous()
     n, k = w.shape[-2:]
     e = w.shape[0] if w.dim() == 3 else 1
     ld = _pad16(k)
@@ -107,7 +108,7 @@ def _scales(s: torch.Tensor, shape: tuple, what: str, name: str) -> torch.Tensor
         raise TypeError(f"{what}: {name} is fp32, not {s.dtype}")
     if tuple(s.shape) != shape:
         raise ValueError(f"{what}: expected {name} {list(shape)}, got {list(s.shape)}")
-    return s.contiguous()
+    return _lib.stored(s).contiguous()
 
 
 def _output(out, out_dtype, m: int, n: int, device, what: str):
@@ -119,6 +120,8 @@ def _output(out, out_dtype, m: int, n: int, device, what: str):
         raise TypeError(f"{what}: out is {out.dtype}, not {out_dtype}")
     if tuple(out.shape) != (m, n) or out.device != device:
         raise ValueError(f"{what}: expected out [{m}, {n}] on {device}, got {list(out.shape)} on {out.device}")
+    if out.is_neg():
+        raise ValueError(f"{what}: out is a negated view")
     if out.stride(1) != 1 and n > 1 or out.stride(0) < n and m > 1:
         raise ValueError(f"{what}: rows of out must be contiguous and apart from one another (strides {out.stride()})")
     return out
@@ -135,6 +138,7 @@ def matmul_fp8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale:
     if a.dim() != 2 or w.dim() != 2 or a.shape[1] != w.shape[1] or a.shape[1] < 1:
         raise ValueError(f"matmul_fp8: expected [M, K] and [N, K] with K >= 1, got {tuple(a.shape)} and {tuple(w.shape)}")
     _sizes("matmul_fp8", a, w)
+    a, w = _lib.stored(a), _lib.stored(w)
     lda, ldw = _row_stride(a, "matmul_fp8", "a"), _row_stride(w, "matmul_fp8", "w")
     (m, k), n = a.shape, w.shape[0]
     a_scale = _scales(a_scale, (m, _groups(k)), "matmul_fp8", "a_scale")
@@ -159,6 +163,7 @@ def matmul_fp8_experts(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, 
     if a.dim() != 2 or w.dim() != 3 or a.shape[1] != w.shape[2] or a.shape[1] < 1 or w.shape[0] < 1:
         raise ValueError(f"{what}: expected [P, K] and [E, N, K] with K >= 1, got {tuple(a.shape)} and {tuple(w.shape)}")
     _sizes(what, a, w)
+    a, w = _lib.stored(a), _lib.stored(w)
     lda, ldw = _row_stride(a, what, "a"), _row_stride(w, what, "w")
     (m, k), (e, n, _) = a.shape, w.shape
     if e > 1 and w.stride(0) != n * ldw:
@@ -170,7 +175,7 @@ def matmul_fp8_experts(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, 
     a_scale = _scales(a_scale, (m, _groups(k)), what, "a_scale")
     w_scale = _scales(w_scale, (e, _groups(n), _groups(k)), what, "w_scale")
     device = _lib.one_device(what, a, a_scale, w, w_scale, experts, offsets)
-    experts, offsets = experts.contiguous(), offsets.contiguous()
+    experts, offsets = _lib.stored(experts).contiguous(), _lib.stored(offsets).contiguous()
     zero = out is None
     out = _output(out, out_dtype or (torch.bfloat16 if zero else None), m, n, device, what)
     _lib.call(device, what, _lib.lib().b200moe_matmul_fp8_experts, a.data_ptr(), lda, a_scale.data_ptr(), m, w.data_ptr(), ldw, w_scale.data_ptr(), e, experts.data_ptr(),

@@ -24,6 +24,7 @@ def _logits(logits: torch.Tensor, what: str) -> torch.Tensor:
     if not 1 <= logits.shape[1] <= MAX_EXPERTS or logits.shape[0] > _lib.MAX_SIZE:
         raise ValueError(f"{what} takes 1 to {MAX_EXPERTS} experts and at most {_lib.MAX_SIZE} tokens, not {tuple(logits.shape)}")
     _lib.one_device(what, logits)
+    logits = _lib.stored(logits)
     if logits.stride(1) != 1 and logits.shape[1] > 1 or logits.stride(0) < logits.shape[1] and logits.shape[0] > 1:
         return logits.contiguous()
     return logits
@@ -60,7 +61,7 @@ class _Gate(torch.autograd.Function):
         dtype, e = ctx.like
         tokens, k = weights.shape
         out = torch.empty((tokens, e), dtype=dtype, device=weights.device)
-        grad = grad.detach().contiguous()
+        grad = _lib.stored(grad.detach()).contiguous()
         _lib.call(out.device, "top_k_gate backward", _lib.lib().b200moe_gate_backward, grad.data_ptr(), weights.data_ptr(), ids.data_ptr(), _lib.ptr(logits),
                   _lib.DTYPES[dtype], e if logits is None else max(logits.stride(0), e), tokens, e, k, int(ctx.renormalize), out.data_ptr())
         return _once(out, "top_k_gate"), None, None
@@ -108,7 +109,7 @@ class _Balance(torch.autograd.Function):
         logits, ids, counts, stats = ctx.saved_tensors
         tokens, e = logits.shape
         out = torch.empty((tokens, e), dtype=logits.dtype, device=logits.device)
-        grad = grad.detach().contiguous()
+        grad = _lib.stored(grad.detach()).contiguous()
         _lib.call(out.device, "balance_loss backward", _lib.lib().b200moe_balance_backward, grad.data_ptr(), logits.data_ptr(), _lib.DTYPES[logits.dtype],
                   max(logits.stride(0), e), tokens, e, ids.data_ptr(), ids.shape[1], counts.data_ptr(), stats.data_ptr(), out.data_ptr())
         return _once(out, "balance_loss"), None
@@ -128,7 +129,7 @@ def balance_loss(logits: torch.Tensor, ids: torch.Tensor):
     if ids.dim() != 2 or ids.shape[0] != logits.shape[0] or not 1 <= ids.shape[1] <= 32:
         raise ValueError(f"balance_loss: expected ids [{logits.shape[0]}, 1 to 32], got {tuple(ids.shape)}")
     _lib.one_device("balance_loss", logits, ids)
-    ids = ids.contiguous()
+    ids = _lib.stored(ids).contiguous()
     if logits.requires_grad and torch.is_grad_enabled():
         return _Balance.apply(logits, ids)
     return _balance(logits, ids)[:2]

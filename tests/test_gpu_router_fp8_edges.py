@@ -66,6 +66,68 @@ def test_an_error_in_a_gradient_reaches_the_caller():
 
 # ---------------------------------------------------------------------------------------------------- tensors that are not stored as they read
 
+def test_negated_views(path):
+    """torch keeps the sign of some views (the imaginary part of a conjugate) as a mark beside the values."""
+    x, ids = randn(20, 64, seed=1), torch.randint(0, 64, (20, 2), generator=torch.Generator().manual_seed(2)).int().cuda()
+    for dtype in (torch.float32, torch.bfloat16):
+        y = x.to(dtype)
+        neg = torch._neg_view(y)
+        assert neg.is_neg()
+        for renormalize in (True, False):
+            for a, b in zip(pkg.top_k_gate(neg, 4, renormalize), pkg.top_k_gate(-y, 4, renormalize)):
+                assert torch.equal(a, b)
+        for a, b in zip(pkg.balance_loss(neg, ids), pkg.balance_loss(-y, ids)):
+            assert torch.equal(a, b)
+        for call in (pkg.quantize_fp8, pkg.quantize_fp8_weight):
+            for a, b in zip(call(neg), call(-y)):
+                assert same(a, b)
+    a, sa = pkg.quantize_fp8(randn(20, 256, seed=3))
+    w, sw = pkg.quantize_fp8_weight(randn(40, 256, seed=4))
+    for bad in (lambda: pkg.matmul_fp8(torch._neg_view(a), sa, w, sw), lambda: pkg.matmul_fp8(a, sa, torch._neg_view(w), sw),
+                lambda: pkg.matmul_fp8(a, sa, w, sw, out=torch._neg_view(torch.zeros(20, 40, device="cuda")))):
+        with pytest.raises((RuntimeError, ValueError)):      # codes cannot be negated, an output would read as its negative
+            bad()
+    assert torch.equal(pkg.matmul_fp8(a, torch._neg_view(sa), w, sw), pkg.matmul_fp8(a, -sa, w, sw))
+    assert torch.equal(pkg.matmul_fp8(a, sa, w, torch._neg_view(sw)), pkg.matmul_fp8(a, sa, w, -sw))
+
+
+def test_gradients_that_come_as_negated_views(path):
+    """What arrives where weights are the imaginary part of a number whose conjugate is used."""
+    logits, c = randn(20, 16, seed=1), torch.complex(randn(20, 4, seed=2), randn(20, 4, seed=3))
+    for renormalize in (True, False):
+        def grad_of(gate):
+            x, seen = logits.clone().requires_grad_(True), []
+            w = gate(x)
+            w.register_hook(lambda g: seen.append(g.is_neg()) and None)
+            (torch.complex(torch.ones_like(w), w).conj() * c).real.sum().backward()
+            return x.grad, seen
+
+        def plain(x):
+            w = torch.softmax(x.double(), 1).gather(1, pkg.top_k_gate(logits, 4)[1].long())
+            return (w / w.sum(1, keepdim=True) if renormalize else w).float()
+        got, seen = grad_of(lambda x: pkg.top_k_gate(x, 4, renormalize)[0])
+        assert seen == [True]
+        want = grad_of(plain)[0]
+        # a gradient is a few products and sums of terms that are at most |g| <= 4 in size, each step off by 2^-24 of them: 2^-16 is far above, a wrong sign far above that
+        assert float((got - want).abs().max()) <= 2.0 ** -16 and float(want.abs().max()) > 2.0 ** -4
+        x = logits.clone().requires_grad_(True)
+        loss = pkg.balance_loss(x, pkg.top_k_gate(logits, 4)[1])[0]
+        g1, = torch.autograd.grad(loss, x, torch._neg_view(torch.ones_like(loss)), retain_graph=True)
+        g2, = torch.autograd.grad(loss, x, torch.full_like(loss, -1.0))
+        assert torch.equal(g1, g2) and float(g1.abs().max()) > 0
+
+
+def test_gradients_that_come_without_memory(path):
+    """The gradient of sgn is a tensor of zeros that has no memory."""
+    for renormalize in (True, False):
+        x = randn(20, 16, seed=1).requires_grad_(True)
+        torch.sgn(pkg.top_k_gate(x, 4, renormalize)[0]).sum().backward()
+        assert float(x.grad.abs().max()) == 0.0
+    x = randn(20, 16, seed=1).requires_grad_(True)
+    torch.sgn(pkg.balance_loss(x, pkg.top_k_gate(x.detach(), 4)[1])[0]).backward()
+    assert float(x.grad.abs().max()) == 0.0
+
+
 # ---------------------------------------------------------------------------------------------------- rows outside every run
 
 def best_us(fn, n=7):
