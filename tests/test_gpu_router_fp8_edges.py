@@ -142,3 +142,49 @@ def best_us(fn, n=7):
         b.synchronize()
         times.append(a.elapsed_time(b) * 1e3)
     return min(times)
+
+
+@pytest.mark.parametrize("n", [1, 7, 8, 130, 1408, 5003])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rows_outside_every_run_are_zeros(n, dtype):
+    """Before, between (experts that are not there) and behind the runs, with rows on 16 bytes and off them, whatever memory held."""
+    p, k = 700, 256
+    a, sa = pkg.quantize_fp8(randn(p, k, seed=1))
+    w, sw = pkg.quantize_fp8_weight(randn(3, n, k, seed=2))
+    experts = torch.tensor([2, -1, 0, 7, 1], dtype=torch.int32, device="cuda")
+    offsets = torch.tensor([5, 40, 290, 291, 400, 410], dtype=torch.int32, device="cuda")
+    kept = torch.full((p, n), 3.0, dtype=dtype, device="cuda")
+    pkg.matmul_fp8_experts(a, sa, w, sw, experts, offsets, out=kept)
+    dirty = torch.full((p, n), 7.0, dtype=dtype, device="cuda")      # (the next new tensor of this size is that memory)
+    del dirty
+    got = pkg.matmul_fp8_experts(a, sa, w, sw, experts, offsets, out_dtype=dtype)
+    for s in (slice(0, 5), slice(40, 290), slice(291, 400), slice(410, p)):
+        assert float(got[s].abs().max()) == 0.0 and bool((kept[s] == 3).all())
+    for s in (slice(5, 40), slice(290, 291), slice(400, 410)):
+        assert torch.equal(got[s], kept[s])
+
+
+def test_rows_outside_every_run_beyond_31_bits():
+    """A row of 2^29 values of 32 bits is 2^31 bytes."""
+    n = 1 << 29
+    a, sa = pkg.quantize_fp8(randn(2, 16, seed=1))
+    w, sw = torch.zeros(1, n, 16, dtype=torch.uint8, device="cuda").view(FP8), torch.ones(1, n // 128, 1, device="cuda")
+    w.view(torch.uint8)[0, -1] = 0x38      # ones
+    dirty = torch.full((2, n), 7.0, device="cuda")
+    del dirty
+    got = pkg.matmul_fp8_experts(a, sa, w, sw, torch.tensor([0], dtype=torch.int32, device="cuda"), torch.tensor([0, 1], dtype=torch.int32, device="cuda"), out_dtype=torch.float32)
+    assert float(got[1].abs().max()) == 0.0 and float(got[0, :-1].abs().max()) == 0.0
+    want = float((a[0].double() * sa[0].double()).sum())      # 16 exact products, summed in fp32, times a scale
+    assert abs(float(got[0, -1]) - want) <= 17 * 2.0 ** -23 * float((a[0].double() * sa[0].double()).abs().sum())
+
+
+def test_rows_outside_every_run_take_the_time_of_their_bytes():
+    """Half of a prompt's pairs are padding. The rows that are zeroed are 100 MB, 16 us at the rate of memory; a single SM would need more than a millisecond."""
+    p, n, k = 32768, 1536, 256
+    a, sa = pkg.quantize_fp8(randn(p, k, seed=1))
+    w, sw = pkg.quantize_fp8_weight(randn(16, n, k, seed=2))
+    experts, offsets = torch.arange(16, dtype=torch.int32, device="cuda"), (torch.arange(17, device="cuda") * (p // 32)).int()
+    out = torch.empty(p, n, dtype=torch.bfloat16, device="cuda")
+    left = best_us(lambda: pkg.matmul_fp8_experts(a, sa, w, sw, experts, offsets, out=out))
+    zeroed = best_us(lambda: pkg.matmul_fp8_experts(a, sa, w, sw, experts, offsets))
+    assert zeroed <= left + 200, f"{left:.0f} us without the zeros, {zeroed:.0f} with them"
