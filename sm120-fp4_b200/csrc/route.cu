@@ -2,7 +2,8 @@
 // sm120fp4/kernels/fc1_w4a16.py:272-279 (stable argsort of the flattened ids) and with the fixed-size padded form the
 // reference's GPU router writes (sm120fp4/kernels/moe_w4a16.py:48-83: unused expert slots -1, unused offsets P).
 // The reference ranks each pair with an O(P^2) loop in one block; here a stable counting sort over chunks of pairs
-// scales to prefill sizes (P = 65,536 and beyond): no atomic decides any position.
+// scales to prefill sizes (P = 65,536 and beyond): no atomic decides any position. Pairs of empty slots (ids below 0, or from E on) are in no run: the places behind
+// the last one, as many, are -1.
 #include "common.cuh"
 #include <atomic>
 
@@ -33,7 +34,7 @@ __global__ void __launch_bounds__(128) k_route_hist(const int* __restrict__ ids,
 __global__ void __launch_bounds__(1024) k_route_scan(int* __restrict__ hist, int nchunks, int P, int E, int Umax,
                                                      int* __restrict__ experts, int* __restrict__ offsets,
                                                      int* __restrict__ expert_base /* [E], start of expert e in pairs */,
-                                                     int* __restrict__ num_touched) {
+                                                     int* __restrict__ num_touched, int* __restrict__ num_routed) {
   __shared__ int base[ROUTE_MAXE], uidx[ROUTE_MAXE];
   const int t = threadIdx.x;
   int c = 0;
@@ -74,20 +75,22 @@ __global__ void __launch_bounds__(1024) k_route_scan(int* __restrict__ hist, int
   }
   if (t == 0) {
     if (U <= Umax) offsets[U] = routed;
-    if (num_touched) *num_touched = U;
+    *num_touched = U;
+    *num_routed = routed;
   }
 }
 
 // Pass 3: one warp per chunk walks its pairs in index order, 32 at a time. Within a step, pairs of the same expert are
 // ranked by lane; across steps a per-expert running count in shared memory carries the order. Position of pair p =
-// expert_base[e] + (pairs of e in earlier chunks) + (pairs of e earlier in this chunk).
+// expert_base[e] + (pairs of e in earlier chunks) + (pairs of e earlier in this chunk). The chunk's own places behind the last run are set to -1.
 __global__ void __launch_bounds__(32) k_route_place(const int* __restrict__ ids, int P, int E, const int* __restrict__ hist,
-                                                    const int* __restrict__ expert_base, int* __restrict__ pairs) {
+                                                    const int* __restrict__ expert_base, const int* __restrict__ num_routed, int* __restrict__ pairs) {
   extern __shared__ int run[];
-  const int lane = threadIdx.x;
+  const int lane = threadIdx.x, routed = *num_routed;
   for (int e = lane; e < E; e += 32) run[e] = expert_base[e] + hist[(long long)blockIdx.x * E + e];
   __syncwarp();
   const int p0 = blockIdx.x * ROUTE_CHUNK, p1 = min(P, p0 + ROUTE_CHUNK);
+  for (int p = max(p0, routed) + lane; p < p1; p += 32) pairs[p] = -1;
   int mine[ROUTE_CHUNK / 32];   // this lane's ids of the chunk, all loads in flight at once
 #pragma unroll
   for (int k = 0; k < ROUTE_CHUNK / 32; ++k) mine[k] = p0 + 32 * k + lane < p1 ? ids[p0 + 32 * k + lane] : -1;
@@ -122,7 +125,7 @@ __global__ void __launch_bounds__(1024) k_route_small(const int* __restrict__ id
                                                       int* __restrict__ num_touched) {
   __shared__ int wc[32][kRouteSmallMaxE];     // pairs of expert e in warp w's range, then the start of that range's run in `pairs`
   __shared__ int tot[kRouteSmallMaxE], uidx[kRouteSmallMaxE];
-  __shared__ int s_bad;
+  __shared__ int s_bad, s_routed;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   for (int i = tid; i < 32 * kRouteSmallMaxE; i += 1024) (&wc[0][0])[i] = 0;
   if (tid == 0) s_bad = 0;
@@ -170,9 +173,11 @@ __global__ void __launch_bounds__(1024) k_route_small(const int* __restrict__ id
       if (U <= Umax) offsets[U] = routed;
       if (num_touched) *num_touched = U;
       if (bad) *bad = s_bad;
+      s_routed = routed;
     }
   }
   __syncthreads();
+  for (int p = s_routed + tid; p < P; p += 1024) pairs[p] = -1;   // behind the last run
   for (int e = lane; e < kRouteSmallMaxE; e += 32) wc[warp][e] += tot[e];   // this warp's running position per expert
   __syncwarp();
   for (int s = p0; s < p1; s += 32) {
@@ -198,7 +203,7 @@ using namespace b200;
 extern "C" long long b200moe_route_workspace_bytes(int P, int E) {
   if (P < 0 || E <= 0) return B200MOE_ERR_ARG;
   const long long nchunks = (P + ROUTE_CHUNK - 1) / ROUTE_CHUNK;
-  return (nchunks * E + E + 2) * (long long)sizeof(int);
+  return (nchunks * E + E + 3) * (long long)sizeof(int);
 }
 
 // ids int32 [P] -> experts int32 [Umax], offsets int32 [Umax+1], pairs int32 [P]; Umax slots as the caller sized them
@@ -215,6 +220,7 @@ extern "C" int b200moe_route(const int* ids, int P, int E, int Umax, int* expert
   int* expert_base = hist + (long long)nchunks * E;
   int* bad = expert_base + E;
   int* num_touched = bad + 1;
+  int* num_routed = bad + 2;
   if (P > 0 && P <= kRouteSmallMaxP && E <= kRouteSmallMaxE) {   // small batch: one launch
     k_route_small<<<1, 1024, 0, st>>>(ids, P, E, Umax, experts, offsets, pairs, bad, num_touched);
     B200_LAUNCH_CHECK();
@@ -225,10 +231,10 @@ extern "C" int b200moe_route(const int* ids, int P, int E, int Umax, int* expert
     k_route_hist<<<nchunks, 128, E * sizeof(int), st>>>(ids, P, E, hist, bad);
     B200_LAUNCH_CHECK();
   }
-  k_route_scan<<<1, 1024, 0, st>>>(hist, nchunks, P, E, Umax, experts, offsets, expert_base, num_touched);
+  k_route_scan<<<1, 1024, 0, st>>>(hist, nchunks, P, E, Umax, experts, offsets, expert_base, num_touched, num_routed);
   B200_LAUNCH_CHECK();
   if (nchunks > 0) {
-    k_route_place<<<nchunks, 32, E * sizeof(int), st>>>(ids, P, E, hist, expert_base, pairs);
+    k_route_place<<<nchunks, 32, E * sizeof(int), st>>>(ids, P, E, hist, expert_base, num_routed, pairs);
     B200_LAUNCH_CHECK();
   }
   return B200MOE_OK;
@@ -260,7 +266,7 @@ extern "C" int b200moe_route_status(const void* workspace, int P, int E, void* s
 // until the process exits.
 constexpr int kRouteStaticMaxPairs = 65536;   // 8192 tokens x top-8
 constexpr int kRouteStaticMaxExperts = 256;
-constexpr int kRouteStaticInts = (kRouteStaticMaxPairs / b200::ROUTE_CHUNK) * kRouteStaticMaxExperts + kRouteStaticMaxExperts + 2;
+constexpr int kRouteStaticInts = (kRouteStaticMaxPairs / b200::ROUTE_CHUNK) * kRouteStaticMaxExperts + kRouteStaticMaxExperts + 3;
 static __device__ __align__(256) int g_route_static[kRouteStaticInts];
 
 // In host code `g_route_static` is only a handle for the symbol, not an address a kernel can use: the device address is
@@ -301,15 +307,16 @@ extern "C" int b200moe_route_static(const int* ids, int P, int E, int Umax, int*
   int* expert_base = hist + (long long)nchunks * E;
   int* bad = expert_base + E;
   int* num_touched = bad + 1;
+  int* num_routed = bad + 2;
   B200_CUDA_TRY(cudaMemsetAsync(bad, 0, 2 * sizeof(int), st));
   if (nchunks > 0) {
     k_route_hist<<<nchunks, 128, E * sizeof(int), st>>>(ids, P, E, hist, bad);
     B200_LAUNCH_CHECK();
   }
-  k_route_scan<<<1, 1024, 0, st>>>(hist, nchunks, P, E, Umax, experts, offsets, expert_base, num_touched);
+  k_route_scan<<<1, 1024, 0, st>>>(hist, nchunks, P, E, Umax, experts, offsets, expert_base, num_touched, num_routed);
   B200_LAUNCH_CHECK();
   if (nchunks > 0) {
-    k_route_place<<<nchunks, 32, E * sizeof(int), st>>>(ids, P, E, hist, expert_base, pairs);
+    k_route_place<<<nchunks, 32, E * sizeof(int), st>>>(ids, P, E, hist, expert_base, num_routed, pairs);
     B200_LAUNCH_CHECK();
   }
   return B200MOE_OK;

@@ -6,7 +6,7 @@ of a row (activations) or per 128x128 block (weights), the quantisers that make 
     y = matmul_fp8(q, s, w, w_scale)                     # w [N, K], w_scale [ceil(N / 128), ceil(K / 128)] -> [M, N]
 
     experts, offsets, pairs = route_tables(ids, E)       # the experts of a layer, one run of rows each
-    q, s = quantize_fp8(x, src_row=pairs // top_k)
+    q, s = quantize_fp8(x, src_row=pairs // top_k)       # (empty slots are -1 in pairs, and zero rows here)
     y = matmul_fp8_experts(q, s, w, w_scale, experts, offsets)      # row i is what pair pairs[i] gets
 
 Nothing here synchronises or keeps state between calls; every call but matmul_fp8_status can be captured into a CUDA graph and runs on the tensors' device, on its current stream."""

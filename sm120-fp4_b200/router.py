@@ -24,7 +24,8 @@ def _workspace(device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
 
 
 def route(ids: torch.Tensor, num_experts: int, experts: torch.Tensor, offsets: torch.Tensor, pairs: torch.Tensor) -> None:
-    """Fills the caller's tables on the current stream. The scratch memory of the counting sort is kept per (device, stream)
+    """Fills the caller's tables on the current stream. An id below 0 (or from num_experts on) is an empty slot, whose pair is in no run: `pairs` is -1 behind the last
+    one. The scratch memory of the counting sort is kept per (device, stream)
     and only grows, so a call of a size seen before allocates nothing, and calls on different streams do not share scratch. A call that is
     captured into a CUDA graph has scratch of its own, in the graph's memory."""
     if ids.dtype != torch.int32 or experts.dtype != torch.int32 or offsets.dtype != torch.int32 or pairs.dtype != torch.int32:
@@ -44,7 +45,7 @@ def route(ids: torch.Tensor, num_experts: int, experts: torch.Tensor, offsets: t
 
 
 def route_tables(ids: torch.Tensor, num_experts: int):
-    """Allocate and fill (experts [min(E, P)], offsets [min(E, P) + 1], pairs [P]) for `ids`."""
+    """Allocate and fill (experts [min(E, P)], offsets [min(E, P) + 1], pairs [P]) for `ids`; behind the last run -1 in experts and in pairs."""
     ids = ids.to(torch.int32).contiguous()
     p = ids.numel()
     umax = min(num_experts, p)

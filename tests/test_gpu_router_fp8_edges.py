@@ -188,3 +188,58 @@ def test_rows_outside_every_run_take_the_time_of_their_bytes():
     left = best_us(lambda: pkg.matmul_fp8_experts(a, sa, w, sw, experts, offsets, out=out))
     zeroed = best_us(lambda: pkg.matmul_fp8_experts(a, sa, w, sw, experts, offsets))
     assert zeroed <= left + 200, f"{left:.0f} us without the zeros, {zeroed:.0f} with them"
+
+
+# ---------------------------------------------------------------------------------------------------- padded batches
+
+@pytest.mark.parametrize("tokens,k,e,static", [(3, 2, 8, False), (40, 4, 16, False), (512, 8, 256, False), (513, 8, 256, False), (700, 8, 300, False), (5000, 4, 60, False), (20000, 8, 128, False),
+                                               (3, 2, 8, True), (513, 8, 256, True), (8192, 8, 256, True)])
+def test_pairs_behind_the_last_run(tokens, k, e, static):
+    """Empty slots and ids that are not there stand in no run; what is behind the last one is -1, not what memory held."""
+    p = tokens * k
+    for empty in (0.0, 0.4, 1.0):
+        g = torch.Generator().manual_seed(tokens)
+        ids = torch.randint(0, e, (p,), generator=g).int()
+        ids[torch.rand(p, generator=g) < empty] = -1
+        if empty == 0.4:
+            ids[1] = e + 3
+        umax = min(e, p)
+        ex, off, pairs = (torch.full((n,), 77, dtype=torch.int32, device="cuda") for n in (umax, umax + 1, p))
+        dev = ids.cuda()
+        if static:
+            L.check(L.lib().b200moe_route_static(L.ptr(dev), p, e, umax, L.ptr(ex), L.ptr(off), L.ptr(pairs), L.stream_ptr()))
+        else:
+            pkg.route(dev, e, ex, off, pairs)
+        used = (ids >= 0) & (ids < e)
+        routed = int(used.sum())
+        order = torch.where(used, ids, torch.tensor(e)).sort(stable=True)[1].int()
+        assert int(off[-1]) == routed and torch.equal(pairs.cpu()[:routed], order[:routed]) and bool((pairs[routed:] == -1).all())
+        if not static:
+            assert torch.equal(pkg.route_tables(dev, e)[2], pairs)
+
+
+def test_tables_with_room_for_fewer_experts_than_are_touched():
+    ids = torch.arange(64, dtype=torch.int32, device="cuda").repeat(100)
+    ids[::3] = -1
+    for p in (600, 6400):
+        ex, off, pairs = (torch.full((n,), 77, dtype=torch.int32, device="cuda") for n in (10, 11, p))
+        pkg.route(ids[:p], 64, ex, off, pairs)
+        routed = int((ids[:p] >= 0).sum())
+        assert ex.tolist() == list(range(10)) and bool((pairs[:routed] >= 0).all()) and bool((pairs[routed:] == -1).all())
+
+
+@pytest.mark.parametrize("t,live,k,inner", [(40, 25, 4, 256), (3000, 1801, 2, 256), (3000, 1801, 8, 1024), (4096, 1, 8, 512)])
+def test_padded_batch_is_the_same_from_call_to_call(t, live, k, inner):
+    """The documented way from ids to codes: rows behind the last run are zeros, codes and scales alike, whatever memory held."""
+    x, logit = randn(t, inner, seed=1).bfloat16(), randn(t, 32, seed=2)
+    logit[live:] = -math.inf
+    ids = pkg.top_k_gate(logit, k)[1]
+    for poison in (0, 5, 1 << 29):
+        dirty = [torch.full((t * k,), poison, dtype=torch.int32, device="cuda") for _ in range(4)]
+        del dirty
+        experts, offsets, pairs = pkg.route_tables(ids, 32)
+        q, s = pkg.quantize_fp8(x, src_row=pairs // k)
+        assert int(offsets[-1]) == live * k
+        assert int(q.view(torch.uint8)[live * k:].max()) == 0 and float(s[live * k:].abs().max()) == 0.0
+        rq, rs = pkg.quantize_fp8(x[(pairs[:live * k] // k).long()])
+        assert same(q[:live * k].contiguous(), rq.contiguous()) and torch.equal(s[:live * k], rs)
