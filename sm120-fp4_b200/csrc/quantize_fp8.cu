@@ -8,13 +8,29 @@
 
 namespace b200 {
 
+// A lane's 16 values, one of eight lanes that share a group of 128: their codes, and the group's scale.
+template <typename T> __device__ __forceinline__ uint4 codes_of_16(const uint4 (&w)[Elem<T>::kSize], float& scale) {
+  constexpr int W = Elem<T>::kSize;      // 16-byte words of 16 values
+  float v[16], m = 0.f;
+#pragma unroll
+  for (int i = 0; i < W; ++i) unpack16<T>(w[i], v + i * (16 / W));
+#pragma unroll
+  for (int i = 0; i < 16; ++i) m = max_nan(m, fabsf(v[i]));
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const Fp8Scale s = fp8_scale(m);
+  scale = s.scale;
+  return make_uint4(cvt_e4m3x4(v[0] * s.factor, v[1] * s.factor, v[2] * s.factor, v[3] * s.factor), cvt_e4m3x4(v[4] * s.factor, v[5] * s.factor, v[6] * s.factor, v[7] * s.factor),
+                    cvt_e4m3x4(v[8] * s.factor, v[9] * s.factor, v[10] * s.factor, v[11] * s.factor),
+                    cvt_e4m3x4(v[12] * s.factor, v[13] * s.factor, v[14] * s.factor, v[15] * s.factor));
+}
 
 // Rows, 16 bytes at a time: K and both row strides are multiples of 16 values, so that a lane's 16 values are whole. Eight lanes share a
 // group of 128; a lane whose values lie beyond K (the last group of a row) takes part in the maximum with zeros.
 template <typename T>
 __global__ void __launch_bounds__(256) k_quantize_fp8_rows(const T* __restrict__ x, long long ldx, int x_rows, const int* __restrict__ src_row, int rows, int K,
                                                            uint8_t* __restrict__ codes, long long ldc, float* __restrict__ scales) {
-  constexpr int W = 16 * Elem<T>::kSize / 16;      // 16-byte words of a lane's values
+  constexpr int W = Elem<T>::kSize;
   const int KB = (K + 127) >> 7;
   const long long units = (long long)rows * KB;
   grid_dependency_wait();
@@ -30,56 +46,84 @@ __global__ void __launch_bounds__(256) k_quantize_fp8_rows(const T* __restrict__
     uint4 w[W];
 #pragma unroll
     for (int i = 0; i < W; ++i) w[i] = have ? *(reinterpret_cast<const uint4*>(x + (long long)src * ldx + c) + i) : make_uint4(0u, 0u, 0u, 0u);
-    float v[16];
-#pragma unroll
-    for (int i = 0; i < W; ++i) unpack16<T>(w[i], v + i * (16 / W));
-    float m = 0.f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) m = max_nan(m, fabsf(v[i]));
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const Fp8Scale s = fp8_scale(m);
+    float scale;
+    const uint4 q = codes_of_16<T>(w, scale);
     if (!in) continue;
-    if (c < K) {
-      uint4 q;
-      q.x = cvt_e4m3x4(v[0] * s.factor, v[1] * s.factor, v[2] * s.factor, v[3] * s.factor);
-      q.y = cvt_e4m3x4(v[4] * s.factor, v[5] * s.factor, v[6] * s.factor, v[7] * s.factor);
-      q.z = cvt_e4m3x4(v[8] * s.factor, v[9] * s.factor, v[10] * s.factor, v[11] * s.factor);
-      q.w = cvt_e4m3x4(v[12] * s.factor, v[13] * s.factor, v[14] * s.factor, v[15] * s.factor);
-      *reinterpret_cast<uint4*>(codes + (long long)row * ldc + c) = q;
-    }
-    if ((threadIdx.x & 7) == 0) scales[(long long)row * KB + g] = gone ? 0.f : s.scale;
+    if (c < K) *reinterpret_cast<uint4*>(codes + (long long)row * ldc + c) = q;
+    if ((threadIdx.x & 7) == 0) scales[(long long)row * KB + g] = gone ? 0.f : scale;
   }
 }
 
-// Rows that are asked for several times (a token's copies for its experts): each source row is read and quantised once and its codes are stored to all of its
+// Rows that are asked for several times (a token's copies for its experts): each source row is read and quantised once and its codes are stored to its
 // destinations, which hang on a list per source row: head i32 [x_rows], next i32 [rows], made by two small kernels. The order of a list is that of the atomics,
 // and does not matter: every destination gets the same bytes. Reading the source once per destination took 47 us for 4096 rows of 2816 eight times over (184 MB out
 // of L2); the destinations' 92 MB are what HBM has to take.
+// A list is walked by one warp for each 512 columns, 77 ns a destination. So that a row which is wanted very often is not left to them, a block of 256 destinations puts
+// kFromBlock of a row on its list at most, counted by a hash of the row; the others read the row themselves, spread over the block's warps. A list then has one in
+// 32 of all destinations at most (us, bounded / any length: 32768 of 2816 bf16, half of them one row, 110 / 1276; all of them, 171 / 3010; evenly spread 23.8 / 23.7).
 __global__ void __launch_bounds__(256) k_no_heads(int* __restrict__ head, int x_rows) {
   grid_dependency_wait();
   grid_launch_dependents();
   const int i = blockIdx.x * 256 + threadIdx.x;
   if (i < x_rows) head[i] = -1;
 }
-__global__ void __launch_bounds__(256) k_link_rows(const int* __restrict__ src_row, int rows, int x_rows, int K, int* __restrict__ head, int* __restrict__ next,
-                                                   uint8_t* __restrict__ codes, long long ldc, float* __restrict__ scales) {
-  const int r = blockIdx.x * 256 + threadIdx.x, lane = threadIdx.x & 31, KB = (K + 127) >> 7;
+constexpr int kLinked = 256, kFromBlock = 8, kLinkThreads = 512;      // destinations of a block
+template <typename T>
+__global__ void __launch_bounds__(kLinkThreads) k_link_rows(const T* __restrict__ x, long long ldx, int x_rows, const int* __restrict__ src_row, int rows, int K,
+                                                            int* __restrict__ head, int* __restrict__ next, uint8_t* __restrict__ codes, long long ldc,
+                                                            float* __restrict__ scales) {
+  constexpr int W = Elem<T>::kSize, kAhead = 2, kHash = 1024;
+  __shared__ int seen[kHash], source[kLinked], left[kLinked], left_n;
+  const int tid = threadIdx.x, lane = tid & 31, r0 = blockIdx.x * kLinked, r = r0 + tid, KB = (K + 127) >> 7;
+  for (int i = tid; i < kHash; i += kLinkThreads) seen[i] = 0;
+  if (tid == 0) left_n = 0;
+  __syncthreads();
   grid_dependency_wait();
-  grid_launch_dependents();
-  const int s = r < rows ? src_row[r] : 0;
-  const bool gone = r < rows && (s < 0 || s >= x_rows);
-  if (r < rows && !gone) next[r] = atomicExch(head + s, r);
-  for (unsigned todo = __ballot_sync(0xffffffffu, gone); todo; todo &= todo - 1) {      // empty rows: zeros, by the whole warp
-    const long long e = r - lane + __ffs(todo) - 1;
-    for (int i = lane; i < K / 16; i += 32) *reinterpret_cast<uint4*>(codes + e * ldc + i * 16) = make_uint4(0u, 0u, 0u, 0u);
-    for (int i = lane; i < KB; i += 32) scales[e * KB + i] = 0.f;
+  if (tid < kLinked && r < rows) {
+    int s = src_row[r];
+    if (s >= x_rows) s = -1;      // an empty row: zero codes and scales
+    if (s >= 0 && atomicAdd(&seen[(uint32_t)s * 2654435769u >> 22], 1) < kFromBlock) {
+      next[r] = atomicExch(head + s, r);
+    } else {
+      source[tid] = s;
+      left[atomicAdd(&left_n, 1)] = tid;
+    }
+  }
+  __syncthreads();
+  grid_launch_dependents();      // (from the start on, the next kernel's blocks crowd onto the SMs that have none of these: 512 rows 64 times over 31 us instead of 25)
+  for (int i = tid >> 5; i < left_n; i += kLinkThreads / 32) {      // a warp each
+    const int at = left[i], from = source[at];
+    uint8_t* to = codes + (long long)(r0 + at) * ldc;
+    float* s = scales + (long long)(r0 + at) * KB;
+    if (from < 0) {
+      for (int j = lane; j < K / 16; j += 32) *reinterpret_cast<uint4*>(to + j * 16) = make_uint4(0u, 0u, 0u, 0u);
+      for (int j = lane; j < KB; j += 32) s[j] = 0.f;
+      continue;
+    }
+    const T* row = x + (long long)from * ldx;
+    for (int c0 = 0; c0 < K; c0 += 512 * kAhead) {
+      uint4 w[kAhead][W];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const int c = c0 + j * 512 + lane * 16;
+#pragma unroll
+        for (int h = 0; h < W; ++h) w[j][h] = c < K ? *(reinterpret_cast<const uint4*>(row + c) + h) : make_uint4(0u, 0u, 0u, 0u);
+      }
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const int c = c0 + j * 512 + lane * 16;
+        float scale;
+        const uint4 q = codes_of_16<T>(w[j], scale);
+        if (c < K) *reinterpret_cast<uint4*>(to + c) = q;
+        if ((lane & 7) == 0 && c < K) s[c >> 7] = scale;
+      }
+    }
   }
 }
 template <typename T>
 __global__ void __launch_bounds__(256) k_quantize_fp8_copies(const T* __restrict__ x, long long ldx, int x_rows, int K, const int* __restrict__ head, const int* __restrict__ next,
                                                              uint8_t* __restrict__ codes, long long ldc, float* __restrict__ scales) {
-  constexpr int W = 16 * Elem<T>::kSize / 16;
+  constexpr int W = Elem<T>::kSize;
   const int KB = (K + 127) >> 7, quads = (KB + 3) >> 2;      // a warp takes four groups of a row
   const long long u = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int row = (int)(u / quads), g = (int)(u - (long long)row * quads) * 4 + (threadIdx.x >> 3 & 3), c = g * 128 + (threadIdx.x & 7) * 16;
@@ -90,23 +134,12 @@ __global__ void __launch_bounds__(256) k_quantize_fp8_copies(const T* __restrict
 #pragma unroll
   for (int i = 0; i < W; ++i) w[i] = c < K ? *(reinterpret_cast<const uint4*>(x + (long long)row * ldx + c) + i) : make_uint4(0u, 0u, 0u, 0u);
   int r = head[row];
-  float v[16], m = 0.f;
-#pragma unroll
-  for (int i = 0; i < W; ++i) unpack16<T>(w[i], v + i * (16 / W));
-#pragma unroll
-  for (int i = 0; i < 16; ++i) m = max_nan(m, fabsf(v[i]));
-#pragma unroll
-  for (int o = 1; o < 8; o <<= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-  const Fp8Scale s = fp8_scale(m);
-  uint4 q;
-  q.x = cvt_e4m3x4(v[0] * s.factor, v[1] * s.factor, v[2] * s.factor, v[3] * s.factor);
-  q.y = cvt_e4m3x4(v[4] * s.factor, v[5] * s.factor, v[6] * s.factor, v[7] * s.factor);
-  q.z = cvt_e4m3x4(v[8] * s.factor, v[9] * s.factor, v[10] * s.factor, v[11] * s.factor);
-  q.w = cvt_e4m3x4(v[12] * s.factor, v[13] * s.factor, v[14] * s.factor, v[15] * s.factor);
+  float scale;
+  const uint4 q = codes_of_16<T>(w, scale);
   while (r >= 0) {
     const int after = next[r];
     if (c < K) *reinterpret_cast<uint4*>(codes + (long long)r * ldc + c) = q;
-    if ((threadIdx.x & 7) == 0 && g < KB) scales[(long long)r * KB + g] = s.scale;
+    if ((threadIdx.x & 7) == 0 && g < KB) scales[(long long)r * KB + g] = scale;
     r = after;
   }
 }
@@ -245,8 +278,8 @@ static int quantize_fp8_rows(const void* x, long long ldx, int x_rows, const int
     int *head = lists, *next = lists + x_rows;
     void* a0[] = {&head, &x_rows};
     if (int rc = launch_kernel((const void*)k_no_heads, (x_rows + 255) / 256, 256, 0, true, a0, st)) return rc;
-    void* a1[] = {&src_row, &rows, &x_rows, &K, &head, &next, &ct, &ldc, &scales};
-    if (int rc = launch_kernel((const void*)k_link_rows, (rows + 255) / 256, 256, 0, true, a1, st)) return rc;
+    void* a1[] = {&xt, &ldx, &x_rows, &src_row, &rows, &K, &head, &next, &ct, &ldc, &scales};
+    if (int rc = launch_kernel((const void*)k_link_rows<T>, (rows + kLinked - 1) / kLinked, kLinkThreads, 0, true, a1, st)) return rc;
     const long long warps = (long long)x_rows * ((K + 511) / 512);
     if (warps > 8ll * 0x7fffffff) return B200MOE_ERR_LIMIT;
     void* a2[] = {&xt, &ldx, &x_rows, &K, &head, &next, &ct, &ldc, &scales};

@@ -243,3 +243,39 @@ def test_padded_batch_is_the_same_from_call_to_call(t, live, k, inner):
         assert int(q.view(torch.uint8)[live * k:].max()) == 0 and float(s[live * k:].abs().max()) == 0.0
         rq, rs = pkg.quantize_fp8(x[(pairs[:live * k] // k).long()])
         assert same(q[:live * k].contiguous(), rq.contiguous()) and torch.equal(s[:live * k], rs)
+
+
+# ---------------------------------------------------------------------------------------------------- rows that are asked for very often
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_rows_that_are_asked_for_very_often(dtype):
+    """One row for half of the destinations, a few rows for all of them, counts that differ, and one row in all."""
+    x = randn(4096, 1056, seed=1).to(dtype)
+    q, s = pkg.quantize_fp8(x)
+    g = torch.Generator().manual_seed(3)
+    src = torch.arange(32768) // 8
+    half = src.clone()
+    half[16384:] = 11
+    for src in (half, half.flip(0), torch.full((32768,), 4095), src % 3, torch.randint(0, 4096, (32768,), generator=g), torch.randint(-500, 5000, (30001,), generator=g),
+                (torch.rand(32768, generator=g) ** 4 * 4096).long(), torch.arange(32768) % 4096):
+        src = src.int().cuda()
+        inside = (src >= 0) & (src < 4096)
+        at = src.clamp(0, 4095).long()
+        gq, gs = pkg.quantize_fp8(x, src_row=src)
+        want = torch.where(inside[:, None], q.view(torch.uint8)[at], torch.zeros((), dtype=torch.uint8, device="cuda"))
+        assert torch.equal(gq.view(torch.uint8), want) and torch.equal(gs, torch.where(inside[:, None], s[at], torch.zeros((), device="cuda")))
+    one = x[:1]
+    gq, gs = pkg.quantize_fp8(one, src_row=torch.zeros(20000, dtype=torch.int32, device="cuda"))
+    assert torch.equal(gq.view(torch.uint8), q[:1].view(torch.uint8).expand(20000, -1)) and torch.equal(gs, s[:1].expand(20000, -1))
+
+
+def test_a_row_that_is_asked_for_very_often_takes_the_time_of_its_bytes():
+    """16384 destinations of one row are 46 MB of codes, 7 us at the rate of memory; one after the other, 80 ns each, they would take more than a millisecond."""
+    x = randn(4096, 2816, seed=1).bfloat16()
+    even = (torch.arange(32768, device="cuda") // 8).int()
+    skewed = even.clone()
+    skewed[16384:] = 11
+    usual = best_us(lambda: pkg.quantize_fp8(x, src_row=even))
+    often = best_us(lambda: pkg.quantize_fp8(x, src_row=skewed))
+    one = best_us(lambda: pkg.quantize_fp8(x[:2], src_row=skewed.clamp(max=1)))
+    assert often <= usual + 400 and one <= usual + 400, f"{usual:.0f} us evenly, {often:.0f} with one row for half of them, {one:.0f} with two rows in all"
