@@ -176,6 +176,13 @@ def stored(t: torch.Tensor) -> torch.Tensor:
     return t.resolve_neg()
 
 
+def no_gradient(what: str, *tensors) -> None:
+    """Refuses tensors whose derivatives are asked for, for calls that have none: outputs without a history would read as a derivative of zero."""
+    for t in tensors:
+        if t is not None and (t.requires_grad and torch.is_grad_enabled() or torch.autograd.forward_ad.unpack_dual(t).tangent is not None):
+            raise RuntimeError(f"{what} has no derivative: detach its inputs, or call it under torch.no_grad()")
+
+
 def one_device(what: str, *tensors) -> torch.device:
     """The device that all of them are on: a GPU."""
     device = tensors[0].device

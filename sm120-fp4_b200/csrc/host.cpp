@@ -153,6 +153,8 @@ bool plain_logits(const at::Tensor& x) {
          (x.stride(0) >= x.size(1) || x.size(0) == 1);
 }
 long long row_stride(const at::Tensor& x) { return std::max(x.stride(0), x.size(1)); }
+// (the FP8 calls have no derivatives: inputs that ask for one are refused on the general path)
+bool no_gradient(const at::Tensor& t) { return !(t.requires_grad() && at::GradMode::is_enabled()) && !t._fw_grad(0).defined(); }
 bool vector_of(const at::Tensor& t, at::ScalarType type) { return here(t) && t.dim() == 1 && t.scalar_type() == type && t.is_contiguous(); }
 void checked(int rc, const char* what) {      // (the message as one string: no streams)
   if (rc) TORCH_CHECK(false, std::string(what) + ": " + ops.error_string(rc) + " (" + std::to_string(rc) + ")");
@@ -343,7 +345,7 @@ PyObject* py_quantize_fp8(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (n != 2 || !tensors(args, args[1] == Py_None ? 1 : 2)) Py_RETURN_NONE;
   const at::Tensor x = THPVariable_Unpack(args[0]), src = args[1] == Py_None ? at::Tensor() : THPVariable_Unpack(args[1]);
-  if (!here(x) || x.dim() != 2 || dtype_code(x.scalar_type()) < 0 || x.size(0) < 1 || x.size(1) < 1 || x.size(0) > kMaxSize || x.size(1) > kMaxSize || x.stride(1) != 1 ||
+  if (!here(x) || !no_gradient(x) || x.dim() != 2 || dtype_code(x.scalar_type()) < 0 || x.size(0) < 1 || x.size(1) < 1 || x.size(0) > kMaxSize || x.size(1) > kMaxSize || x.stride(1) != 1 ||
       (x.stride(0) < x.size(1) && x.size(0) > 1) || (src.defined() && (!vector_of(src, at::kInt) || src.size(0) > kMaxSize)))
     Py_RETURN_NONE;
   const int64_t k = x.size(1), rows = src.defined() ? src.size(0) : x.size(0), ld = (k + 15) & ~15ll;
@@ -366,7 +368,7 @@ PyObject* py_quantize_fp8_weight(PyObject*, PyObject* const* args, Py_ssize_t n)
   HANDLE_TH_ERRORS
   if (n != 1 || !tensors(args, 1)) Py_RETURN_NONE;
   const at::Tensor w = THPVariable_Unpack(args[0]);
-  if (!here(w) || (w.dim() != 2 && w.dim() != 3) || dtype_code(w.scalar_type()) < 0 || w.numel() < 1 || !w.is_contiguous() || w.size(-1) > kMaxSize || w.size(-2) > 65535 * 128 ||
+  if (!here(w) || !no_gradient(w) || (w.dim() != 2 && w.dim() != 3) || dtype_code(w.scalar_type()) < 0 || w.numel() < 1 || !w.is_contiguous() || w.size(-1) > kMaxSize || w.size(-2) > 65535 * 128 ||
       w.size(0) > kMaxSize)
     Py_RETURN_NONE;
   const int64_t e = w.dim() == 3 ? w.size(0) : 1, rows = w.size(-2), k = w.size(-1), ld = (k + 15) & ~15ll, nb = (rows + 127) / 128, kb = (k + 127) / 128;
@@ -385,11 +387,11 @@ PyObject* py_quantize_fp8_weight(PyObject*, PyObject* const* args, Py_ssize_t n)
 
 // bytes between rows of codes that the products take as they are, 0 for others
 int64_t codes_stride(const at::Tensor& t) {
-  if (!here(t) || t.scalar_type() != at::kFloat8_e4m3fn) return 0;
+  if (!here(t) || !no_gradient(t) || t.scalar_type() != at::kFloat8_e4m3fn) return 0;
   const int64_t k = t.size(-1), ld = t.size(-2) > 1 ? t.stride(-2) : (k + 15) & ~15ll;
   return k >= 1 && k <= kMaxSize && (t.stride(-1) == 1 || k == 1) && ld >= k && ld % 16 == 0 && (uintptr_t)t.data_ptr() % 16 == 0 ? ld : 0;
 }
-bool scales_of(const at::Tensor& s, at::IntArrayRef size) { return here(s) && s.scalar_type() == at::kFloat && s.sizes() == size && s.is_contiguous(); }
+bool scales_of(const at::Tensor& s, at::IntArrayRef size) { return here(s) && no_gradient(s) && s.scalar_type() == at::kFloat && s.sizes() == size && s.is_contiguous(); }
 
 // matmul_fp8(a, a_scale, w, w_scale, dtype), matmul_fp8_experts(a, a_scale, w, w_scale, experts, offsets, dtype): a new output
 PyObject* matmul(PyObject* const* args, bool experts) {

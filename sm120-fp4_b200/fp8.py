@@ -9,6 +9,7 @@ of a row (activations) or per 128x128 block (weights), the quantisers that make 
     q, s = quantize_fp8(x, src_row=pairs // top_k)       # (empty slots are -1 in pairs, and zero rows here)
     y = matmul_fp8_experts(q, s, w, w_scale, experts, offsets)      # row i is what pair pairs[i] gets
 
+These calls have no derivatives: an input that requires a gradient, with gradients enabled, or that carries a tangent is refused (RuntimeError).
 Nothing here synchronises or keeps state between calls; every call but matmul_fp8_status can be captured into a CUDA graph and runs on the tensors' device, on its current stream."""
 from __future__ import annotations
 
@@ -47,6 +48,7 @@ def quantize_fp8(x: torch.Tensor, src_row: torch.Tensor | None = None):
     if x.dtype not in _lib.DTYPES:
         raise TypeError(f"quantize_fp8 takes bf16, fp16 or fp32, not {x.dtype}")
     _sizes("quantize_fp8", x, src_row)
+    _lib.no_gradient("quantize_fp8", x)
     device = _lib.one_device("quantize_fp8", x)
     m, k = x.shape
     x = _lib.stored(x)
@@ -81,6 +83,7 @@ def quantize_fp8_weight(w: torch.Tensor):
     if w.dtype not in _lib.DTYPES:
         raise TypeError(f"quantize_fp8_weight takes bf16, fp16 or fp32, not {w.dtype}")
     _sizes("quantize_fp8_weight", w)
+    _lib.no_gradient("quantize_fp8_weight", w)
     device = _lib.one_device("quantize_fp8_weight", w)
     w = _lib.stored(w).contiguous()
     n, k = w.shape[-2:]
@@ -138,6 +141,7 @@ def matmul_fp8(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale:
     if a.dim() != 2 or w.dim() != 2 or a.shape[1] != w.shape[1] or a.shape[1] < 1:
         raise ValueError(f"matmul_fp8: expected [M, K] and [N, K] with K >= 1, got {tuple(a.shape)} and {tuple(w.shape)}")
     _sizes("matmul_fp8", a, w)
+    _lib.no_gradient("matmul_fp8", a, a_scale, w, w_scale, out)
     a, w = _lib.stored(a), _lib.stored(w)
     lda, ldw = _row_stride(a, "matmul_fp8", "a"), _row_stride(w, "matmul_fp8", "w")
     (m, k), n = a.shape, w.shape[0]
@@ -163,6 +167,7 @@ def matmul_fp8_experts(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, 
     if a.dim() != 2 or w.dim() != 3 or a.shape[1] != w.shape[2] or a.shape[1] < 1 or w.shape[0] < 1:
         raise ValueError(f"{what}: expected [P, K] and [E, N, K] with K >= 1, got {tuple(a.shape)} and {tuple(w.shape)}")
     _sizes(what, a, w)
+    _lib.no_gradient(what, a, a_scale, w, w_scale, out)
     a, w = _lib.stored(a), _lib.stored(w)
     lda, ldw = _row_stride(a, what, "a"), _row_stride(w, what, "w")
     (m, k), (e, n, _) = a.shape, w.shape

@@ -47,6 +47,27 @@ def test_forward_mode_is_refused(path):
             torch.func.jvp(call, (x,), (torch.ones_like(x),))
 
 
+def test_fp8_calls_refuse_inputs_that_ask_for_a_derivative(path):
+    x, w = randn(8, 256, seed=1), randn(32, 256, seed=2)
+    a, sa = pkg.quantize_fp8(x)
+    wq, sw = pkg.quantize_fp8_weight(w)
+    ask = lambda t: t.clone().requires_grad_(True)
+    refused = [lambda: pkg.quantize_fp8(ask(x)), lambda: pkg.quantize_fp8(x * ask(x)), lambda: pkg.quantize_fp8_weight(ask(w)), lambda: pkg.quantize_fp8_weight(torch.nn.Parameter(w)),
+               lambda: pkg.matmul_fp8(a, ask(sa), wq, sw), lambda: pkg.matmul_fp8(a, sa, wq, ask(sw))]
+    for call in refused:
+        with pytest.raises(RuntimeError, match="no derivative"):
+            call()
+        with torch.no_grad():
+            out = call()
+        assert not any(t.requires_grad for t in (out if type(out) is tuple else (out,)))
+    with fwd.dual_level():
+        for call in (lambda: pkg.quantize_fp8(fwd.make_dual(x, torch.ones_like(x))), lambda: pkg.matmul_fp8(a, fwd.make_dual(sa, torch.ones_like(sa)), wq, sw)):
+            with pytest.raises(RuntimeError, match="no derivative"):
+                call()
+    with torch.inference_mode():
+        assert same(pkg.quantize_fp8(ask(x))[0], a)
+
+
 def test_an_error_in_a_gradient_reaches_the_caller():
     """The library says no inside a backward pass, on a thread of the autograd engine: an exception like any other."""
     h, host, no = L.lib(), L.host(), C.CFUNCTYPE(C.c_int, *L.SIGNATURES["b200moe_gate_backward"][1])(lambda *args: L.ERR_ARG)

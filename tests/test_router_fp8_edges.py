@@ -25,3 +25,24 @@ def test_the_host_extension_has_no_cxx_library_of_its_own():
     assert host is not L.NO_HOST
     with open(host.__file__, "rb") as f:
         assert b"St7codecvtIDsc" not in f.read()      # (a part of the library that nothing here names)
+
+
+def test_fp8_calls_refuse_inputs_that_ask_for_a_derivative():
+    """Outputs without a history would read as a derivative of zero."""
+    codes = lambda *shape: torch.zeros(*shape, dtype=torch.uint8).view(torch.float8_e4m3fn)
+    a, sa, w, sw, we, swe = codes(4, 256), torch.ones(4, 2), codes(32, 256), torch.ones(1, 2), codes(3, 32, 256), torch.ones(3, 1, 2)
+    experts, offsets = torch.zeros(2, dtype=torch.int32), torch.zeros(3, dtype=torch.int32)
+    calls = [(pkg.quantize_fp8, [torch.zeros(4, 8)], [0]), (pkg.quantize_fp8_weight, [torch.zeros(4, 8)], [0]), (pkg.quantize_fp8_weight, [torch.zeros(2, 4, 8)], [0]),
+             (pkg.matmul_fp8, [a, sa, w, sw], [1, 3]), (pkg.matmul_fp8_experts, [a, sa, we, swe, experts, offsets], [1, 3])]
+    for call, args, floats in calls:
+        for i in floats:
+            asked = [t.clone().requires_grad_(True) if j == i else t for j, t in enumerate(args)]
+            with pytest.raises(RuntimeError, match="no derivative"):
+                call(*asked)
+            with torch.no_grad(), pytest.raises(RuntimeError, match="GPU"):      # gets as far as ever
+                call(*asked)
+            with fwd.dual_level(), pytest.raises(RuntimeError, match="no derivative"):
+                call(*[fwd.make_dual(t, torch.ones_like(t)) if j == i else t for j, t in enumerate(args)])
+    for call, args in ((pkg.matmul_fp8, (a, sa, w, sw)), (pkg.matmul_fp8_experts, (a, sa, we, swe, experts, offsets))):
+        with pytest.raises(RuntimeError, match="no derivative"):
+            call(*args, out=torch.zeros(4, 32, requires_grad=True))
