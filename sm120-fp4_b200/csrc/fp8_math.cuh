@@ -1,4 +1,4 @@
-// Shared pieces of the FP8 and router operators: element types, 16-byte loads as floats, E4M3 conversion.
+// Shared pieces of the FP8 and router operators: element types, 16-byte loads as floats, maxima that keep NaN, E4M3 conversion.
 #pragma once
 #include "ptx.cuh"
 
@@ -52,6 +52,12 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   float d;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
   return d;
+}
+// the largest of a warp's values, NaN where a lane has one; all lanes have to be here, so it stays where it is called
+__device__ __forceinline__ float warp_max(float v) {
+  float m;
+  asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+  return m;
 }
 // four floats -> four E4M3 bytes, element order kept; to nearest, ties to even, saturating at 448, NaN kept
 __device__ __forceinline__ uint32_t cvt_e4m3x4(float a, float b, float c, float d) {

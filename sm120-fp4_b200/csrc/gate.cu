@@ -66,11 +66,6 @@ __device__ __forceinline__ float warp_sum(float v) {
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-__device__ __forceinline__ float warp_max(float v) {      // NaN where a lane has one
-  float m;
-  asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
-  return m;
-}
 // Softmax numerator exp(x - m) as 2^((x - m) log2(e)): the difference, the product and log2(e) are off by 2^-24, 2^-24 and 2^-26 of |x - m|, relative in the
 // result, ex2 by 2^-22. (x log2(e) - m log2(e) in one fma has one rounding less, and overflows where logits are near their type's largest value.)
 constexpr float kLog2e = 1.4426950408889634f;

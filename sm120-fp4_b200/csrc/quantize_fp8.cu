@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(256) k_quantize_fp8_rows_any(const T* __restri
       float m = 0.f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) m = max_nan(m, fabsf(v[j][i]));
-      asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(m));
+      m = warp_max(m);
       const Fp8Scale s = fp8_scale(m);
       const uint32_t q = cvt_e4m3x4(v[j][0] * s.factor, v[j][1] * s.factor, v[j][2] * s.factor, v[j][3] * s.factor);
       uint8_t* o = codes + (long long)row * ldc + c;

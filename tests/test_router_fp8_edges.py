@@ -1,4 +1,7 @@
 """Corners of the router and FP8 operators that show without a GPU: what is refused, and before anything else."""
+import re
+from pathlib import Path
+
 import pytest
 import torch
 
@@ -46,3 +49,11 @@ def test_fp8_calls_refuse_inputs_that_ask_for_a_derivative():
     for call, args in ((pkg.matmul_fp8, (a, sa, w, sw)), (pkg.matmul_fp8_experts, (a, sa, we, swe, experts, offsets))):
         with pytest.raises(RuntimeError, match="no derivative"):
             call(*args, out=torch.zeros(4, 32, requires_grad=True))
+
+
+def test_instructions_of_a_whole_warp_stay_where_they_are_called():
+    """An asm statement that is not volatile may be moved into a branch that uses its result, where not all lanes are."""
+    csrc = Path(pkg.__path__[0]) / "csrc"
+    for f in sorted(csrc.glob("*.cu*")):
+        for statement in re.findall(r"\basm\s*\([^;]*", f.read_text()):      # (up to the first semicolon: the instruction)
+            assert not re.search(r"\b(redux|shfl|vote|match|bar|barrier|elect)\.", statement), f"{f.name}: {statement}"
