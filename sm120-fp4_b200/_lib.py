@@ -16,7 +16,15 @@ LIB_PATH = Path(os.environ["B200MOE_LIB"]) if os.environ.get("B200MOE_LIB") else
 _lib = None
 _host = None
 ONE_CLUSTER = 8192 * 16   # values of one matrix up to which the quantiser keeps them in registers and takes no workspace
-NO_HOST = SimpleNamespace(**{name: lambda *args: None for name in ("quantize_own_scale", "quantize_128x4", "top_k_gate", "balance_loss", "quantize_fp8", "quantize_fp8_weight", "matmul_fp8", "matmul_fp8_experts")})
+
+
+def _cannot_tell(x: torch.Tensor, what: str) -> None:
+    raise RuntimeError(f"{what}: without the host extension it cannot be seen whether a graph of the same leaf is still alive, beside which a capture that takes gradients ends "
+                       f"the process; build it with `python {_PKG / 'build.py'}`, or capture with logits that are no leaf")
+
+
+NO_HOST = SimpleNamespace(check_capture=_cannot_tell, **{name: lambda *args: None for name in (
+    "quantize_own_scale", "quantize_128x4", "top_k_gate", "balance_loss", "quantize_fp8", "quantize_fp8_weight", "matmul_fp8", "matmul_fp8_experts")})
 
 ERR_ARG, ERR_SHAPE, ERR_CUDA, ERR_DEVICE, ERR_TIMEOUT, ERR_WORKSPACE, ERR_LIMIT, ERR_RANGE, ERR_ORDER = -1, -2, -3, -4, -5, -6, -7, -8, -9
 

@@ -180,8 +180,8 @@ void check_capture(const at::Tensor& x, const char* what) {
   const auto node = torch::autograd::impl::try_get_grad_accumulator(x);
   if (!node) return;
   const auto made_on = node->stream();
-  TORCH_CHECK(!made_on || *made_on == c10::cuda::getCurrentCUDAStream().unwrap(), what,
-              ": a graph of the same leaf that was made on another stream is still alive; drop its outputs before a capture that takes gradients");
+  TORCH_CHECK(!made_on || *made_on == c10::cuda::getCurrentCUDAStream().unwrap(),
+              std::string(what) + ": a graph of the same leaf that was made on another stream is still alive; drop its outputs before a capture that takes gradients");
 }
 
 using torch::autograd::SavedVariable;
@@ -318,6 +318,19 @@ PyObject* py_top_k_gate(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// check_capture(logits, name of the call), for calls that take the general path
+PyObject* py_check_capture(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const char* what = n == 2 && THPVariable_Check(args[0]) && PyUnicode_Check(args[1]) ? PyUnicode_AsUTF8(args[1]) : nullptr;
+  if (!what) {
+    if (!PyErr_Occurred()) PyErr_SetString(PyExc_TypeError, "check_capture takes a tensor and a name");
+    return nullptr;
+  }
+  check_capture(THPVariable_Unpack(args[0]), what);
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
 // balance_loss(logits, ids)
 PyObject* py_balance_loss(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -440,6 +453,7 @@ PyMethodDef methods[] = {{"bind", (PyCFunction)(void (*)(void))py_bind, METH_FAS
                          {"quantize_own_scale", (PyCFunction)(void (*)(void))py_quantize_own_scale, METH_FASTCALL, nullptr},
                          {"quantize_128x4", (PyCFunction)(void (*)(void))py_quantize_128x4, METH_FASTCALL, nullptr},
                          {"bind_ops", (PyCFunction)(void (*)(void))py_bind_ops, METH_FASTCALL, nullptr},
+                         {"check_capture", (PyCFunction)(void (*)(void))py_check_capture, METH_FASTCALL, nullptr},
                          {"top_k_gate", (PyCFunction)(void (*)(void))py_top_k_gate, METH_FASTCALL, nullptr},
                          {"balance_loss", (PyCFunction)(void (*)(void))py_balance_loss, METH_FASTCALL, nullptr},
                          {"quantize_fp8", (PyCFunction)(void (*)(void))py_quantize_fp8, METH_FASTCALL, nullptr},

@@ -3,8 +3,8 @@ keeps experts evenly used, with the number of pairs of each. Both have gradients
 torch (softmax, top-k, renormalise: sm120fp4/kernels/moe_layer.py:195-200).
 
 Nothing here synchronises or keeps state between calls: forward and backward can be captured into a CUDA graph. A capture of a backward pass wants, as with
-every autograd function, that no graph of the same leaves that was made on another stream is alive: logits that are such a leaf are refused (RuntimeError), where the host
-extension takes the call; for leaves further back it is the caller's to see to."""
+every autograd function, that no graph of the same leaves that was made on another stream is alive: logits that are such a leaf are refused (RuntimeError), all that are
+a leaf where the host extension, which can tell, is not there; for leaves further back it is the caller's to see to."""
 from __future__ import annotations
 
 import torch
@@ -28,6 +28,16 @@ def _logits(logits: torch.Tensor, what: str) -> torch.Tensor:
     if logits.stride(1) != 1 and logits.shape[1] > 1 or logits.stride(0) < logits.shape[1] and logits.shape[0] > 1:
         return logits.contiguous()
     return logits
+
+
+def _check_capture(logits: torch.Tensor, what: str) -> None:
+    """A leaf's gradient is handed over on the stream on which its accumulator was made. Where an eager graph keeps that alive, a backward pass that is being captured on
+    another stream ends the process: refused while it still can be."""
+    if not (logits.requires_grad and logits.is_leaf and torch.is_grad_enabled()):
+        return
+    with torch.cuda.device(logits.device):
+        if torch.cuda.is_current_stream_capturing():
+            (_lib._host or _lib.host()).check_capture(logits, what)
 
 
 def _gate(logits: torch.Tensor, top_k: int, renormalize: bool):
@@ -76,9 +86,10 @@ def top_k_gate(logits: torch.Tensor, top_k: int, renormalize: bool = True):
     if out is not None:
         return out if type(out) is tuple else _lib.check(out, "top_k_gate")
     top_k = int(top_k)
-    logits = _logits(logits, "top_k_gate")
+    leaf, logits = logits, _logits(logits, "top_k_gate")
     if not 1 <= top_k <= min(MAX_TOP_K, logits.shape[1]):
         raise ValueError(f"top_k_gate takes 1 to {min(MAX_TOP_K, logits.shape[1])} of {logits.shape[1]} experts, not {top_k}")
+    _check_capture(leaf, "top_k_gate")
     if logits.requires_grad and torch.is_grad_enabled():
         return _Gate.apply(logits, top_k, bool(renormalize))
     return _gate(logits, top_k, bool(renormalize))
@@ -123,13 +134,14 @@ def balance_loss(logits: torch.Tensor, ids: torch.Tensor):
     out = (_lib._host or _lib.host()).balance_loss(logits, ids)      # (as in top_k_gate)
     if out is not None:
         return out if type(out) is tuple else _lib.check(out, "balance_loss")
-    logits = _logits(logits, "balance_loss")
+    leaf, logits = logits, _logits(logits, "balance_loss")
     if ids.dtype != torch.int32:
         raise TypeError(f"balance_loss takes int32 ids, not {ids.dtype}")
     if ids.dim() != 2 or ids.shape[0] != logits.shape[0] or not 1 <= ids.shape[1] <= 32:
         raise ValueError(f"balance_loss: expected ids [{logits.shape[0]}, 1 to 32], got {tuple(ids.shape)}")
     _lib.one_device("balance_loss", logits, ids)
     ids = _lib.stored(ids).contiguous()
+    _check_capture(leaf, "balance_loss")
     if logits.requires_grad and torch.is_grad_enabled():
         return _Balance.apply(logits, ids)
     return _balance(logits, ids)[:2]

@@ -85,6 +85,27 @@ def test_an_error_in_a_gradient_reaches_the_caller():
     assert x.grad is not None
 
 
+def test_capture_beside_a_live_graph_is_refused_on_either_path(path):
+    """Logits that the native side does not take as they are (here a matrix stored by columns) are looked at all the same."""
+    x = randn(16, 20, seed=5).t().requires_grad_(True)
+    assert x.is_leaf and x.stride(1) != 1
+    ids = pkg.top_k_gate(x.detach(), 2)[1]
+    alive = pkg.balance_loss(x, ids)[0]
+    torch.cuda.synchronize()
+    why = "still alive" if path == "native" else "without the host extension"
+    for call in (lambda: pkg.top_k_gate(x, 2), lambda: pkg.balance_loss(x, ids)):
+        with pytest.raises(RuntimeError, match=why):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call()
+    del alive
+    if path == "native":
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            g, = torch.autograd.grad(pkg.balance_loss(x, ids)[0], x)
+        graph.replay()
+        assert torch.equal(g, torch.autograd.grad(pkg.balance_loss(x, ids)[0], x)[0])
+
+
 # ---------------------------------------------------------------------------------------------------- tensors that are not stored as they read
 
 def test_negated_views(path):

@@ -57,3 +57,23 @@ def test_instructions_of_a_whole_warp_stay_where_they_are_called():
     for f in sorted(csrc.glob("*.cu*")):
         for statement in re.findall(r"\basm\s*\([^;]*", f.read_text()):      # (up to the first semicolon: the instruction)
             assert not re.search(r"\b(redux|shfl|vote|match|bar|barrier|elect)\.", statement), f"{f.name}: {statement}"
+
+
+def test_a_capture_that_cannot_be_checked_is_refused(monkeypatch):
+    """Without the host extension nobody sees whether an eager graph of the same leaf is alive, beside which a captured backward pass ends the process."""
+    import contextlib
+    import sm120fp4_b200._lib as L
+    from sm120fp4_b200 import gate
+    monkeypatch.setattr(L, "_host", L.NO_HOST)
+    monkeypatch.setattr(torch.cuda, "device", lambda device: contextlib.nullcontext())
+    capturing = []
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: bool(capturing))
+    leaf = torch.zeros(4, 8, requires_grad=True)
+    gate._check_capture(leaf, "x")
+    capturing.append(1)
+    with pytest.raises(RuntimeError, match="without the host extension"):
+        gate._check_capture(leaf, "x")
+    gate._check_capture(leaf * 1.0, "x")
+    gate._check_capture(leaf.detach(), "x")
+    with torch.no_grad():
+        gate._check_capture(leaf, "x")
