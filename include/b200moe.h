@@ -276,7 +276,7 @@ int b200moe_gate(const void* logits, int dtype, long long stride, int tokens, in
 int b200moe_gate_backward(const float* grad_weights, const float* weights, const int* ids, const void* logits, int dtype, long long stride, int tokens, int E,
                           int k, int renormalize, void* grad_logits, void* stream);
 /* balance_loss: loss f32 [1] = E * sum_e (counts_e / sum counts) * (mean over live tokens of softmax(logits)_e), counts i32 [E] = pairs of each expert in
- * ids i32 [tokens, k], k <= 32. An id outside 0..E-1 is an empty slot; a token of empty slots alone is not live: it counts nowhere and its gradient is 0. No
+ * ids i32 [tokens, k], k <= 32 and tokens * k < 2^31. An id outside 0..E-1 is an empty slot; a token of empty slots alone is not live: it counts nowhere and its gradient is 0. No
  * live token: loss 0. stats f32 [2] is kept for the backward pass (1 / pairs, E / live tokens). The workspace holds nothing between calls. */
 long long b200moe_balance_workspace_bytes(int tokens, int E);
 int b200moe_balance_loss(const void* logits, int dtype, long long stride, int tokens, int E, const int* ids, int k, float* loss, int* counts, float* stats,

@@ -475,7 +475,7 @@ int b200moe_balance_loss(const void* logits, int dtype, long long stride, int to
                          void* workspace, long long workspace_bytes, void* stream) {
   using namespace b200;
   if (dtype < 0 || dtype > 2 || tokens < 0 || E < 1 || k < 1 || (stride < E && tokens > 1)) return B200MOE_ERR_ARG;
-  if (E > GATE_MAXE || k > 32 || tokens > (1 << 30)) return B200MOE_ERR_LIMIT;
+  if (E > GATE_MAXE || k > 32 || tokens > (1 << 30) || (long long)tokens * k > 0x7fffffff) return B200MOE_ERR_LIMIT;      // (counts of 32 bits)
   if (!loss || !counts || !stats || (tokens && (!logits || !ids || !workspace)) || ((uintptr_t)logits & (dtype == DT_F32 ? 3 : 1)) || ((uintptr_t)workspace & 3)) return B200MOE_ERR_ARG;
   if (workspace_bytes < b200moe_balance_workspace_bytes(tokens, E)) return B200MOE_ERR_WORKSPACE;
   int blocks = balance_blocks(tokens);
@@ -502,7 +502,7 @@ int b200moe_balance_backward(const float* grad_loss, const void* logits, int dty
                              const float* stats, void* grad_logits, void* stream) {
   using namespace b200;
   if (dtype < 0 || dtype > 2 || tokens < 0 || E < 1 || k < 1 || (stride < E && tokens > 1)) return B200MOE_ERR_ARG;
-  if (E > GATE_MAXE || k > 32 || tokens > (1 << 30)) return B200MOE_ERR_LIMIT;
+  if (E > GATE_MAXE || k > 32 || tokens > (1 << 30) || (long long)tokens * k > 0x7fffffff) return B200MOE_ERR_LIMIT;      // (counts of 32 bits)
   if (tokens == 0) return B200MOE_OK;
   if (!grad_loss || !logits || !ids || !counts || !stats || !grad_logits || (((uintptr_t)logits | (uintptr_t)grad_logits) & (dtype == DT_F32 ? 3 : 1))) return B200MOE_ERR_ARG;
   return with_type(dtype, [&](auto* tp) {

@@ -336,7 +336,8 @@ PyObject* py_balance_loss(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (n != 2 || !tensors(args, 2)) Py_RETURN_NONE;
   const at::Tensor x = THPVariable_Unpack(args[0]), ids = THPVariable_Unpack(args[1]);
-  if (!plain_logits(x) || !here(ids) || ids.dim() != 2 || ids.scalar_type() != at::kInt || !ids.is_contiguous() || ids.size(0) != x.size(0) || ids.size(1) < 1 || ids.size(1) > 32)
+  if (!plain_logits(x) || !here(ids) || ids.dim() != 2 || ids.scalar_type() != at::kInt || !ids.is_contiguous() || ids.size(0) != x.size(0) || ids.size(1) < 1 || ids.size(1) > 32 ||
+      ids.numel() > 0x7fffffff)
     Py_RETURN_NONE;
   at::Tensor loss, counts, stats;
   int rc = 0;

@@ -11,7 +11,7 @@ import torch
 
 from . import _lib
 
-MAX_EXPERTS, MAX_TOP_K = 512, 16
+MAX_EXPERTS, MAX_TOP_K, MAX_PAIRS = 512, 16, (1 << 31) - 1
 
 
 def _logits(logits: torch.Tensor, what: str) -> torch.Tensor:
@@ -130,10 +130,12 @@ def balance_loss(logits: torch.Tensor, ids: torch.Tensor):
     """logits [T, E], ids int32 [T, k] (the router's choice) -> (loss f32 [], counts int32 [E]):
     loss = E * sum_e f_e P_e with f_e expert e's share of all pairs and P_e the mean over tokens of softmax(logits)_e; it is 1 where experts are used
     evenly. counts are the pairs of each expert. An id outside 0..E-1 is an empty slot, and a token of empty slots alone (padding) counts nowhere; without any
-    live token the loss is 0. Differentiable with respect to the logits through P (f is a count). k up to 32, experts up to 512."""
+    live token the loss is 0. Differentiable with respect to the logits through P (f is a count). k up to 32, experts up to 512, pairs up to 2^31 - 1."""
     out = (_lib._host or _lib.host()).balance_loss(logits, ids)      # (as in top_k_gate)
     if out is not None:
         return out if type(out) is tuple else _lib.check(out, "balance_loss")
+    if ids.numel() > MAX_PAIRS:
+        raise ValueError(f"balance_loss takes at most {MAX_PAIRS} pairs (counts are of 32 bits), not {ids.numel()}")
     leaf, logits = logits, _logits(logits, "balance_loss")
     if ids.dtype != torch.int32:
         raise TypeError(f"balance_loss takes int32 ids, not {ids.dtype}")

@@ -77,3 +77,17 @@ def test_a_capture_that_cannot_be_checked_is_refused(monkeypatch):
     gate._check_capture(leaf.detach(), "x")
     with torch.no_grad():
         gate._check_capture(leaf, "x")
+
+
+def test_more_pairs_than_a_count_holds_are_refused():
+    """Counts are of 32 bits: 2^31 pairs of one expert would come out negative."""
+    import sm120fp4_b200._lib as L
+    tokens, h, p = 1 << 29, L.lib(), 4096      # (an address that is never read)
+    x, ids = torch.zeros(1, 8).expand(tokens, 8), torch.zeros(1, 4, dtype=torch.int32).expand(tokens, 4)
+    with pytest.raises(ValueError, match="pairs"):
+        pkg.balance_loss(x, ids)
+    with pytest.raises(RuntimeError, match="GPU"):
+        pkg.balance_loss(x[:-1], ids[:-1])
+    assert h.b200moe_balance_loss(p, 0, 8, tokens, 8, p, 4, p, p, p, p, 1 << 30, None) == L.ERR_LIMIT
+    assert h.b200moe_balance_backward(p, p, 0, 8, tokens, 8, p, 4, p, p, p, None) == L.ERR_LIMIT
+    assert h.b200moe_balance_loss(p, 0, 8, tokens - 1, 8, p, 4, p, p, p, p, 3, None) == L.ERR_WORKSPACE
