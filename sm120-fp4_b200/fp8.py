@@ -192,4 +192,6 @@ def matmul_fp8_status(device: torch.device | str | int | None = None) -> None:
     """Raises if a bounded wait inside a matmul_fp8 / matmul_fp8_experts call ran out on this device (default: the current one) since the last look: results are then
     incomplete. Synchronises the device's current stream."""
     device = torch.device("cuda" if device is None else device)
+    if device.type != "cuda":
+        raise ValueError(f"matmul_fp8_status looks at a GPU, not at {device}")
     _lib.call(torch.device("cuda", torch.cuda.current_device()) if device.index is None else device, "matmul_fp8_status", _lib.lib().b200moe_matmul_fp8_status)

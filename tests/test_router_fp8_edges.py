@@ -91,3 +91,10 @@ def test_more_pairs_than_a_count_holds_are_refused():
     assert h.b200moe_balance_loss(p, 0, 8, tokens, 8, p, 4, p, p, p, p, 1 << 30, None) == L.ERR_LIMIT
     assert h.b200moe_balance_backward(p, p, 0, 8, tokens, 8, p, 4, p, p, p, None) == L.ERR_LIMIT
     assert h.b200moe_balance_loss(p, 0, 8, tokens - 1, 8, p, 4, p, p, p, p, 3, None) == L.ERR_WORKSPACE
+
+
+def test_status_of_a_device_that_is_no_gpu_is_refused():
+    """It would have been that of the current GPU, and its flag cleared."""
+    for device in ("cpu", torch.device("meta")):
+        with pytest.raises(ValueError, match="GPU"):
+            pkg.matmul_fp8_status(device)
