@@ -307,6 +307,10 @@ int b200moe_matmul_fp8_experts(const void* a, long long a_stride, const float* a
                                const int* experts, const int* offsets, int runs, int N, int K, void* out, int out_dtype, long long out_stride, int zero_rest,
                                void* stream);
 int b200moe_matmul_fp8_status(void* stream);
+/* For tests: either product (experts and offsets null: one matrix, E 1) with waits that run out at once. give_up: 1 the copies', 2 the products', 4 the scales', 8 the
+ * sums' side, 16 of the first block of a pair alone; 0 is the ordinary call. Rows outside every run are left. The output is incomplete, status says so. */
+int b200moe_matmul_fp8_probe(const void* a, long long a_stride, const float* a_scales, int rows, const void* w, long long w_stride, const float* w_scales, int E,
+                             const int* experts, const int* offsets, int runs, int N, int K, void* out, int out_dtype, long long out_stride, int give_up, void* stream);
 
 #ifdef __cplusplus
 }

@@ -98,6 +98,7 @@ SIGNATURES = {
     "b200moe_matmul_fp8": (_I, [_P, _LL, _P, _P, _LL, _P, _I, _I, _I, _P, _I, _LL, _P]),
     "b200moe_matmul_fp8_experts": (_I, [_P, _LL, _P, _I, _P, _LL, _P, _I, _P, _P, _I, _I, _I, _P, _I, _LL, _I, _P]),
     "b200moe_matmul_fp8_status": (_I, [_P]),
+    "b200moe_matmul_fp8_probe": (_I, [_P, _LL, _P, _I, _P, _LL, _P, _I, _P, _P, _I, _I, _I, _P, _I, _LL, _I, _P]),
 }
 # exported only by a diagnostic build (include/b200moe_diag.h); bound when present
 DIAG_SIGNATURES = {

@@ -31,7 +31,13 @@ struct MatmulParams {
   const int *experts, *offsets;                   // null: one matrix, all rows
   int U, E, M, N, K, KB, NB, out_dtype, zero_rest, vec;
   long long ldo;
+  int give_up;                                    // 0; of the probe: whose waits run out at their first look
 };
+// Looks at a barrier until a role gives its wait up.
+enum { kRoleProducer = 1, kRoleMma = 2, kRoleScales = 4, kRoleEpilogue = 8, kRoleFirstOfPair = 16 };
+template <int kRole> __device__ __forceinline__ uint32_t looks_of(const MatmulParams& p, int rank) {
+  return p.give_up && (p.give_up & kRole) && !(p.give_up & kRoleFirstOfPair && rank) ? 0u : 1u << 20;
+}
 
 __device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate, uint32_t pred) {
   asm volatile(
@@ -113,6 +119,7 @@ __device__ __forceinline__ bool mbar_wait_lanes(uint32_t bar, uint32_t parity, b
   *abort_flag = 1;
   return false;
 }
+__device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
 __device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory"); }
 __device__ __forceinline__ void tmem_ld_32x32b_x32(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(
@@ -441,7 +448,7 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
       const MmTile tl = mm_tile<NT, kSwap, kPair>(p, first, off, kSwap && t < 0 ? 0 : t);
       if (rounds.shared(i)) cluster_arrive();
       for (int kb = kb0; kb < kb1 && !dead; ++kb) {
-        if (!mbar_wait_warp(smem_u32(&empty[st]), ph, abort_flag)) { dead = true; break; }
+        if (!mbar_wait_warp(smem_u32(&empty[st]), ph, abort_flag, looks_of<kRoleProducer>(p, rank))) { dead = true; break; }
         const uint32_t bar = smem_u32(&full[st]), sa = smem_u32(smem + st * S::kStageBytes);
         const int wrow = tl.expert * p.N + tl.n0;
         if constexpr (kPair) {      // each CTA brings its half of both operands; the bytes of both count at the leader's barrier
@@ -463,10 +470,12 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
     // would reach the barriers of the CTA that comes after it.
     if (!dead && !mbar_wait_lanes(smem_u32(&empty[lane < S::kStages ? lane : 0]), lane < st ? ph ^ 1 : ph, lane >= S::kStages, abort_flag)) dead = true;
     if (dead) {      // copies in flight land before the CTA may end (with a limit)
-      for (int i = issued > S::kStages ? issued - S::kStages : 0; i < issued; ++i)
-        for (int n = 0; n < 1 << 16 && (!kPair || rank == 0) && !mbar_try_wait(&full[i % S::kStages], (i / S::kStages) & 1); ++n) {}
-      if (kPair)
-        for (int n = 0; n < 200; ++n) __nanosleep(1000);      // (a pair's second CTA has no barrier of its own copies)
+      if constexpr (kPair) {      // (their barriers are the first CTA's, which count both CTAs' bytes, and the other may have stopped elsewhere: 200 us)
+        for (int n = 0; n < 200; ++n) __nanosleep(1000);
+      } else {
+        for (int i = issued > S::kStages ? issued - S::kStages : 0; i < issued; ++i)
+          for (int n = 0; n < 1 << 16 && !mbar_ready(smem_u32(&full[i % S::kStages]), (i / S::kStages) & 1); ++n) {}
+      }
     }
   } else if (warp == S::kEpi + 1) {                                  // ---- MMA issue
     const uint32_t el = elect_one();
@@ -482,14 +491,17 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
       }
       for (int kb = kb0, ready = 0; kb < kb1 && !dead && (!kPair || rank == 0); ++kb, --ready) {
         if constexpr (S::kAhead < 4) {      // the operands first: they are there long before the accumulator is free
-          if (!mbar_wait_warp(smem_u32(&full[st]), ph, abort_flag) || !mbar_wait_warp(smem_u32(&acc_empty[buf]), bph, abort_flag)) { dead = true; break; }
+          if (!mbar_wait_warp(smem_u32(&full[st]), ph, abort_flag, looks_of<kRoleMma>(p, rank)) || !mbar_wait_warp(smem_u32(&acc_empty[buf]), bph, abort_flag, looks_of<kRoleMma>(p, rank))) {
+            dead = true;
+            break;
+          }
         } else if (!ready) {      // lane 2j: the operands of the step after the next j, lane 2j + 1: its accumulator
           const int j = lane >> 1 < S::kAhead ? lane >> 1 : 0;
           int q = (lane & 1 ? buf : st) + j;
           const int wrap = lane & 1 ? S::kBufs : S::kStages;
           uint32_t par = lane & 1 ? bph : ph;
           if (q >= wrap) q -= wrap, par ^= 1;
-          ready = mbar_wait_steps<2>(smem_u32(lane & 1 ? &acc_empty[q] : &full[q]), par, min(S::kAhead, kb1 - kb), lane, abort_flag);
+          ready = mbar_wait_steps<2>(smem_u32(lane & 1 ? &acc_empty[q] : &full[q]), par, min(S::kAhead, kb1 - kb), lane, abort_flag, looks_of<kRoleMma>(p, rank));
           if (!ready) { dead = true; break; }
         }
         tc_fence_after();
@@ -511,11 +523,10 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
       }
       if (rounds.shared(i)) __syncwarp(), cluster_wait(), cluster_sync_all();
     }
-    if (dead) {
-      if constexpr (kPair) umma2_commit_p(&drained, 1, el & (rank == 0));
-      else umma_commit_u32(smem_u32(&drained), el);
-      for (int n = 0; n < 1 << 16 && (!kPair || rank == 0) && !mbar_try_wait(&drained, 0); ++n) {}
-    }
+    // Everything issued is done before the CTA may end, whoever else has given up (with a limit).
+    if constexpr (kPair) umma2_commit_p(&drained, 1, el & (rank == 0));
+    else umma_commit_u32(smem_u32(&drained), el);
+    for (int n = 0; n < 1 << 16 && (!kPair || rank == 0) && !mbar_ready(smem_u32(&drained), 0); ++n) {}
   } else if (warp == S::kEpi + 2) {                                  // ---- scales: four groups ahead in registers, then a slot beside each accumulator
     constexpr int kHere = kSwap ? NT : 128, R = (kHere + 31) / 32;
     int buf = 0, bph = 1;
@@ -557,7 +568,7 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
             int q = buf + (lane < S::kAhead ? lane : 0);
             uint32_t par = bph;
             if (q >= S::kBufs) q -= S::kBufs, par ^= 1;
-            ready = mbar_wait_steps<1>(smem_u32(&scale_empty[q]), par, min(min(S::kAhead, 4 - j), kb1 - kb - j), lane, abort_flag);
+            ready = mbar_wait_steps<1>(smem_u32(&scale_empty[q]), par, min(min(S::kAhead, 4 - j), kb1 - kb - j), lane, abort_flag, looks_of<kRoleScales>(p, rank));
             if (!ready) { dead = true; break; }
           }
           --ready;
@@ -593,12 +604,12 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
       const int rows = kSwap ? min(NT, tl.row_end - tl.row0) : NT;      // columns in use
       for (int kb = kb0, ready = 0; kb < kb1 && !dead; ++kb, --ready) {
         if constexpr (S::kAhead < 4) {
-          if (!mbar_ready(smem_u32(&acc_full[buf]), ph) && !mbar_wait_warp(smem_u32(&acc_full[buf]), ph, abort_flag)) { dead = true; break; }
+          if (!mbar_ready(smem_u32(&acc_full[buf]), ph) && !mbar_wait_warp(smem_u32(&acc_full[buf]), ph, abort_flag, looks_of<kRoleEpilogue>(p, rank))) { dead = true; break; }
         } else if (!ready) {
           int q = buf + (lane < S::kAhead ? lane : 0);
           uint32_t par = ph;
           if (q >= S::kBufs) q -= S::kBufs, par ^= 1;
-          ready = mbar_wait_steps<1>(smem_u32(&acc_full[q]), par, min(S::kAhead, kb1 - kb), lane, abort_flag);
+          ready = mbar_wait_steps<1>(smem_u32(&acc_full[q]), par, min(S::kAhead, kb1 - kb), lane, abort_flag, looks_of<kRoleEpilogue>(p, rank));
           if (!ready) { dead = true; break; }
         }
         tc_fence_after();
@@ -708,7 +719,10 @@ __global__ void __launch_bounds__(MmShape<NT, kSwap, kPair>::kThreads, 1)
       zero_rows(p, off[p.U], p.M, me, warps, lane);
     }
   }
-  if (dead) atomicExch(&g_matmul_fp8_status, 1);
+  if (dead) {
+    atomicExch(&g_matmul_fp8_status, 1);
+    if constexpr (kPair) st_cluster_u32(mapa_shared(smem_u32(&abort_s), rank ^ 1), 1u);      // the other CTA, which waits for this one, stops as well
+  }
   tc_fence_before();
   __syncthreads();
   if constexpr (kPair) {
@@ -857,7 +871,7 @@ int b200moe_matmul_fp8(const void* a, long long a_stride, const float* a_scales,
   using namespace b200;
   if (int rc = matmul_args(a, a_stride, a_scales, w, w_stride, w_scales, M, N, K, out, out_dtype, out_stride)) return rc;
   if (M == 0 || N == 0) return B200MOE_OK;
-  const MatmulParams p = {a_scales, w_scales, out, nullptr, nullptr, 0, 1, M, N, K, (K + 127) / 128, (N + 127) / 128, out_dtype, 0, stores_16(out, out_dtype, N, out_stride), out_stride};
+  const MatmulParams p = {a_scales, w_scales, out, nullptr, nullptr, 0, 1, M, N, K, (K + 127) / 128, (N + 127) / 128, out_dtype, 0, stores_16(out, out_dtype, N, out_stride), out_stride, 0};
   return matmul(p, a, a_stride, w, w_stride, (cudaStream_t)stream);
 }
 
@@ -875,7 +889,19 @@ int b200moe_matmul_fp8_experts(const void* a, long long a_stride, const float* a
   }
   if (!experts || !offsets) return B200MOE_ERR_ARG;
   const MatmulParams p = {a_scales, w_scales, out, experts, offsets, runs, E, rows, N, K, (K + 127) / 128, (N + 127) / 128, out_dtype, zero_rest,
-                          stores_16(out, out_dtype, N, out_stride), out_stride};
+                          stores_16(out, out_dtype, N, out_stride), out_stride, 0};
+  return matmul(p, a, a_stride, w, w_stride, (cudaStream_t)stream);
+}
+
+int b200moe_matmul_fp8_probe(const void* a, long long a_stride, const float* a_scales, int rows, const void* w, long long w_stride, const float* w_scales, int E,
+                             const int* experts, const int* offsets, int runs, int N, int K, void* out, int out_dtype, long long out_stride, int give_up, void* stream) {
+  using namespace b200;
+  if (E < 1 || runs < 0 || give_up < 0 || give_up > 31 || !experts != !offsets || (!experts && E != 1)) return B200MOE_ERR_ARG;
+  if (int rc = matmul_args(a, a_stride, a_scales, w, w_stride, w_scales, rows, N, K, out, out_dtype, out_stride)) return rc;
+  if (runs > MM_MAXU || (long long)E * N > (1ll << 31) - 512) return B200MOE_ERR_LIMIT;
+  if (rows == 0 || N == 0 || (experts && runs == 0)) return B200MOE_OK;
+  const MatmulParams p = {a_scales, w_scales, out, experts, offsets, runs, E, rows, N, K, (K + 127) / 128, (N + 127) / 128, out_dtype, 0, stores_16(out, out_dtype, N, out_stride),
+                          out_stride, give_up};
   return matmul(p, a, a_stride, w, w_stride, (cudaStream_t)stream);
 }
 

@@ -321,3 +321,44 @@ def test_a_row_that_is_asked_for_very_often_takes_the_time_of_its_bytes():
     often = best_us(lambda: pkg.quantize_fp8(x, src_row=skewed))
     one = best_us(lambda: pkg.quantize_fp8(x[:2], src_row=skewed.clamp(max=1)))
     assert often <= usual + 400 and one <= usual + 400, f"{usual:.0f} us evenly, {often:.0f} with one row for half of them, {one:.0f} with two rows in all"
+
+
+# ---------------------------------------------------------------------------------------------------- waits that run out
+
+FORMS = [(1, 1000, 512, 0), (1, 2048, 2048, 0), (40, 20000, 2048, 0), (100, 2048, 2048, 0), (16, 700, 1024, 8), (1000, 1408, 2816, 8), (512, 4096, 4096, 0), (6000, 1000, 1024, 8)]
+
+
+@pytest.mark.parametrize("m,n,k,experts,give_up", [(*f, g) for f in FORMS for g in (1, 2, 4, 8, 15)] + [(*FORMS[f], 16 + g) for f in (1, 6, 7) for g in (1, 2, 4, 8, 15)])
+def test_waits_that_run_out(m, n, k, experts, give_up):
+    """One side of a product's pipeline stops where it would first have to wait (the copies', the products', the scales', the sums', all; in all blocks, or in the first of a
+    cluster): the others stop after it, the call ends, its status says so once, and the next call is right. Few rows whole and split over clusters, tiles of 64 and 128 rows,
+    experts' runs of few rows and of many, pairs of blocks for one matrix and for several."""
+    import time
+    a, sa = pkg.quantize_fp8(randn(m, k, seed=1))
+    w, sw = pkg.quantize_fp8_weight(randn(max(experts, 1), n, k, seed=2))
+    out = torch.empty(m, n, dtype=torch.bfloat16, device="cuda")
+    tables = (torch.arange(experts, dtype=torch.int32, device="cuda"), (torch.arange(experts + 1, device="cuda") * (m // max(experts, 1))).int()) if experts else (None, None)
+
+    def call(side):
+        L.check(L.lib().b200moe_matmul_fp8_probe(a.data_ptr(), a.stride(0) if m > 1 else k, sa.data_ptr(), m, w.data_ptr(), w.stride(1), sw.data_ptr(), w.shape[0], L.ptr(tables[0]),
+                                                 L.ptr(tables[1]), experts, n, k, out.data_ptr(), 0, n, side, L.stream_ptr()), "probe")
+    pkg.matmul_fp8_status()
+    call(0)
+    pkg.matmul_fp8_status()
+    want = out.clone()
+    assert torch.equal(want, pkg.matmul_fp8_experts(a, sa, w, sw, *tables) if experts else pkg.matmul_fp8(a, sa, w[0], sw[0]))
+    torch.cuda.synchronize()
+    start = time.perf_counter()
+    call(give_up)
+    torch.cuda.synchronize()
+    assert time.perf_counter() - start < 5
+    try:
+        pkg.matmul_fp8_status()
+        assert give_up & 15 in (2, 4, 8) and torch.equal(out, want)      # (that side never had to wait; the copies' begins with a wait)
+    except L.B200MoEError as e:
+        assert e.code == L.ERR_TIMEOUT
+        pkg.matmul_fp8_status()
+    out.fill_(7)
+    call(0)
+    pkg.matmul_fp8_status()
+    assert torch.equal(out, want)
