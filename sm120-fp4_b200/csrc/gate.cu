@@ -10,6 +10,7 @@
 #include "common.cuh"
 #include "fp8_math.cuh"
 #include "tcgen05.cuh"
+#include <initializer_list>
 #include <type_traits>
 
 namespace b200 {
@@ -421,6 +422,11 @@ static int balance_blocks(int tokens) {      // 16 tokens or more each
 
 extern "C" {
 
+static bool words(std::initializer_list<const void*> at) {      // all on 4 bytes
+  uintptr_t bits = 0;
+  for (const void* p : at) bits |= (uintptr_t)p;
+  return (bits & 3) == 0;
+}
 static int gate_args(int dtype, long long stride, int tokens, int E, int k) {
   if (dtype < 0 || dtype > 2 || tokens < 0 || E < 1 || k < 1 || k > E || (stride < E && tokens > 1)) return B200MOE_ERR_ARG;
   if (E > b200::GATE_MAXE || k > b200::GATE_MAXK || tokens > (1 << 30)) return B200MOE_ERR_LIMIT;
@@ -431,7 +437,7 @@ int b200moe_gate(const void* logits, int dtype, long long stride, int tokens, in
   using namespace b200;
   if (int rc = gate_args(dtype, stride, tokens, E, k)) return rc;
   if (tokens == 0) return B200MOE_OK;
-  if (!logits || !weights || !ids || ((uintptr_t)logits & (dtype == DT_F32 ? 3 : 1))) return B200MOE_ERR_ARG;
+  if (!logits || !weights || !ids || !words({weights, ids}) || ((uintptr_t)logits & (dtype == DT_F32 ? 3 : 1))) return B200MOE_ERR_ARG;
   return with_type(dtype, [&](auto* tp) {
     using T = std::remove_pointer_t<decltype(tp)>;
     return with_values(E, [&](auto v) {
@@ -449,7 +455,7 @@ int b200moe_gate_backward(const float* grad_weights, const float* weights, const
   using namespace b200;
   if (int rc = gate_args(dtype, stride, tokens, E, k)) return rc;
   if (tokens == 0) return B200MOE_OK;
-  if (!grad_weights || !weights || !ids || !grad_logits || (!renormalize && !logits) || (((uintptr_t)logits | (uintptr_t)grad_logits) & (dtype == DT_F32 ? 3 : 1)))
+  if (!grad_weights || !weights || !ids || !grad_logits || (!renormalize && !logits) || !words({grad_weights, weights, ids}) || (((uintptr_t)logits | (uintptr_t)grad_logits) & (dtype == DT_F32 ? 3 : 1)))
     return B200MOE_ERR_ARG;
   return with_type(dtype, [&](auto* tp) {
     using T = std::remove_pointer_t<decltype(tp)>;
@@ -476,7 +482,8 @@ int b200moe_balance_loss(const void* logits, int dtype, long long stride, int to
   using namespace b200;
   if (dtype < 0 || dtype > 2 || tokens < 0 || E < 1 || k < 1 || (stride < E && tokens > 1)) return B200MOE_ERR_ARG;
   if (E > GATE_MAXE || k > 32 || tokens > (1 << 30) || (long long)tokens * k > 0x7fffffff) return B200MOE_ERR_LIMIT;      // (counts of 32 bits)
-  if (!loss || !counts || !stats || (tokens && (!logits || !ids || !workspace)) || ((uintptr_t)logits & (dtype == DT_F32 ? 3 : 1)) || ((uintptr_t)workspace & 3)) return B200MOE_ERR_ARG;
+  if (!loss || !counts || !stats || (tokens && (!logits || !ids || !workspace)) || ((uintptr_t)logits & (dtype == DT_F32 ? 3 : 1)) || !words({ids, loss, counts, stats, workspace}))
+    return B200MOE_ERR_ARG;
   if (workspace_bytes < b200moe_balance_workspace_bytes(tokens, E)) return B200MOE_ERR_WORKSPACE;
   int blocks = balance_blocks(tokens);
   float* part = (float*)workspace;
@@ -504,7 +511,7 @@ int b200moe_balance_backward(const float* grad_loss, const void* logits, int dty
   if (dtype < 0 || dtype > 2 || tokens < 0 || E < 1 || k < 1 || (stride < E && tokens > 1)) return B200MOE_ERR_ARG;
   if (E > GATE_MAXE || k > 32 || tokens > (1 << 30) || (long long)tokens * k > 0x7fffffff) return B200MOE_ERR_LIMIT;      // (counts of 32 bits)
   if (tokens == 0) return B200MOE_OK;
-  if (!grad_loss || !logits || !ids || !counts || !stats || !grad_logits || (((uintptr_t)logits | (uintptr_t)grad_logits) & (dtype == DT_F32 ? 3 : 1))) return B200MOE_ERR_ARG;
+  if (!grad_loss || !logits || !ids || !counts || !stats || !grad_logits || !words({grad_loss, ids, counts, stats}) || (((uintptr_t)logits | (uintptr_t)grad_logits) & (dtype == DT_F32 ? 3 : 1))) return B200MOE_ERR_ARG;
   return with_type(dtype, [&](auto* tp) {
     using T = std::remove_pointer_t<decltype(tp)>;
     return with_values(E, [&](auto v) {

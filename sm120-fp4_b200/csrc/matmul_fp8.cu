@@ -887,7 +887,7 @@ int b200moe_matmul_fp8_experts(const void* a, long long a_stride, const float* a
     if (zero_rest) B200_CUDA_TRY(cudaMemset2DAsync(out, out_stride * size, 0, N * size, rows, (cudaStream_t)stream));
     return B200MOE_OK;
   }
-  if (!experts || !offsets) return B200MOE_ERR_ARG;
+  if (!experts || !offsets || (((uintptr_t)experts | (uintptr_t)offsets) & 3)) return B200MOE_ERR_ARG;
   const MatmulParams p = {a_scales, w_scales, out, experts, offsets, runs, E, rows, N, K, (K + 127) / 128, (N + 127) / 128, out_dtype, zero_rest,
                           stores_16(out, out_dtype, N, out_stride), out_stride, 0};
   return matmul(p, a, a_stride, w, w_stride, (cudaStream_t)stream);
@@ -896,7 +896,7 @@ int b200moe_matmul_fp8_experts(const void* a, long long a_stride, const float* a
 int b200moe_matmul_fp8_probe(const void* a, long long a_stride, const float* a_scales, int rows, const void* w, long long w_stride, const float* w_scales, int E,
                              const int* experts, const int* offsets, int runs, int N, int K, void* out, int out_dtype, long long out_stride, int give_up, void* stream) {
   using namespace b200;
-  if (E < 1 || runs < 0 || give_up < 0 || give_up > 31 || !experts != !offsets || (!experts && E != 1)) return B200MOE_ERR_ARG;
+  if (E < 1 || runs < 0 || give_up < 0 || give_up > 31 || !experts != !offsets || (!experts && E != 1) || (((uintptr_t)experts | (uintptr_t)offsets) & 3)) return B200MOE_ERR_ARG;
   if (int rc = matmul_args(a, a_stride, a_scales, w, w_stride, w_scales, rows, N, K, out, out_dtype, out_stride)) return rc;
   if (runs > MM_MAXU || (long long)E * N > (1ll << 31) - 512) return B200MOE_ERR_LIMIT;
   if (rows == 0 || N == 0 || (experts && runs == 0)) return B200MOE_OK;

@@ -342,7 +342,7 @@ int b200moe_quantize_fp8(const void* x, int dtype, long long x_stride, int x_row
   if (!src_row && rows != x_rows) return B200MOE_ERR_ARG;
   if ((!x && x_rows) || !codes || !scales) return B200MOE_ERR_ARG;
   const int size = dtype == DT_F32 ? 4 : 2;
-  if (((uintptr_t)x & (size - 1)) || (((uintptr_t)scales | (uintptr_t)workspace) & 3)) return B200MOE_ERR_ARG;
+  if (((uintptr_t)x & (size - 1)) || (((uintptr_t)scales | (uintptr_t)workspace | (uintptr_t)src_row) & 3)) return B200MOE_ERR_ARG;
   const long long need = src_row ? b200moe_quantize_fp8_workspace_bytes(x_rows, rows, K) : 0;
   if (need && (!workspace || workspace_bytes < need)) return B200MOE_ERR_WORKSPACE;
   cudaStream_t st = (cudaStream_t)stream;

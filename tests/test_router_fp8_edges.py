@@ -98,3 +98,21 @@ def test_status_of_a_device_that_is_no_gpu_is_refused():
     for device in ("cpu", torch.device("meta")):
         with pytest.raises(ValueError, match="GPU"):
             pkg.matmul_fp8_status(device)
+
+
+def test_tables_and_sums_off_4_bytes_are_refused():
+    """Every pointer to words, one at a time; the kernels would fault on it. (Addresses are never read: a call that is not refused cannot run here.)"""
+    import sm120fp4_b200._lib as L
+    if torch.cuda.is_available():
+        pytest.skip("calls with addresses that are none, refused or not")
+    h, p = L.lib(), 4096
+    calls = [(h.b200moe_gate, [p, 0, 8, 4, 8, 2, 1, p, p, None], [7, 8]), (h.b200moe_gate_backward, [p, p, p, p, 0, 8, 4, 8, 2, 0, p, None], [0, 1, 2]),
+             (h.b200moe_balance_loss, [p, 0, 8, 4, 8, p, 2, p, p, p, p, 1 << 20, None], [5, 7, 8, 9, 10]), (h.b200moe_balance_backward, [p, p, 0, 8, 4, 8, p, 2, p, p, p, None], [0, 6, 8, 9]),
+             (h.b200moe_quantize_fp8, [p, 0, 16, 4, p, 4, 16, p, 16, p, None, 0, None], [4, 9]), (h.b200moe_quantize_fp8_blocks, [p, 0, 1, 4, 16, p, 16, p, None], [7]),
+             (h.b200moe_matmul_fp8, [p, 16, p, p, 16, p, 4, 4, 16, p, 0, 4, None], [2, 5]),
+             (h.b200moe_matmul_fp8_experts, [p, 16, p, 4, p, 16, p, 2, p, p, 1, 4, 16, p, 0, 4, 0, None], [2, 6, 8, 9]),
+             (h.b200moe_matmul_fp8_probe, [p, 16, p, 4, p, 16, p, 2, p, p, 1, 4, 16, p, 0, 4, 0, None], [2, 6, 8, 9])]
+    for call, args, words in calls:
+        assert call(*args) in (L.ERR_CUDA, L.ERR_DEVICE)      # as it stands it gets as far as the device that is not here
+        for i in words:
+            assert call(*args[:i], p + 2, *args[i + 1:]) == L.ERR_ARG, f"{call.__name__}, argument {i}"
