@@ -173,6 +173,16 @@ at::Tensor stored(const at::Tensor& grad) {
   return t.resolve_neg().contiguous();
 }
 
+// A saved tensor as the forward pass saw it. Hooks on saved tensors may give back another one, whose memory would be read as if it were the first.
+at::Tensor unpacked(const torch::autograd::SavedVariable& saved, at::IntArrayRef size, at::ScalarType type, const at::Tensor& grad, const char* what,
+                    std::shared_ptr<torch::autograd::Node> made_by = nullptr) {
+  const at::Tensor t = saved.unpack(std::move(made_by));
+  TORCH_CHECK(t.layout() == at::kStrided && t.device() == grad.device() && t.scalar_type() == type && t.sizes() == size,
+              std::string(what) + " backward: a hook gave back a saved tensor of another size, type or device");
+  if (plain_tensor(t) && (t.is_contiguous() || (t.dim() == 2 && t.stride(1) == 1 && t.stride(0) >= t.size(1)))) return t;
+  return stored(t);
+}
+
 // A leaf's gradient is handed over on the stream on which its accumulator was made. Where an eager graph keeps that alive, a backward pass that is being captured
 // on another stream would have the engine wait across the two, which ends the process: refused while it still can be.
 void check_capture(const at::Tensor& x, const char* what) {
@@ -200,7 +210,7 @@ int run_gate(const at::Tensor& x, int64_t k, bool renormalize, at::Tensor& weigh
 }
 struct GateBackward : torch::autograd::Node {
   SavedVariable weights, ids, x;      // (normalised weights do not depend on the experts left out: no x)
-  int64_t e = 0;
+  int64_t tokens = 0, e = 0, k = 0;
   at::ScalarType dtype = at::kFloat;
   bool renormalize = true;
   std::string name() const override { return "TopKGateBackward"; }
@@ -211,7 +221,9 @@ struct GateBackward : torch::autograd::Node {
   variable_list apply(variable_list&& grads) override {
     std::lock_guard<std::mutex> lock(mutex_);
     if (!grads[0].defined() || !task_should_compute_output(0)) return {at::Tensor()};
-    const at::Tensor w = weights.unpack(shared_from_this()), i = ids.unpack(), l = renormalize ? at::Tensor() : x.unpack(), grad = stored(grads[0]);
+    const at::Tensor grad = stored(grads[0]), w = unpacked(weights, {tokens, k}, at::kFloat, grad, "top_k_gate", shared_from_this()).contiguous(),
+                     i = unpacked(ids, {tokens, k}, at::kInt, grad, "top_k_gate").contiguous(),
+                     l = renormalize ? at::Tensor() : unpacked(x, {tokens, e}, dtype, grad, "top_k_gate");
     const at::Tensor out = fresh({w.size(0), e}, dtype, w);
     checked(ops.gate_backward(grad.data_ptr(), w.data_ptr(), i.data_ptr(), l.defined() ? l.data_ptr() : nullptr, dtype_code(dtype), l.defined() ? row_stride(l) : e, (int)w.size(0),
                               (int)e, (int)w.size(1), renormalize, out.data_ptr(), raw_stream()),
@@ -222,7 +234,7 @@ struct GateBackward : torch::autograd::Node {
 int gate_with_grad(const at::Tensor& x, int64_t k, bool renormalize, at::Tensor& weights, at::Tensor& ids) {
   const auto node = node_of<GateBackward>(x);
   if (const int rc = run_gate(x, k, renormalize, weights, ids)) return rc;
-  node->e = x.size(1), node->dtype = x.scalar_type(), node->renormalize = renormalize;
+  node->tokens = x.size(0), node->e = x.size(1), node->k = k, node->dtype = x.scalar_type(), node->renormalize = renormalize;
   torch::autograd::set_history(weights, node);
   node->weights = SavedVariable(weights, true), node->ids = SavedVariable(ids, false);
   if (!renormalize) node->x = SavedVariable(x, false);
@@ -240,6 +252,8 @@ int run_balance(const at::Tensor& x, const at::Tensor& ids, at::Tensor& loss, at
 }
 struct BalanceBackward : torch::autograd::Node {
   SavedVariable x, ids, counts, stats;
+  int64_t tokens = 0, e = 0, k = 0;
+  at::ScalarType dtype = at::kFloat;
   std::string name() const override { return "BalanceLossBackward"; }
   void release_variables() override {
     std::lock_guard<std::mutex> lock(mutex_);
@@ -248,7 +262,8 @@ struct BalanceBackward : torch::autograd::Node {
   variable_list apply(variable_list&& grads) override {
     std::lock_guard<std::mutex> lock(mutex_);
     if (!grads[0].defined() || !task_should_compute_output(0)) return {at::Tensor()};
-    const at::Tensor l = x.unpack(), i = ids.unpack(), c = counts.unpack(), s = stats.unpack(), grad = stored(grads[0]);
+    const at::Tensor grad = stored(grads[0]), l = unpacked(x, {tokens, e}, dtype, grad, "balance_loss"), i = unpacked(ids, {tokens, k}, at::kInt, grad, "balance_loss").contiguous(),
+                     c = unpacked(counts, {e}, at::kInt, grad, "balance_loss"), s = unpacked(stats, {2}, at::kFloat, grad, "balance_loss");
     const at::Tensor out = fresh({l.size(0), l.size(1)}, l.scalar_type(), l);
     checked(ops.balance_backward(grad.data_ptr(), l.data_ptr(), dtype_code(l.scalar_type()), row_stride(l), (int)l.size(0), (int)l.size(1), i.data_ptr(), (int)i.size(1), c.data_ptr(),
                                  s.data_ptr(), out.data_ptr(), raw_stream()),
@@ -259,6 +274,7 @@ struct BalanceBackward : torch::autograd::Node {
 int balance_with_grad(const at::Tensor& x, const at::Tensor& ids, at::Tensor& loss, at::Tensor& counts, at::Tensor& stats) {
   const auto node = node_of<BalanceBackward>(x);
   if (const int rc = run_balance(x, ids, loss, counts, stats)) return rc;
+  node->tokens = x.size(0), node->e = x.size(1), node->k = ids.size(1), node->dtype = x.scalar_type();
   torch::autograd::set_history(loss, node);
   node->x = SavedVariable(x, false), node->ids = SavedVariable(ids, false), node->counts = SavedVariable(counts, false), node->stats = SavedVariable(stats, false);
   return 0;

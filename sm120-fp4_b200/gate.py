@@ -56,20 +56,30 @@ def _once(out: torch.Tensor, what: str) -> torch.Tensor:
     return torch._C._functions.DelayedError(f"{what} is differentiable once".encode(), 1)(out.detach().requires_grad_(True))
 
 
+def _unpacked(t: torch.Tensor, shape: tuple, dtype: torch.dtype, grad: torch.Tensor, what: str) -> torch.Tensor:
+    """A saved tensor as the forward pass saw it. Hooks on saved tensors may give back another one, whose memory would be read as if it were the first."""
+    if t.layout != torch.strided or t.device != grad.device or t.dtype != dtype or tuple(t.shape) != shape:
+        raise RuntimeError(f"{what} backward: a hook gave back a saved tensor of another size, type or device")
+    t = _lib.stored(t.detach())
+    return t if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.contiguous()
+
+
 class _Gate(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, top_k, renormalize):
         weights, ids = _gate(logits, top_k, renormalize)
         ctx.mark_non_differentiable(ids)
         ctx.save_for_backward(weights, ids, None if renormalize else logits)      # (normalised weights do not depend on the experts left out)
-        ctx.like, ctx.renormalize = (logits.dtype, logits.shape[1]), renormalize
+        ctx.like, ctx.renormalize = (logits.dtype, *logits.shape, top_k), renormalize
         return weights, ids
 
     @staticmethod
     def backward(ctx, grad, _):
         weights, ids, logits = ctx.saved_tensors
-        dtype, e = ctx.like
-        tokens, k = weights.shape
+        dtype, tokens, e, k = ctx.like
+        weights, ids = (_unpacked(t, (tokens, k), of, grad, "top_k_gate").contiguous() for t, of in ((weights, torch.float32), (ids, torch.int32)))
+        if logits is not None:
+            logits = _unpacked(logits, (tokens, e), dtype, grad, "top_k_gate")
         out = torch.empty((tokens, e), dtype=dtype, device=weights.device)
         grad = _lib.stored(grad.detach()).contiguous()
         _lib.call(out.device, "top_k_gate backward", _lib.lib().b200moe_gate_backward, grad.data_ptr(), weights.data_ptr(), ids.data_ptr(), _lib.ptr(logits),
@@ -113,13 +123,15 @@ class _Balance(torch.autograd.Function):
         loss, counts, stats = _balance(logits, ids)
         ctx.mark_non_differentiable(counts)
         ctx.save_for_backward(logits, ids, counts, stats)
+        ctx.like = (logits.dtype, *logits.shape, ids.shape[1])
         return loss, counts
 
     @staticmethod
     def backward(ctx, grad, _):
-        logits, ids, counts, stats = ctx.saved_tensors
-        tokens, e = logits.shape
-        out = torch.empty((tokens, e), dtype=logits.dtype, device=logits.device)
+        dtype, tokens, e, k = ctx.like
+        logits, ids, counts, stats = (_unpacked(t, shape, of, grad, "balance_loss") for t, shape, of in zip(
+            ctx.saved_tensors, ((tokens, e), (tokens, k), (e,), (2,)), (dtype, torch.int32, torch.int32, torch.float32)))
+        ids, out = ids.contiguous(), torch.empty((tokens, e), dtype=dtype, device=logits.device)
         grad = _lib.stored(grad.detach()).contiguous()
         _lib.call(out.device, "balance_loss backward", _lib.lib().b200moe_balance_backward, grad.data_ptr(), logits.data_ptr(), _lib.DTYPES[logits.dtype],
                   max(logits.stride(0), e), tokens, e, ids.data_ptr(), ids.shape[1], counts.data_ptr(), stats.data_ptr(), out.data_ptr())

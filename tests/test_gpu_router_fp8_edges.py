@@ -68,6 +68,39 @@ def test_fp8_calls_refuse_inputs_that_ask_for_a_derivative(path):
         assert same(pkg.quantize_fp8(ask(x))[0], a)
 
 
+def test_saved_tensors_that_come_back_as_others(path):
+    """Hooks on saved tensors may move and copy them: what comes back is looked at before its memory is read."""
+    hooks = torch.autograd.graph.saved_tensors_hooks
+    big = randn(12, 80, seed=3)
+
+    def grads(pack, unpack, renormalize):
+        x = big[:, 5:69].detach().clone().requires_grad_(True)
+        with hooks(pack, unpack):
+            w, ids = pkg.top_k_gate(x, 3, renormalize)
+            loss = pkg.balance_loss(x, ids)[0]
+        return torch.autograd.grad(w.square().sum(), x)[0], torch.autograd.grad(loss, x)[0]
+    spread = lambda t: torch.stack([t, t], t.dim())[..., 0]      # the same values, apart in memory
+    for renormalize in (True, False):
+        want = grads(lambda t: t, lambda t: t, renormalize)
+        for pack, unpack in ((lambda t: t.cpu(), lambda t: t.cuda()), (lambda t: t.clone(), spread), (lambda t: t.detach().clone(), lambda t: t.t().contiguous().t() if t.dim() == 2 else t),
+                             (lambda t: -t if t.is_floating_point() else t.clone(), lambda t: torch._neg_view(t) if t.is_floating_point() else t)):
+            for a, b in zip(grads(pack, unpack, renormalize), want):
+                assert torch.equal(a, b)
+        bad = [lambda t: t.cpu(), lambda t: t.double() if t.is_floating_point() else t.long(), lambda t: t[:1], lambda t: t[None], lambda t: t.bfloat16() if t.is_floating_point() else t.short()]
+        for unpack in bad:
+            x = big.clone().requires_grad_(True)
+            with hooks(lambda t: t, unpack):
+                w, ids = pkg.top_k_gate(x, 3, renormalize)
+                loss = pkg.balance_loss(x, ids)[0]
+            for out in (w.square().sum(), loss):
+                with pytest.raises(RuntimeError, match="gave back"):
+                    torch.autograd.grad(out, x)
+    with torch.autograd.graph.save_on_cpu(pin_memory=True):
+        x = big.clone().requires_grad_(True)
+        pkg.top_k_gate(x, 3, False)[0].sum().backward()
+    assert bool(torch.isfinite(x.grad).all())
+
+
 def test_an_error_in_a_gradient_reaches_the_caller():
     """The library says no inside a backward pass, on a thread of the autograd engine: an exception like any other."""
     h, host, no = L.lib(), L.host(), C.CFUNCTYPE(C.c_int, *L.SIGNATURES["b200moe_gate_backward"][1])(lambda *args: L.ERR_ARG)
