@@ -116,3 +116,35 @@ def test_tables_and_sums_off_4_bytes_are_refused():
         assert call(*args) in (L.ERR_CUDA, L.ERR_DEVICE)      # as it stands it gets as far as the device that is not here
         for i in words:
             assert call(*args[:i], p + 2, *args[i + 1:]) == L.ERR_ARG, f"{call.__name__}, argument {i}"
+
+
+def test_route_runs_on_the_gpu_that_its_tables_are_on(monkeypatch):
+    """Tables on the host reached the kernels, those of another GPU the current one's stream."""
+    import contextlib
+    from types import SimpleNamespace
+    import sm120fp4_b200._lib as L
+    from sm120fp4_b200 import router
+    ids, tables = torch.zeros(4, 2, dtype=torch.int32), [torch.zeros(n, dtype=torch.int32) for n in (8, 9, 8)]
+    with pytest.raises(RuntimeError, match="GPU"):
+        pkg.route(ids, 8, *tables)
+    with pytest.raises(RuntimeError, match="GPU"):
+        pkg.route_tables(ids, 8)
+    here, seen = [0], []
+
+    @contextlib.contextmanager
+    def guard(device):
+        before, here[0] = here[0], device.index
+        yield
+        here[0] = before
+    monkeypatch.setattr(torch.cuda, "device", guard)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: here[0], raising=False)
+    monkeypatch.setattr(L, "stream_ptr", lambda: 100 + here[0])
+    monkeypatch.setattr(router, "_workspace", lambda device, stream, n: torch.zeros(n, dtype=torch.uint8))
+    monkeypatch.setattr(L, "lib", lambda: SimpleNamespace(b200moe_route_workspace_bytes=lambda p, e: 64, b200moe_route=lambda *args: seen.append((here[0], args[1:4], args[-1])) or 0))
+    for index in (0, 3):
+        monkeypatch.setattr(torch.Tensor, "device", property(lambda self: torch.device("cuda", index)))
+        monkeypatch.setattr(torch.Tensor, "is_cuda", property(lambda self: True))
+        pkg.route(ids, 8, *tables)
+    assert seen == [(0, (8, 8, 8), 100), (3, (8, 8, 8), 103)] and here == [0]
+    with pytest.raises(ValueError, match="contiguous"):
+        pkg.route(ids, 8, torch.zeros(16, dtype=torch.int32)[::2], *tables[1:])
