@@ -26,7 +26,7 @@ extern "C" {
 
 typedef struct b200moe_layer b200moe_layer; /* opaque decode-layer handle (host memory) */
 
-int b200moe_version(void);   /* 102: router from logits, balance loss, FP8 quantisers and products */
+int b200moe_version(void);   /* 102: router from logits, balance loss, FP8 quantisers and products; 103: route leaves -1 in pairs behind the last run */
 const char* b200moe_error_string(int code);
 const char* b200moe_last_cuda_error(void);
 

@@ -71,7 +71,7 @@ struct b200moe_layer {
 
 static inline long long align_up(long long v, long long a) { return (v + a - 1) / a * a; }
 
-extern "C" int b200moe_version(void) { return 102; }
+extern "C" int b200moe_version(void) { return 103; }
 
 extern "C" const char* b200moe_error_string(int code) {
   switch (code) {

@@ -3,8 +3,8 @@
 //            dl = w_j (g_j - sum g w) at id_j (normalised), or p_e (g_e - sum g w) for all experts
 //   balance  L = E sum_e f_e P_e, f_e = n_e / sum n, P_e = mean over live tokens of softmax(l)_e
 //            dl = g E / T' p_e (f_e - sum_j p_j f_j)
-// Measured on the GPU: gate of 16384 x 128 fp32 9.6 us and its gradient 5.7 (issue of about 300 instructions a token, 69 % of the slots), of one token 1.8; balance loss of
-// 65536 x 256 bf16 14.7 us + 2, its gradient 20 (about 150 and 190 instructions a token; the bytes are 5 and 10 us). Cold caches, but for the one token.
+// Measured on the GPU: gate of 16384 x 128 fp32 9.6 us (333 instructions a token, 69 % of the issue slots) and its gradient 5.7 (83, 31 %: latency), of one token 1.8; balance loss
+// of 65536 x 256 bf16 14.7 us + 2, its gradient 20 (145 and 186 instructions a token, 70 and 64 % of the slots; the bytes are 5 and 10 us). Cold caches, but for the one token.
 // A warp per token with its logits in registers; sums in fp32, statistics by shuffles, no atomic decides a value. A logit of -inf is an
 // expert that may not be taken: a slot for which none is left gets id -1 (an empty slot of the layer) and weight 0.
 #include "common.cuh"
@@ -151,7 +151,7 @@ template <int V, bool kPacked> struct Candidates {
   }
 };
 
-// Bound by issue (eight of 128 experts in 32 bits: about 300 instructions a token; with a scan of all candidates in every round 11.2 us instead of 9.4 at 16384 tokens).
+// Bound by issue (eight of 128 experts in 32 bits: 333 instructions a token; with a scan of all candidates in every round 11.2 us instead of 9.4 at 16384 tokens).
 template <typename T, int V, bool kVec>
 __global__ void __launch_bounds__(256) k_gate(const T* __restrict__ logits, long long stride, int tokens, int E, int k, int renorm, float* __restrict__ weights,
                                               int* __restrict__ ids) {
