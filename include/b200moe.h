@@ -64,7 +64,8 @@ int b200moe_quantize_own_scale_probe(const void* x, int dtype, int groups, int r
 /* ---- router: sm120fp4/kernels/moe_w4a16.py:85-91 (route; padded form of k_route :48-83) and the torch router of
  * sm120fp4/kernels/fc1_w4a16.py:272-279. ids i32 [P] -> experts i32 [Umax] (ascending, -1 padding), offsets i32
  * [Umax+1] (exclusive scan, P padding), pairs i32 [P] (pair indices grouped by expert, ascending within). An id below 0 is an empty slot: its pair is in
- * no run, the padding of offsets is then where the last run ends, and what is behind that in pairs is -1 (which b200moe_quantize_fp8 takes as an empty row). */
+ * no run, the padding of offsets is then where the last run ends, and what is behind that in pairs is -1 (b200moe_quantize_fp8 takes rows below 0 as empty ones: pairs
+ * become rows by a division that rounds down). */
 long long b200moe_route_workspace_bytes(int P, int E);
 int b200moe_route(const int* ids, int P, int E, int Umax, int* experts, int* offsets, int* pairs, void* workspace,
                   long long workspace_bytes, void* stream);

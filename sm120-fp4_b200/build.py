@@ -51,7 +51,10 @@ HOST_BUILT_BY = PKG / "build" / "host.command"
 def one_cxx_library(cxx: str) -> list[str]:
     """The extension takes the C++ library that torch has loaded. A compiler that knows it as an archive only would put a second one into the extension, and the two share
     some of their objects and not others: writing a number to a stream ends the process."""
-    r = subprocess.run([cxx, "-print-file-name=libstdc++.so"], stdout=subprocess.PIPE, text=True)
+    try:
+        r = subprocess.run([cxx, "-print-file-name=libstdc++.so"], stdout=subprocess.PIPE, text=True)
+    except OSError:      # (no such compiler, which the build itself says)
+        return []
     return ["-nostdlib++"] if r.stdout.strip() == "libstdc++.so" else []      # (the bare name: there is no such file)
 
 
