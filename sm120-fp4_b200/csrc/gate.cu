@@ -2,9 +2,9 @@
 //   gate     ids = the k largest logits of a token (ties: the lowest index), w_j = softmax(l)[id_j], divided by their sum if asked
 //            dl = w_j (g_j - sum g w) at id_j (normalised), or p_e (g_e - sum g w) for all experts
 //   balance  L = E sum_e f_e P_e, f_e = n_e / sum n, P_e = mean over live tokens of softmax(l)_e
-//            dl = g E / T' p_e (f_e - sum_j p_j f_j)
+//            dl = g E / T' p_e (f_e - sum_j p_j f_j), with f_e - 1 / E for f_e
 // Measured on the GPU: gate of 16384 x 128 fp32 9.6 us (333 instructions a token, 69 % of the issue slots) and its gradient 5.7 (83, 31 %: latency), of one token 1.8; balance loss
-// of 65536 x 256 bf16 14.7 us + 2, its gradient 20 (145 and 186 instructions a token, 70 and 64 % of the slots; the bytes are 5 and 10 us). Cold caches, but for the one token.
+// of 65536 x 256 bf16 14.7 us + 2, its gradient 20 (145 and 195 instructions a token, 70 and 66 % of the slots; the bytes are 5 and 10 us). Cold caches, but for the one token.
 // A warp per token with its logits in registers; sums in fp32, statistics by shuffles, no atomic decides a value. A logit of -inf is an
 // expert that may not be taken: a slot for which none is left gets id -1 (an empty slot of the layer) and weight 0.
 #include "common.cuh"
@@ -371,10 +371,17 @@ __global__ void __launch_bounds__(256, V <= 8 ? 8 : 4) k_balance_backward(const 
                                                           T* __restrict__ out) {
   const int lane = threadIdx.x & 31;
   grid_dependency_wait();
-  const float inv = stats[0], c = *grad * stats[1];
+  // p_e (f_e - sum p f) is the same with f_e - 1 / E in the place of f_e, which is what is left of it where experts are used evenly, and a quotient of whole numbers:
+  // (E (n_e - q) - r) / (E sum n) with sum n = q E + r. Taken from the shares themselves, the difference would drown in their roundings there.
+  const float c = *grad * stats[1], inv = stats[0] / (float)E;
+  int n[V], pairs = 0;
+#pragma unroll
+  for (int j = 0; j < V; ++j) n[j] = lane * V + j < E ? counts[lane * V + j] : 0, pairs += n[j];
+  const unsigned sum = __reduce_add_sync(0xffffffffu, (unsigned)pairs), q = sum / (unsigned)E;      // (below 2^31)
+  const float r = (float)(sum - q * (unsigned)E);
   float f[V];
 #pragma unroll
-  for (int j = 0; j < V; ++j) f[j] = lane * V + j < E ? (float)counts[lane * V + j] * inv : 0.f;
+  for (int j = 0; j < V; ++j) f[j] = lane * V + j < E ? fmaf((float)(n[j] - (int)q), (float)E, -r) * inv : 0.f;
   for (int t = blockIdx.x * 8 + (threadIdx.x >> 5); t < tokens; t += gridDim.x * 8) {
     const int e = lane < k ? ids[(long long)t * k + lane] : -1;
     float x[V];

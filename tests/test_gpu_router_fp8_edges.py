@@ -139,6 +139,34 @@ def test_capture_beside_a_live_graph_is_refused_on_either_path(path):
         assert torch.equal(g, torch.autograd.grad(pkg.balance_loss(x, ids)[0], x)[0])
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("t,e,k", [(64, 8, 8), (4096, 64, 4), (4096, 60, 1), (2048, 512, 8), (6, 1, 1)])
+def test_balance_gradient_where_experts_are_used_almost_evenly(t, e, k, dtype):
+    """With f_e = 1/E + d_e the gradient is g E/T p_e (d_e - sum p d): it is 0 where all d are, and its roundings count against d, not against f. Per term: d is a quotient of
+    whole numbers (5 roundings: two of the numerator, 1/sum n, that over E, the product), p as in a softmax (a numerator 2.25 |x - m| + 4 roundings, twice, a sum of V + 5 and a quotient), the sum over
+    E of V + 5 additions more, and six products and differences. |x - m| <= 8 here."""
+    values = next(v for v in (1, 2, 4, 8, 16) if e <= 32 * v)
+    x = (torch.rand(t, e, generator=torch.Generator().manual_seed(e)) * 8 - 4).to(dtype).cuda()
+    ids = (torch.arange(t * k) % e).int().view(t, k).cuda()
+    for moved in (0, 1, 3):
+        if e == 1 and moved:
+            continue
+        ids.view(-1)[:moved] = e - 1
+        counts = torch.bincount(ids.view(-1).long(), minlength=e)
+        d = (counts.double() * e - t * k) / (t * k * e)
+        leaf = x.clone().requires_grad_(True)
+        loss, got_counts = pkg.balance_loss(leaf, ids)
+        assert torch.equal(got_counts, counts.int())
+        g, = torch.autograd.grad(loss, leaf)
+        p = torch.softmax(x.double(), 1)
+        want, size = e / t * p * (d - (p @ d)[:, None]), e / t * p * (d.abs() + (p @ d.abs())[:, None])
+        rel_p = 2 * (2.25 * 8 + 4) + values + 6
+        tol = 2.0 ** -24 * (5 + 2 * rel_p + values + 5 + 6) * size + torch.finfo(dtype).eps / 2 * want.abs() + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps + 2.0 ** -126
+        assert bool(((g.double() - want).abs() <= tol).all())
+        if int(counts.min()) == int(counts.max()):
+            assert float(g.abs().max()) == 0.0
+
+
 # ---------------------------------------------------------------------------------------------------- tensors that are not stored as they read
 
 def test_negated_views(path):
